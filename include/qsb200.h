@@ -168,6 +168,94 @@ int qs_tensor_error(int ggml_type, const void* blocks, int64_t blocks_row_bytes,
 int qs_tensor_error_noalloc(int ggml_type, const void* blocks, int64_t blocks_row_bytes, const void* x,
                             int x_type, int64_t n_rows, int64_t k, const float* qw, double* out, void* stream);
 
+/* ---- operators on packed blocks ------------------------------------------------------
+ * What a user of packed weights computes next: a layer's norm into 8-bit activations, the
+ * choice of experts, and products of packed weights with those activations. No counterpart in
+ * the reference, which stops at the packed file.
+ */
+
+/*
+ * RMS norm of n_rows rows of k values, with the residual's addition, into Q8_0 blocks:
+ *   t = x + residual, rounded to x_type and written to `total` (t = x without a residual)
+ *   y = t * weight / sqrt(mean(t^2) + eps); per 32 values d = f16(max |y| / 127) and levels
+ *   round(127 |y| / max |y|) with y's sign, halves away from zero, as in exact arithmetic.
+ *   x, residual, total   x_type (F32 / F16 / BF16), row strides in elements, rows 16-byte
+ *                        aligned; residual and total are both given or both NULL; total may be
+ *                        x or residual themselves, but not overlap them in another way
+ *   weight               k finite float32, 16-byte aligned
+ *   eps                  positive
+ *   k                    a multiple of 32
+ *   dst                  row r at dst + r * dst_row_bytes, any alignment
+ * A row that holds inf or NaN gets NaN scales and zero levels.
+ */
+int qs_rms_norm_q8(const void* x, int x_type, int64_t x_row_stride, const void* residual, int64_t residual_row_stride,
+                   void* total, int64_t total_row_stride, const float* weight, double eps, int64_t n_rows, int64_t k,
+                   void* dst, int64_t dst_row_bytes, void* stream);
+
+#define QS_MAX_EXPERTS 1024
+#define QS_SCORE_SOFTMAX 0
+#define QS_SCORE_SIGMOID 1
+#define QS_GROUP_MAX 0   /* a group counts as its best expert */
+#define QS_GROUP_TOP2 1  /* ... as the sum of its two best */
+
+/*
+ * The experts of every token: top_k of n_experts by score + bias, best first, ties to the lowest
+ * expert, compared in 64 bits.
+ *   score          softmax or sigmoid of the row's logits (F32 / F16 / BF16, row stride in elements)
+ *   bias           n_experts float32 or NULL; for the choice alone, not in the weights
+ *   n_groups       equal runs of experts (<= 64); only the groups_kept best are chosen from
+ *   ids, weights   n_rows x top_k; weight = score (over the sum of the chosen scores if
+ *                  renormalize) * scale; 0 where that sum is 0
+ * An expert whose logit or score + bias is -inf or NaN is never chosen; where too few are
+ * left the id is -1 and the weight 0. top_k <= 32.
+ */
+int qs_route(const void* logits, int logits_type, int64_t logits_row_stride, int64_t n_rows, int n_experts, int top_k,
+             int score, const float* bias, int n_groups, int groups_kept, int group_score, int renormalize, float scale,
+             int32_t* ids, float* weights, void* stream);
+
+/*
+ * The slots (entries of ids, in order) grouped by expert: order (n_slots) lists the slots of
+ * expert 0, then 1, ..., each in rising order, and last those without an expert (ids outside
+ * [0, n_experts)); offsets (n_experts + 1) holds where each expert's start, and where the last begin.
+ * n_slots <= 2^20.
+ */
+int qs_expert_plan(const int32_t* ids, int64_t n_slots, int n_experts, int32_t* order, int32_t* offsets, void* stream);
+
+/*
+ * out[r, j] = sum_c W[j, c] X[r, c]: packed weights of any type above (n rows of k values), X
+ * n_rows rows of Q8_0 blocks (qs_rms_norm_q8, or qs_quantize with QS_TYPE_Q8_0). The levels
+ * are multiplied as exact integers; scales and sums are float32, rounded once to out_type.
+ *   w                     weight row j at w + j * w_row_bytes; w and w_row_bytes multiples of 16
+ *                         bytes for Q4_K and Q5_K, 8 for Q5_1 and IQ4_XS, 4 for Q4_1 and Q2_K, else 2
+ *   x                     row r at x + r * x_row_bytes, any alignment
+ *   out                   F32 / F16 / BF16, row stride in elements; overlaps no input
+ *   workspace             16-byte aligned, of at least qs_matmul_workspace bytes (may be NULL if
+ *                         that is 0); its contents do not matter before or after. Calls that may
+ *                         run at the same time need a workspace each.
+ * n_rows <= 2^20 and n_rows * n <= 2^38.
+ */
+int qs_matmul(int ggml_type, const void* w, int64_t w_row_bytes, int64_t n, int64_t k, const void* x, int64_t x_row_bytes,
+              int64_t n_rows, void* out, int out_type, int64_t out_row_stride, void* workspace, int64_t workspace_bytes,
+              void* stream);
+int qs_matmul_workspace(int ggml_type, int64_t n, int64_t k, int64_t n_rows, int64_t* bytes);
+
+/*
+ * The same product with one weight matrix per expert: slot s = t * top_k + j of token t uses
+ * matrix ids[s] at w + ids[s] * w_expert_bytes, and activation row t, or s where x_per_slot.
+ *   ids, order, offsets   n_tokens x top_k choices and their qs_expert_plan
+ *   weights               NULL: out has a row per slot, zeros where the slot has no expert.
+ *                         Else n_tokens x top_k float32: out has a row per token, the sum over its
+ *                         slots with an expert of weight * product, in slot order.
+ * n_tokens * top_k <= 2^20. Strides, alignment and workspace as qs_matmul; sum: weights given.
+ */
+int qs_matmul_experts(int ggml_type, const void* w, int64_t w_row_bytes, int64_t w_expert_bytes, int n_experts, int64_t n,
+                      int64_t k, const void* x, int64_t x_row_bytes, int x_per_slot, const int32_t* ids,
+                      const int32_t* order, const int32_t* offsets, int64_t n_tokens, int top_k, const float* weights,
+                      void* out, int out_type, int64_t out_row_stride, void* workspace, int64_t workspace_bytes,
+                      void* stream);
+int qs_matmul_experts_workspace(int ggml_type, int n_experts, int64_t n, int64_t k, int64_t n_tokens, int top_k,
+                                int x_per_slot, int sum, int64_t* bytes);
+
 /*
  * Fault word of `device`: bit 0 is set when a quantize kernel gave up waiting for one of its
  * own bulk copies (every wait in the kernels is bounded; on that path the kernel records

@@ -7,6 +7,7 @@
 
 #include "../../include/qsb200.h"
 #include "qs_kernels.h"
+#include "qs_matmul.cuh"
 
 namespace {
 
@@ -414,6 +415,336 @@ QS_API int qs_tensor_error_noalloc(int ggml_type, const void* blocks, int64_t bl
         return fail(QS_EINVAL, "launch needs %d partial sums; the static scratch holds %d", need, QS_NOALLOC_MAX_PARTIALS);
     e = qs::launch_tensor_error_noalloc(ggml_type, c, out, ctx, *d);
     return e == cudaSuccess ? QS_OK : cuda_fail(e, "tensor error launch (static scratch)");
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// operators on packed blocks: norm into Q8_0, routing, products
+// ---------------------------------------------------------------------------
+namespace {
+
+bool is_src(int t) { return t == QS_SRC_F32 || t == QS_SRC_F16 || t == QS_SRC_BF16; }
+int src_size(int t) { return t == QS_SRC_F32 ? 4 : 2; }
+bool aligned(const void* p, int a) { return ((uintptr_t)p & (uintptr_t)(a - 1)) == 0; }
+
+// Alignment that the product kernels load blocks of a type with: the largest power of two (up
+// to 16) that divides the block size and the places of its level bytes.
+int block_align(int type) {
+    switch (type) {
+    case qs::QS_Q4_K: case qs::QS_Q5_K: return 16;
+    case qs::QS_Q5_1: case qs::QS_IQ4_XS: return 8;
+    case qs::QS_Q4_1: case qs::QS_Q2_K: return 4;
+    default: return 2;
+    }
+}
+
+bool has_min(int type) {
+    return type == qs::QS_Q4_1 || type == qs::QS_Q5_1 || type == qs::QS_Q2_K || type == qs::QS_Q4_K || type == qs::QS_Q5_K;
+}
+
+// How a product runs: which kernel, its tile, how often the row is split, and the workspace.
+struct MmPlan {
+    bool few;
+    int bn, splits, units, units_pad, planes;
+    int64_t xq_off, xd_off, part_off, bytes;
+    bool part;
+};
+
+// slots: output rows before a weighted sum; groups: weight matrices that share them; x_rows:
+// activation rows. SMs: the tile kernel keeps two CTAs on each of a B200's 148.
+MmPlan mm_plan(int type, int64_t n, int64_t k, int64_t slots, int64_t groups, int64_t x_rows, bool sum) {
+    MmPlan p;
+    memset(&p, 0, sizeof(p));
+    p.units = (int)(k / 32);
+    p.units_pad = (p.units + 3) / 4 * 4;
+    p.planes = 1 + (has_min(type) ? (type == qs::QS_Q2_K ? 2 : 1) : 0);
+    p.splits = 1;
+    const int64_t avg = (slots + groups - 1) / groups;
+    p.few = groups == 1 ? slots <= 8 : avg <= 4;
+    if (!p.few) {
+        p.bn = avg <= 32 ? 32 : avg <= 64 ? 64 : 128;
+        const int64_t chunks = groups == 1 ? (slots + p.bn - 1) / p.bn : slots / p.bn + (groups < slots ? groups : slots) / 2 + 1;
+        const int64_t tiles = (n + 127) / 128 * chunks, steps = p.units_pad / 4;
+        if (tiles < 2 * 148) {
+            int64_t s = (2 * 148 + tiles - 1) / tiles;
+            if (s > steps / 4) s = steps / 4;  // 4 steps at least: shorter ones cost more to join than they gain
+            if (s > 1) {
+                const int64_t per = (steps + s - 1) / s;
+                p.splits = (int)((steps + per - 1) / per);
+            }
+        }
+    }
+    p.part = sum || p.splits > 1;
+    int64_t at = 0;
+    auto take = [&](int64_t b) { const int64_t o = at; at += (b + 255) / 256 * 256; return o; };
+    if (!p.few) {
+        p.xq_off = take(x_rows * p.units_pad * 32);
+        p.xd_off = take(x_rows * p.units_pad * 4 * p.planes);
+    }
+    if (p.part) p.part_off = take((int64_t)p.splits * slots * n * 4);
+    p.bytes = at;
+    return p;
+}
+
+// Checks of sizes shared by the products and their workspace queries.
+int check_mm(int ggml_type, int64_t n, int64_t k, int64_t rows, int64_t per_token, const TypeInfo** out) {
+    const TypeInfo* ti = find_type(ggml_type);
+    if (!ti) return fail(QS_ENOTSUP, "ggml type %d is not supported", ggml_type);
+    if (k <= 0 || k % ti->qk) return fail(QS_EINVAL, "row length %lld is not a positive multiple of %d", (long long)k, ti->qk);
+    if (k > (int64_t)1 << 30) return fail(QS_EINVAL, "row length %lld is over 2^30", (long long)k);
+    if (n <= 0 || n > (int64_t)1 << 30) return fail(QS_EINVAL, "weight row count %lld is not in 1 .. 2^30", (long long)n);
+    if (rows < 0) return fail(QS_EINVAL, "negative row count");
+    // 65535 chunks of 32 slots, and the joining kernel's threads
+    if (rows > (1 << 20) / per_token || rows * per_token * n > (int64_t)1 << 38)
+        return fail(QS_EINVAL, "%lld rows of %lld outputs are too many for one call", (long long)(rows * per_token), (long long)n);
+    *out = ti;
+    return QS_OK;
+}
+
+int check_mm_operands(const TypeInfo* ti, const void* w, int64_t w_row_bytes, int64_t k, const void* x, int64_t x_row_bytes, const void* out,
+                      int out_type, int64_t out_row_stride, int64_t n) {
+    const int64_t row_bytes = k / ti->qk * ti->bytes;
+    if (!w || !x || !out) return fail(QS_EINVAL, "null weights, activations or out");
+    if (!is_src(out_type)) return fail(QS_EINVAL, "output type %d is not F32/F16/BF16", out_type);
+    if (w_row_bytes < row_bytes) return fail(QS_EINVAL, "weight row stride %lld < packed row size %lld", (long long)w_row_bytes, (long long)row_bytes);
+    if (x_row_bytes < k / 32 * 34) return fail(QS_EINVAL, "activation row stride %lld < Q8_0 row size %lld", (long long)x_row_bytes, (long long)(k / 32 * 34));
+    if (out_row_stride < n) return fail(QS_EINVAL, "out_row_stride %lld < %lld", (long long)out_row_stride, (long long)n);
+    const int al = block_align(ti->type);
+    if (!aligned(w, al) || w_row_bytes % al) return fail(QS_EINVAL, "weights and their row stride must be multiples of %d bytes for ggml type %d", al, ti->type);
+    if (!aligned(out, src_size(out_type))) return fail(QS_EINVAL, "out is not aligned to its elements");
+    return QS_OK;
+}
+
+// Fill the kernel call from the plan and run it.
+int run_mm(int ggml_type, const MmPlan& p, qs::MmArgs& a, int64_t x_rows, int per_out, const float* weights, const int* ids, void* workspace,
+           const qs::LaunchCtx& ctx) {
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    a.units = p.units;
+    a.units_pad = p.units_pad;
+    a.splits = p.splits;
+    a.part = p.part ? reinterpret_cast<float*>(ws + p.part_off) : nullptr;
+    a.x_plane = x_rows * p.units_pad;
+    cudaError_t e;
+    if (p.few) {
+        e = qs::launch_mm_few(ggml_type, a, ctx);
+    } else {
+        int8_t* xq = reinterpret_cast<int8_t*>(ws + p.xq_off);
+        float* xd = reinterpret_cast<float*>(ws + p.xd_off);
+        a.xq = xq;
+        a.xd = xd;
+        e = qs::launch_mm_pack(a, (int)x_rows, xq, xd, p.planes, ctx);
+        if (e == cudaSuccess) e = qs::launch_mm_tile(ggml_type, a, p.bn, ctx);
+    }
+    if (e == cudaSuccess && p.part) e = qs::launch_mm_finish(a, per_out, weights, ids, ctx);
+    return e == cudaSuccess ? QS_OK : cuda_fail(e, "matmul launch");
+}
+
+int check_workspace(const void* workspace, int64_t bytes, int64_t need) {
+    if (bytes < need) return fail(QS_EINVAL, "workspace of %lld bytes, %lld are needed", (long long)bytes, (long long)need);
+    if (need > 0 && !workspace) return fail(QS_EINVAL, "null workspace");
+    if (need > 0 && !aligned(workspace, 16)) return fail(QS_EINVAL, "workspace must be 16-byte aligned");
+    return QS_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+QS_API int qs_rms_norm_q8(const void* x, int x_type, int64_t x_row_stride, const void* residual, int64_t residual_row_stride, void* total,
+                          int64_t total_row_stride, const float* weight, double eps, int64_t n_rows, int64_t k, void* dst,
+                          int64_t dst_row_bytes, void* stream) {
+    if (!is_src(x_type)) return fail(QS_EINVAL, "source type %d is not F32/F16/BF16", x_type);
+    if (k <= 0 || k % 32 || k > (int64_t)1 << 30) return fail(QS_EINVAL, "row length %lld is not a positive multiple of 32 (up to 2^30)", (long long)k);
+    if (n_rows < 0 || n_rows > INT32_MAX) return fail(QS_EINVAL, "row count %lld is not in 0 .. 2^31 - 1", (long long)n_rows);
+    if (!(eps > 0.0) || !(eps < 1e300)) return fail(QS_EINVAL, "eps must be positive and finite");
+    if (!residual != !total) return fail(QS_EINVAL, "residual and total go together");
+    if (dst_row_bytes < k / 32 * 34) return fail(QS_EINVAL, "dst_row_bytes %lld < Q8_0 row size %lld", (long long)dst_row_bytes, (long long)(k / 32 * 34));
+    if (x_row_stride < k || (residual && (residual_row_stride < k || total_row_stride < k))) return fail(QS_EINVAL, "a row stride is below the row length");
+    if (n_rows == 0) return QS_OK;
+    if (!x || !weight || !dst) return fail(QS_EINVAL, "null x, weight or dst");
+    const int el = 16 / src_size(x_type);
+    if (!aligned(x, 16) || x_row_stride % el || !aligned(weight, 16) ||
+        (residual && (!aligned(residual, 16) || !aligned(total, 16) || residual_row_stride % el || total_row_stride % el)))
+        return fail(QS_EINVAL, "rows of x, residual and total, and weight, must start on 16-byte boundaries");
+    CurrentContextGuard keep;
+    int device, rc;
+    DeviceState* d;
+    if ((rc = device_of(x, "x", &device, &d))) return rc;
+    if ((rc = check_on_device(weight, device, "weight")) || (rc = check_on_device(dst, device, "dst")) ||
+        (residual && ((rc = check_on_device(residual, device, "residual")) || (rc = check_on_device(total, device, "total")))))
+        return rc;
+    qs::NormCall c;
+    c.x = x;
+    c.x_type = x_type;
+    c.residual = residual;
+    c.total = total;
+    c.weight = weight;
+    c.eps = eps;
+    c.n_rows = n_rows;
+    c.k = k;
+    c.x_stride = x_row_stride;
+    c.residual_stride = residual_row_stride;
+    c.total_stride = total_row_stride;
+    c.dst = dst;
+    c.dst_row_bytes = dst_row_bytes;
+    cudaError_t e = qs::launch_rms_norm_q8(c, qs::LaunchCtx{static_cast<cudaStream_t>(stream), device, d->num_sms});
+    return e == cudaSuccess ? QS_OK : cuda_fail(e, "rms norm launch");
+}
+
+QS_API int qs_route(const void* logits, int logits_type, int64_t logits_row_stride, int64_t n_rows, int n_experts, int top_k, int score,
+                    const float* bias, int n_groups, int groups_kept, int group_score, int renormalize, float scale, int32_t* ids,
+                    float* weights, void* stream) {
+    if (!is_src(logits_type)) return fail(QS_EINVAL, "logits type %d is not F32/F16/BF16", logits_type);
+    if (n_experts < 1 || n_experts > QS_MAX_EXPERTS) return fail(QS_EINVAL, "%d experts are not in 1 .. %d", n_experts, QS_MAX_EXPERTS);
+    if (score != QS_SCORE_SOFTMAX && score != QS_SCORE_SIGMOID) return fail(QS_EINVAL, "score %d is neither softmax nor sigmoid", score);
+    if (group_score != QS_GROUP_MAX && group_score != QS_GROUP_TOP2) return fail(QS_EINVAL, "group score %d is neither max nor top2", group_score);
+    if (n_groups < 1 || n_groups > 64 || n_experts % n_groups) return fail(QS_EINVAL, "%d groups do not divide %d experts (at most 64)", n_groups, n_experts);
+    if (groups_kept < 1 || groups_kept > n_groups) return fail(QS_EINVAL, "%d of %d groups can not be kept", groups_kept, n_groups);
+    const int usable = n_experts / n_groups * groups_kept;
+    if (top_k < 1 || top_k > 32 || top_k > usable) return fail(QS_EINVAL, "top_k %d is not in 1 .. %d", top_k, usable < 32 ? usable : 32);
+    if (n_rows < 0 || n_rows > INT32_MAX) return fail(QS_EINVAL, "row count %lld is not in 0 .. 2^31 - 1", (long long)n_rows);
+    if (logits_row_stride < n_experts) return fail(QS_EINVAL, "logits row stride %lld < %d experts", (long long)logits_row_stride, n_experts);
+    if (n_rows == 0) return QS_OK;
+    if (!logits || !ids || !weights) return fail(QS_EINVAL, "null logits, ids or weights");
+    if (!aligned(logits, src_size(logits_type)) || !aligned(ids, 4) || !aligned(weights, 4) || (bias && !aligned(bias, 4)))
+        return fail(QS_EINVAL, "a pointer is not aligned to its elements");
+    CurrentContextGuard keep;
+    int device, rc;
+    DeviceState* d;
+    if ((rc = device_of(logits, "logits", &device, &d))) return rc;
+    if ((rc = check_on_device(ids, device, "ids")) || (rc = check_on_device(weights, device, "weights")) ||
+        (bias && (rc = check_on_device(bias, device, "bias"))))
+        return rc;
+    qs::RouteCall c;
+    c.logits = logits;
+    c.logits_type = logits_type;
+    c.logits_stride = logits_row_stride;
+    c.n_rows = n_rows;
+    c.n_experts = n_experts;
+    c.top_k = top_k;
+    c.n_groups = n_groups;
+    c.groups_kept = groups_kept;
+    c.sigmoid = score == QS_SCORE_SIGMOID;
+    c.group_top2 = group_score == QS_GROUP_TOP2;
+    c.renormalize = renormalize != 0;
+    c.bias = bias;
+    c.scale = scale;
+    c.ids = ids;
+    c.weights = weights;
+    cudaError_t e = qs::launch_route(c, qs::LaunchCtx{static_cast<cudaStream_t>(stream), device, d->num_sms});
+    return e == cudaSuccess ? QS_OK : cuda_fail(e, "route launch");
+}
+
+QS_API int qs_expert_plan(const int32_t* ids, int64_t n_slots, int n_experts, int32_t* order, int32_t* offsets, void* stream) {
+    if (n_experts < 1 || n_experts > QS_MAX_EXPERTS) return fail(QS_EINVAL, "%d experts are not in 1 .. %d", n_experts, QS_MAX_EXPERTS);
+    if (n_slots < 0 || n_slots > 1 << 20) return fail(QS_EINVAL, "slot count %lld is not in 0 .. 2^20", (long long)n_slots);
+    if (!offsets || (n_slots > 0 && (!ids || !order))) return fail(QS_EINVAL, "null ids, order or offsets");
+    if (!aligned(ids, 4) || !aligned(order, 4) || !aligned(offsets, 4)) return fail(QS_EINVAL, "a pointer is not aligned to its elements");
+    CurrentContextGuard keep;
+    int device, rc;
+    DeviceState* d;
+    if ((rc = device_of(offsets, "offsets", &device, &d))) return rc;
+    if (n_slots > 0 && ((rc = check_on_device(ids, device, "ids")) || (rc = check_on_device(order, device, "order")))) return rc;
+    cudaError_t e = qs::launch_expert_plan(ids, (int)n_slots, n_experts, order, offsets, qs::LaunchCtx{static_cast<cudaStream_t>(stream), device, d->num_sms});
+    return e == cudaSuccess ? QS_OK : cuda_fail(e, "expert plan launch");
+}
+
+QS_API int qs_matmul_workspace(int ggml_type, int64_t n, int64_t k, int64_t n_rows, int64_t* bytes) {
+    const TypeInfo* ti;
+    if (int rc = check_mm(ggml_type, n, k, n_rows, 1, &ti)) return rc;
+    if (bytes) *bytes = n_rows ? mm_plan(ggml_type, n, k, n_rows, 1, n_rows, false).bytes : 0;
+    return QS_OK;
+}
+
+QS_API int qs_matmul(int ggml_type, const void* w, int64_t w_row_bytes, int64_t n, int64_t k, const void* x, int64_t x_row_bytes, int64_t n_rows,
+                     void* out, int out_type, int64_t out_row_stride, void* workspace, int64_t workspace_bytes, void* stream) {
+    const TypeInfo* ti;
+    int rc = check_mm(ggml_type, n, k, n_rows, 1, &ti);
+    if (rc) return rc;
+    if (n_rows == 0) return QS_OK;
+    if ((rc = check_mm_operands(ti, w, w_row_bytes, k, x, x_row_bytes, out, out_type, out_row_stride, n))) return rc;
+    const MmPlan p = mm_plan(ggml_type, n, k, n_rows, 1, n_rows, false);
+    if ((rc = check_workspace(workspace, workspace_bytes, p.bytes))) return rc;
+    CurrentContextGuard keep;
+    int device;
+    DeviceState* d;
+    if ((rc = device_of(w, "w", &device, &d))) return rc;
+    if ((rc = check_on_device(x, device, "x")) || (rc = check_on_device(out, device, "out")) ||
+        (p.bytes && (rc = check_on_device(workspace, device, "workspace"))))
+        return rc;
+    qs::MmArgs a;
+    memset(&a, 0, sizeof(a));
+    a.w = static_cast<const uint8_t*>(w);
+    a.w_row = w_row_bytes;
+    a.x = static_cast<const uint8_t*>(x);
+    a.x_row = x_row_bytes;
+    a.x_div = 1;
+    a.n = (int)n;
+    a.slots = (int)n_rows;
+    a.out = out;
+    a.out_stride = out_row_stride;
+    a.out_type = out_type;
+    a.kgrid = qs::iq_kgrid(d->iq, ggml_type);
+    return run_mm(ggml_type, p, a, n_rows, 1, nullptr, nullptr, workspace, qs::LaunchCtx{static_cast<cudaStream_t>(stream), device, d->num_sms});
+}
+
+QS_API int qs_matmul_experts_workspace(int ggml_type, int n_experts, int64_t n, int64_t k, int64_t n_tokens, int top_k, int x_per_slot, int sum,
+                                       int64_t* bytes) {
+    const TypeInfo* ti;
+    if (n_experts < 1 || n_experts > QS_MAX_EXPERTS) return fail(QS_EINVAL, "%d experts are not in 1 .. %d", n_experts, QS_MAX_EXPERTS);
+    if (top_k < 1 || top_k > QS_MAX_EXPERTS) return fail(QS_EINVAL, "%d experts per token are not in 1 .. %d", top_k, QS_MAX_EXPERTS);
+    if (int rc = check_mm(ggml_type, n, k, n_tokens, top_k, &ti)) return rc;
+    if (bytes) *bytes = n_tokens ? mm_plan(ggml_type, n, k, n_tokens * top_k, n_experts, x_per_slot ? n_tokens * top_k : n_tokens, sum != 0).bytes : 0;
+    return QS_OK;
+}
+
+QS_API int qs_matmul_experts(int ggml_type, const void* w, int64_t w_row_bytes, int64_t w_expert_bytes, int n_experts, int64_t n, int64_t k,
+                             const void* x, int64_t x_row_bytes, int x_per_slot, const int32_t* ids, const int32_t* order,
+                             const int32_t* offsets, int64_t n_tokens, int top_k, const float* weights, void* out, int out_type,
+                             int64_t out_row_stride, void* workspace, int64_t workspace_bytes, void* stream) {
+    const TypeInfo* ti;
+    int rc;
+    if (n_experts < 1 || n_experts > QS_MAX_EXPERTS) return fail(QS_EINVAL, "%d experts are not in 1 .. %d", n_experts, QS_MAX_EXPERTS);
+    if (top_k < 1 || top_k > QS_MAX_EXPERTS) return fail(QS_EINVAL, "%d experts per token are not in 1 .. %d", top_k, QS_MAX_EXPERTS);
+    if ((rc = check_mm(ggml_type, n, k, n_tokens, top_k, &ti))) return rc;
+    if (n_tokens == 0) return QS_OK;
+    if ((rc = check_mm_operands(ti, w, w_row_bytes, k, x, x_row_bytes, out, out_type, out_row_stride, n))) return rc;
+    if (w_expert_bytes < n * w_row_bytes || w_expert_bytes % block_align(ggml_type))
+        return fail(QS_EINVAL, "expert stride %lld must be a multiple of %d and at least %lld", (long long)w_expert_bytes, block_align(ggml_type), (long long)(n * w_row_bytes));
+    if (!ids || !order || !offsets) return fail(QS_EINVAL, "null ids, order or offsets");
+    if (!aligned(ids, 4) || !aligned(order, 4) || !aligned(offsets, 4) || (weights && !aligned(weights, 4)))
+        return fail(QS_EINVAL, "a pointer is not aligned to its elements");
+    const int64_t slots = n_tokens * top_k, x_rows = x_per_slot ? slots : n_tokens;
+    const MmPlan p = mm_plan(ggml_type, n, k, slots, n_experts, x_rows, weights != nullptr);
+    if ((rc = check_workspace(workspace, workspace_bytes, p.bytes))) return rc;
+    CurrentContextGuard keep;
+    int device;
+    DeviceState* d;
+    if ((rc = device_of(w, "w", &device, &d))) return rc;
+    if ((rc = check_on_device(x, device, "x")) || (rc = check_on_device(out, device, "out")) || (rc = check_on_device(ids, device, "ids")) ||
+        (rc = check_on_device(order, device, "order")) || (rc = check_on_device(offsets, device, "offsets")) ||
+        (weights && (rc = check_on_device(weights, device, "weights"))) || (p.bytes && (rc = check_on_device(workspace, device, "workspace"))))
+        return rc;
+    qs::MmArgs a;
+    memset(&a, 0, sizeof(a));
+    a.w = static_cast<const uint8_t*>(w);
+    a.w_row = w_row_bytes;
+    a.w_exp = w_expert_bytes;
+    a.x = static_cast<const uint8_t*>(x);
+    a.x_row = x_row_bytes;
+    a.x_div = x_per_slot ? 1 : top_k;
+    a.n = (int)n;
+    a.slots = (int)slots;
+    a.order = order;
+    a.offsets = offsets;
+    a.n_exp = n_experts;
+    a.out = out;
+    a.out_stride = out_row_stride;
+    a.out_type = out_type;
+    a.kgrid = qs::iq_kgrid(d->iq, ggml_type);
+    return run_mm(ggml_type, p, a, x_rows, weights ? top_k : 1, weights, weights ? ids : nullptr, workspace,
+                  qs::LaunchCtx{static_cast<cudaStream_t>(stream), device, d->num_sms});
 }
 
 }  // extern "C"

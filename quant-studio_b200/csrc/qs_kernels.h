@@ -84,4 +84,35 @@ cudaError_t noalloc_setup(int device, const NoAllocDevice** out);
 cudaError_t launch_tensor_error_noalloc(int type, const DqCall& c, double* out, const LaunchCtx& ctx,
                                         const NoAllocDevice& d);
 
+// RMS norm with the residual's addition into Q8_0 blocks (qs_norm.cu).
+struct NormCall {
+    const void* x;
+    int x_type;
+    const void* residual;  // or null
+    void* total;           // x + residual in x_type; null without a residual
+    const float* weight;
+    double eps;
+    int64_t n_rows, k;
+    int64_t x_stride, residual_stride, total_stride;  // elements
+    void* dst;
+    int64_t dst_row_bytes;
+};
+cudaError_t launch_rms_norm_q8(const NormCall& c, const LaunchCtx& ctx);
+
+// Routing to experts (qs_route.cu).
+struct RouteCall {
+    const void* logits;
+    int logits_type;
+    int64_t logits_stride;  // elements
+    int64_t n_rows;
+    int n_experts, top_k, n_groups, groups_kept;
+    int sigmoid, group_top2, renormalize;
+    const float* bias;  // or null
+    float scale;
+    int* ids;
+    float* weights;
+};
+cudaError_t launch_route(const RouteCall& c, const LaunchCtx& ctx);
+cudaError_t launch_expert_plan(const int* ids, int n, int n_experts, int* order, int* offsets, const LaunchCtx& ctx);
+
 }  // namespace qs

@@ -1,0 +1,292 @@
+// RMS norm of rows, with the residual's addition, into Q8_0 blocks (sm_100a).
+//
+//   t = x + residual (float32 sum rounded to the rows' type; t = x without a residual)
+//   r = 1 / sqrt(mean(t^2) + eps),  p = t * weight
+//   per 32 values: m = max |p|, levels sign(p) floor(127 |p| / m + 1/2), scale f16(m r / 127)
+//
+// The levels do not depend on r, and |p| / m is compared with the borders between two levels
+// as in 64 bits: in float32 first (error below 3e-5 of a level), and in double where a value lies
+// within 4e-5 of a border. m is kept as a float pair (product and its FMA remainder: exact) and
+// the sum of squares as a float pair per thread (TwoSum) and in double across threads, so the
+// float16 scale is the rounded float32 of the 64-bit value too. A row holding inf or NaN
+// gets NaN scales and zero levels.
+#include "qs_kernels.h"
+
+namespace qs {
+
+namespace {
+
+struct NormArgs {
+    const void* x;
+    const void* res;   // or null
+    void* total;       // null without a residual; may be x or res
+    const float* w;
+    uint8_t* dst;
+    int64_t x_stride, res_stride, total_stride;  // elements
+    int64_t dst_stride;                          // bytes
+    int k;
+    double eps;
+};
+
+__device__ __forceinline__ void two_sum(float& hi, float& lo, float v) {
+    const float s = __fadd_rn(hi, v), b = __fsub_rn(s, hi);
+    lo = __fadd_rn(lo, __fadd_rn(__fsub_rn(hi, __fsub_rn(s, b)), __fsub_rn(v, b)));
+    hi = s;
+}
+
+__device__ __forceinline__ double block_sum(double v, double* red) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();  // red may still be read from an earlier sum
+    if (lane == 0) red[warp] = v;
+    __syncthreads();
+    double s = lane < nw ? red[lane] : 0.0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    return s;
+}
+
+// 8 values of chunk c of the row: t; with a residual it is also written to `total`
+template <int SRC, bool RES>
+__device__ __forceinline__ void load_chunk(const NormArgs& a, int64_t row, int c, float* v) {
+    load_row<8>(a.x, row * a.x_stride + 8 * (int64_t)c, SRC, v);
+    if constexpr (RES) {
+        float r[8];
+        load_row<8>(a.res, row * a.res_stride + 8 * (int64_t)c, SRC, r);
+        const int64_t o = row * a.total_stride + 8 * (int64_t)c;
+        if constexpr (SRC == SRC_F32) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = __fadd_rn(v[i], r[i]);
+            {
+                float4* p = reinterpret_cast<float4*>(static_cast<float*>(a.total) + o);
+                p[0] = make_float4(v[0], v[1], v[2], v[3]);
+                p[1] = make_float4(v[4], v[5], v[6], v[7]);
+            }
+        } else {
+            uint32_t b[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                uint32_t h[2];
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const float s = __fadd_rn(v[2 * i + j], r[2 * i + j]);
+                    if constexpr (SRC == SRC_BF16) {
+                        h[j] = __bfloat16_as_ushort(__float2bfloat16_rn(s));
+                        v[2 * i + j] = __uint_as_float(h[j] << 16);
+                    } else {
+                        h[j] = f16_bits(s);
+                        v[2 * i + j] = f16_val((uint16_t)h[j]);
+                    }
+                }
+                b[i] = h[0] | (h[1] << 16);
+            }
+            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.total) + o) = make_uint4(b[0], b[1], b[2], b[3]);
+        }
+    }
+}
+
+// The same values a second time. `total` may be x or the residual, so with a residual this is
+// what the thread itself stored (a coherent load).
+template <int SRC, bool RES>
+__device__ __forceinline__ void reload_chunk(const NormArgs& a, int64_t row, int c, float* v) {
+    if constexpr (!RES) {
+        load_row<8>(a.x, row * a.x_stride + 8 * (int64_t)c, SRC, v);
+    } else {
+        const int64_t o = row * a.total_stride + 8 * (int64_t)c;
+        if constexpr (SRC == SRC_F32) {
+            const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(a.total) + o);
+            const float4 b0 = __ldcg(p), b1 = __ldcg(p + 1);
+            v[0] = b0.x; v[1] = b0.y; v[2] = b0.z; v[3] = b0.w;
+            v[4] = b1.x; v[5] = b1.y; v[6] = b1.z; v[7] = b1.w;
+        } else {
+            const uint4 b = __ldcg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.total) + o));
+            const uint32_t w4[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const uint32_t h = (w4[j >> 1] >> (16 * (j & 1))) & 0xFFFFu;
+                v[j] = SRC == SRC_BF16 ? __uint_as_float(h << 16) : f16_val((uint16_t)h);
+            }
+        }
+    }
+}
+
+// One row per CTA; a thread owns chunks of 8 values, 4 adjacent lanes one block. CH: chunks a
+// thread keeps in registers between the two passes over the row; CH = 0: rows longer than the
+// registers hold, read twice (the second time from L2).
+template <int SRC, bool RES, int CH>
+__global__ void __launch_bounds__(CH == 0 ? 1024 : CH == 4 ? 512 : 1024) norm_kernel(NormArgs a) {
+    __shared__ double red[32];
+    __shared__ __align__(16) uint8_t stage[32][272];  // 8 blocks per warp
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nchunk = a.k >> 3;
+    const int64_t row = blockIdx.x;
+    constexpr int NC = CH == 0 ? 1 : CH;
+    float v[NC][8];
+    float hi = 0.0f, lo = 0.0f;
+    auto add_squares = [&](const float* t) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float p = __fmul_rn(t[i], t[i]);
+            two_sum(hi, lo, p);
+            // products of 16-bit values are exact in float32
+            if constexpr (SRC == SRC_F32) lo = __fadd_rn(lo, __fmaf_rn(t[i], t[i], -p));
+        }
+    };
+    if constexpr (CH == 0) {
+        for (int c = tid; c < nchunk; c += blockDim.x) {
+            load_chunk<SRC, RES>(a, row, c, v[0]);
+            add_squares(v[0]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < NC; j++) {
+            const int c = tid + j * blockDim.x;
+            if (c < nchunk) load_chunk<SRC, RES>(a, row, c, v[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < NC; j++)
+            if (tid + j * (int)blockDim.x < nchunk) add_squares(v[j]);
+    }
+    double sum = block_sum((double)hi + (double)lo, red);
+    // squares beyond float32's range, or so small that they were lost: once more in double
+    if (!(sum < 1e37) || sum < 1e-27 * (double)a.k) {
+        double s = 0.0;
+        if constexpr (CH == 0) {
+            for (int c = tid; c < nchunk; c += blockDim.x) {
+                reload_chunk<SRC, RES>(a, row, c, v[0]);
+                for (int i = 0; i < 8; i++) s += (double)v[0][i] * (double)v[0][i];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < NC; j++)
+                if (tid + j * (int)blockDim.x < nchunk)
+                    for (int i = 0; i < 8; i++) s += (double)v[j][i] * (double)v[j][i];
+        }
+        sum = block_sum(s, red);
+    }
+    const bool bad = !(sum <= 1.7e308);
+    const double r127 = 1.0 / sqrt(sum / (double)a.k + a.eps) / 127.0;
+    uint8_t* out = a.dst + row * a.dst_stride;
+    const int rounds = (nchunk + blockDim.x - 1) / blockDim.x;
+#pragma unroll
+    for (int j = 0; j < (CH == 0 ? rounds : NC); j++) {
+        const int c0 = j * (int)blockDim.x + warp * 32, c = c0 + lane;
+        if (CH != 0 && j >= rounds) break;
+        if (c0 >= nchunk) break;  // whole warps leave together
+        float* t = v[CH == 0 ? 0 : j];
+        const bool live = c < nchunk;  // nchunk is a multiple of 4: the 4 lanes of a block agree
+        float w[8];
+        if (live) {
+            if constexpr (CH == 0) reload_chunk<SRC, RES>(a, row, c, t);
+            load_f32<8>(a.w + 8 * (int64_t)c, w);
+        }
+        float mh = 0.0f, p[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            p[i] = live ? __fmul_rn(fabsf(t[i]), fabsf(w[i])) : 0.0f;
+            mh = fmaxf(mh, p[i]);
+        }
+        mh = fmaxf(mh, __shfl_xor_sync(0xffffffffu, mh, 1));
+        mh = fmaxf(mh, __shfl_xor_sync(0xffffffffu, mh, 2));
+        const bool plain = mh > 1e-25f && mh < 1e37f;  // products and remainders are normal numbers
+        double m;
+        {
+            float me = -INFINITY;  // the largest remainder among the largest products
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (live && p[i] == mh) me = fmaxf(me, __fmaf_rn(fabsf(t[i]), fabsf(w[i]), -p[i]));
+            me = fmaxf(me, __shfl_xor_sync(0xffffffffu, me, 1));
+            me = fmaxf(me, __shfl_xor_sync(0xffffffffu, me, 2));
+            m = (double)mh + (double)me;
+        }
+        if (!plain) {
+            m = 0.0;
+            for (int i = 0; i < 8; i++)
+                if (live) m = fmax(m, fabs((double)t[i] * (double)w[i]));
+        }
+        // the 4 lanes of a block agree on `plain`; the exchange is for all lanes
+        {
+            const double o1 = __shfl_xor_sync(0xffffffffu, m, 1);
+            if (!plain) m = fmax(m, o1);
+            const double o2 = __shfl_xor_sync(0xffffffffu, m, 2);
+            if (!plain) m = fmax(m, o2);
+        }
+        const float inv = __fdiv_rn(127.0f, mh);
+        uint32_t q[2] = {0, 0};
+        if (live && !bad && m > 0.0) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float u = __fadd_rn(__fmul_rn(p[i], inv), 0.5f);
+                float f = floorf(u);
+                if (!plain || u - f < 4e-5f || u - f > 1.0f - 4e-5f)
+                    f = (float)floor(__dadd_rn(__dmul_rn(127.0, fabs((double)t[i] * (double)w[i]) / m), 0.5));
+                int l = (int)f;
+                if ((__float_as_uint(t[i]) ^ __float_as_uint(w[i])) >> 31) l = -l;
+                q[i >> 2] |= (uint32_t)(l & 0xFF) << (8 * (i & 3));
+            }
+        }
+        // 34-byte blocks: staged per warp, then whole 16-byte pieces where they line up
+        const float df = (float)(m * r127);
+        const uint16_t d = bad || !(m <= 1.7e308) ? (uint16_t)0x7E00 : f16_bits(df);
+        uint8_t* sb = stage[warp] + (lane >> 2) * 34;
+        const int o = 2 + 8 * (lane & 3);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            *reinterpret_cast<uint16_t*>(sb + o + 4 * i) = (uint16_t)q[i];
+            *reinterpret_cast<uint16_t*>(sb + o + 4 * i + 2) = (uint16_t)(q[i] >> 16);
+        }
+        if ((lane & 3) == 0) *reinterpret_cast<uint16_t*>(sb) = d;
+        __syncwarp();
+        uint8_t* g = out + (int64_t)(c0 >> 2) * 34;
+        const int nb = min(8, (nchunk - c0) >> 2) * 34;
+        if (nb == 272 && ((uintptr_t)g & 15) == 0) {
+            if (lane < 17) reinterpret_cast<uint4*>(g)[lane] = reinterpret_cast<const uint4*>(stage[warp])[lane];
+        } else if (((uintptr_t)g & 1) == 0) {
+            for (int i = lane; i < nb / 2; i += 32) reinterpret_cast<uint16_t*>(g)[i] = reinterpret_cast<const uint16_t*>(stage[warp])[i];
+        } else {
+            for (int i = lane; i < nb; i += 32) g[i] = stage[warp][i];
+        }
+    }
+}
+
+template <int SRC, bool RES>
+cudaError_t launch_t(const NormArgs& a, int64_t rows, const LaunchCtx& ctx) {
+    const int nchunk = a.k / 8;
+    const int whole = (nchunk + 31) / 32 * 32;
+    // Few rows: as many threads per row as it has chunks (latency). Many: 4 chunks a thread.
+    const bool few = rows < 4 * (int64_t)ctx.num_sms;
+    if (few && whole <= 1024) norm_kernel<SRC, RES, 1><<<(unsigned)rows, whole, 0, ctx.stream>>>(a);
+    else if (nchunk <= 4 * 512) norm_kernel<SRC, RES, 4><<<(unsigned)rows, ((nchunk + 3) / 4 + 31) / 32 * 32, 0, ctx.stream>>>(a);
+    else norm_kernel<SRC, RES, 0><<<(unsigned)rows, 1024, 0, ctx.stream>>>(a);
+    return cudaGetLastError();
+}
+
+template <int SRC>
+cudaError_t launch_s(const NormArgs& a, int64_t rows, const LaunchCtx& ctx) {
+    return a.res ? launch_t<SRC, true>(a, rows, ctx) : launch_t<SRC, false>(a, rows, ctx);
+}
+
+}  // namespace
+
+cudaError_t launch_rms_norm_q8(const NormCall& c, const LaunchCtx& ctx) {
+    NormArgs a;
+    a.x = c.x;
+    a.res = c.residual;
+    a.total = c.total;
+    a.w = c.weight;
+    a.dst = static_cast<uint8_t*>(c.dst);
+    a.x_stride = c.x_stride;
+    a.res_stride = c.residual_stride;
+    a.total_stride = c.total_stride;
+    a.dst_stride = c.dst_row_bytes;
+    a.k = (int)c.k;
+    a.eps = c.eps;
+    switch (c.x_type) {
+    case SRC_F32: return launch_s<SRC_F32>(a, c.n_rows, ctx);
+    case SRC_F16: return launch_s<SRC_F16>(a, c.n_rows, ctx);
+    default: return launch_s<SRC_BF16>(a, c.n_rows, ctx);
+    }
+}
+
+}  // namespace qs

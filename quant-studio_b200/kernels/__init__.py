@@ -14,7 +14,7 @@ object holding `quantize_<type>` and `SPECS`, under the reference's module name,
 import sys
 import types
 
-from . import _specs
+from . import _specs, ops  # noqa: F401  ops: norm, routing and products on packed blocks
 from .common import QuantSpec, TORCH_DTYPES
 
 # reference module name -> the type names it provides

@@ -63,6 +63,15 @@ def lib() -> ctypes.CDLL:
             L.qs_tensor_error.argtypes = [ctypes.c_int, c_vp, c_i64, c_vp, ctypes.c_int, c_i64, c_i64, c_vp, c_vp, c_vp]
             L.qs_tensor_error_noalloc.argtypes = L.qs_tensor_error.argtypes
             L.qs_device_fault.argtypes = [ctypes.c_int, ctypes.POINTER(ctypes.c_int)]
+            c_i, p_i64 = ctypes.c_int, ctypes.POINTER(c_i64)
+            L.qs_rms_norm_q8.argtypes = [c_vp, c_i, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, ctypes.c_double, c_i64, c_i64, c_vp, c_i64, c_vp]
+            L.qs_route.argtypes = [c_vp, c_i, c_i64, c_i64, c_i, c_i, c_i, c_vp, c_i, c_i, c_i, c_i, ctypes.c_float, c_vp, c_vp, c_vp]
+            L.qs_expert_plan.argtypes = [c_vp, c_i64, c_i, c_vp, c_vp, c_vp]
+            L.qs_matmul.argtypes = [c_i, c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_i, c_i64, c_vp, c_i64, c_vp]
+            L.qs_matmul_workspace.argtypes = [c_i, c_i64, c_i64, c_i64, p_i64]
+            L.qs_matmul_experts.argtypes = [c_i, c_vp, c_i64, c_i64, c_i, c_i64, c_i64, c_vp, c_i64, c_i, c_vp, c_vp, c_vp, c_i64, c_i,
+                                            c_vp, c_vp, c_i, c_i64, c_vp, c_i64, c_vp]
+            L.qs_matmul_experts_workspace.argtypes = [c_i, c_i, c_i64, c_i64, c_i64, c_i, c_i, c_i, p_i64]
             L.qs_last_error.restype = ctypes.c_char_p
             _lib = L
     return _lib
