@@ -56,9 +56,10 @@ struct TileCfg {
     static constexpr int WM = BN == 128 ? 2 : 4, WN = 8 / WM;  // warps along the rows / the slots
     static constexpr int MT = TM / WM / 16, NT = BN / WN / 8;  // 16 x 8 products of a warp
     // one stage: levels of the weights and the slots (128-byte rows, 16-byte pieces swizzled by
-    // the row), weight scales [unit][half][128], minima alike, slot planes [plane][unit][BN]
-    static constexpr int OFF_X = TM * 128, OFF_DL = OFF_X + BN * 128, OFF_ML = OFF_DL + TU * H * TM * 4;
-    static constexpr int OFF_XD = OFF_ML + (SUMS ? TU * H * TM * 4 : 0);
+    // the row), weight scales [unit][half][128] each twice (a packed pair), minima alike, slot
+    // planes [plane][unit][BN]
+    static constexpr int OFF_X = TM * 128, OFF_DL = OFF_X + BN * 128, OFF_ML = OFF_DL + TU * H * TM * 8;
+    static constexpr int OFF_XD = OFF_ML + (SUMS ? TU * H * TM * 8 : 0);
     static constexpr int STAGE = OFF_XD + (1 + SUMS) * TU * BN * 4;
     static constexpr int OUT_PITCH = TM + 4;
     static constexpr int BYTES = 2 * STAGE > BN * OUT_PITCH * 4 ? 2 * STAGE : BN * OUT_PITCH * 4;
@@ -73,12 +74,16 @@ __global__ void __launch_bounds__(TILE_THREADS, 2) tile_kernel(MmArgs a) {
     using C = TileCfg<T, BN>;
     constexpr int UPB = L::QK / 32, H = C::H, SUMS = C::SUMS, MT = C::MT, NT = C::NT;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int s_slot[BN];
+    __shared__ int s_slot[BN], s_row[BN];  // output slots and activation rows of the tile
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const Chunk ch = find_chunk<BN>(a, blockIdx.y);
     if (ch.group < 0) return;
     const int n0 = blockIdx.x * TM, cnt = ch.hi - ch.lo;
-    for (int i = tid; i < BN; i += TILE_THREADS) s_slot[i] = i < cnt ? (a.order ? __ldg(a.order + ch.lo + i) : ch.lo + i) : -1;
+    for (int i = tid; i < BN; i += TILE_THREADS) {
+        const int slot = i < cnt ? (a.order ? __ldg(a.order + ch.lo + i) : ch.lo + i) : -1;
+        s_slot[i] = slot;
+        s_row[i] = slot < 0 ? -1 : slot / a.x_div;
+    }
     __syncthreads();
     const int steps = a.units_pad / TU, per = (steps + a.splits - 1) / a.splits;
     const int k0 = blockIdx.z * per, k1 = min(k0 + per, steps);
@@ -118,22 +123,33 @@ __global__ void __launch_bounds__(TILE_THREADS, 2) tile_kernel(MmArgs a) {
                     make_uint4(wq[i][4 * h], wq[i][4 * h + 1], wq[i][4 * h + 2], wq[i][4 * h + 3]);
 #pragma unroll
             for (int h = 0; h < H; h++) {
-                reinterpret_cast<float*>(st + C::OFF_DL)[(u * H + h) * TM + scale_pos(row)] = wdl[i][h];
-                if constexpr (SUMS > 0) reinterpret_cast<float*>(st + C::OFF_ML)[(u * H + h) * TM + scale_pos(row)] = -wml[i][h];
+                reinterpret_cast<f32x2*>(st + C::OFF_DL)[(u * H + h) * TM + scale_pos(row)] = f2_splat(wdl[i][h]);
+                if constexpr (SUMS > 0) reinterpret_cast<f32x2*>(st + C::OFF_ML)[(u * H + h) * TM + scale_pos(row)] = f2_splat(-wml[i][h]);
             }
         }
     };
+    // a thread's copies: piece tid & 7 of the levels of slots tid / 8, tid / 8 + 32, ...; the planes
+    // by (plane, slot, unit). The sources advance by one step's bytes.
+    constexpr int XC = BN * 8 / TILE_THREADS, DC = ((1 + SUMS) * TU * BN + TILE_THREADS - 1) / TILE_THREADS;
+    int xrow[XC];
+#pragma unroll
+    for (int i = 0; i < XC; i++) xrow[i] = s_row[(tid >> 3) + i * (TILE_THREADS / 8)];
+    int drow[DC];
+#pragma unroll
+    for (int i = 0; i < DC; i++) drow[i] = s_row[((tid + i * TILE_THREADS) >> 2) % BN];
+    const int xpitch = a.units_pad * 32;
     auto copy_x = [&](int step, uint8_t* st) {
         const uint32_t base = smem_u32(st);
-        for (int i = tid; i < BN * 8; i += TILE_THREADS) {
-            const int t = i >> 3, c = i & 7, slot = s_slot[t];
-            const int64_t row = slot < 0 ? 0 : slot / a.x_div;
-            cp16(base + C::OFF_X + t * 128 + ((c ^ (t & 7)) << 4), a.xq + row * a.units_pad * 32 + step * 128 + c * 16, slot >= 0);
+#pragma unroll
+        for (int i = 0; i < XC; i++) {
+            const int t = (tid >> 3) + i * (TILE_THREADS / 8), c = tid & 7;
+            cp16(base + C::OFF_X + t * 128 + ((c ^ (t & 7)) << 4), a.xq + (int64_t)max(xrow[i], 0) * xpitch + (step * 128 + c * 16), xrow[i] >= 0);
         }
-        for (int i = tid; i < (1 + SUMS) * TU * BN; i += TILE_THREADS) {
-            const int u = i & 3, t = (i >> 2) % BN, p = (i >> 2) / BN, slot = s_slot[t];
-            const int64_t row = slot < 0 ? 0 : slot / a.x_div;
-            cp4(base + C::OFF_XD + ((p * TU + u) * BN + t) * 4, a.xd + p * a.x_plane + row * a.units_pad + step * TU + u, slot >= 0);
+#pragma unroll
+        for (int i = 0; i < DC; i++) {
+            const int j = tid + i * TILE_THREADS, u = j & 3, t = (j >> 2) % BN, p = (j >> 2) / BN;
+            if (DC * TILE_THREADS == (1 + SUMS) * TU * BN || j < (1 + SUMS) * TU * BN)
+                cp4(base + C::OFF_XD + ((p * TU + u) * BN + t) * 4, a.xd + p * a.x_plane + (int64_t)max(drow[i], 0) * a.units_pad + (step * TU + u), drow[i] >= 0);
         }
         cp_commit();
     };
@@ -180,14 +196,14 @@ __global__ void __launch_bounds__(TILE_THREADS, 2) tile_kernel(MmArgs a) {
                     f32x2 dl[H][2], ml[H][2];
 #pragma unroll
                     for (int h = 0; h < H; h++) {
-                        const int o = ((u * H + h) * TM + wm * (TM / C::WM) + i * 16 + 2 * g) * 4;
-                        const float2 v = *reinterpret_cast<const float2*>(st + C::OFF_DL + o);
-                        dl[h][0] = f2_splat(v.x);
-                        dl[h][1] = f2_splat(v.y);
+                        const int o = ((u * H + h) * TM + wm * (TM / C::WM) + i * 16 + 2 * g) * 8;
+                        const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(st + C::OFF_DL + o);
+                        dl[h][0] = v.x;
+                        dl[h][1] = v.y;
                         if constexpr (SUMS > 0) {
-                            const float2 m = *reinterpret_cast<const float2*>(st + C::OFF_ML + o);
-                            ml[h][0] = f2_splat(m.x);
-                            ml[h][1] = f2_splat(m.y);
+                            const ulonglong2 m = *reinterpret_cast<const ulonglong2*>(st + C::OFF_ML + o);
+                            ml[h][0] = m.x;
+                            ml[h][1] = m.y;
                         }
                     }
 #pragma unroll

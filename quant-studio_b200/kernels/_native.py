@@ -7,6 +7,7 @@ present, every quantize call raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import subprocess
 import threading
@@ -88,6 +89,7 @@ def row_bytes(ggml_type: int, k: int) -> int:
     return out.value
 
 
+@functools.lru_cache(maxsize=None)
 def block_info(ggml_type: int) -> tuple[int, int]:
     qk, nb = ctypes.c_int(), ctypes.c_int()
     check(lib().qs_block_info(int(ggml_type), ctypes.byref(qk), ctypes.byref(nb)))
@@ -143,13 +145,12 @@ def _blocks_arg(blocks: torch.Tensor, ggml_type: int) -> tuple[int, int]:
 def dequantize(blocks: torch.Tensor, ggml_type: int) -> torch.Tensor:
     """Decode (n_rows, row_bytes) packed blocks to a new (n_rows, k) float32 tensor on the
     same device: the values gguf.quants.dequantize returns for the same bytes."""
-    n, k = _blocks_arg(blocks, ggml_type)
-    out = torch.empty((n, k + (-k) % 4), dtype=torch.float32, device=blocks.device)
-    stream = torch.cuda.current_stream(blocks.device)
-    with torch.cuda.device(blocks.device):
-        check(lib().qs_dequantize(int(ggml_type), blocks.data_ptr(), blocks.stride(0), n, k,
-                                  out.data_ptr(), out.stride(0), stream.cuda_stream))
-    return out[:, :k]
+    n, k = _blocks_arg(blocks, ggml_type)  # k: a multiple of 32
+    out = torch.empty((n, k), dtype=torch.float32, device=blocks.device)
+    # the library makes the blocks' device current for the call
+    check(lib().qs_dequantize(int(ggml_type), blocks.data_ptr(), blocks.stride(0), n, k, out.data_ptr(), out.stride(0),
+                              torch._C._cuda_getCurrentRawStream(blocks.get_device())))
+    return out
 
 
 def _error_args(blocks: torch.Tensor, ggml_type: int, x: torch.Tensor, qw: torch.Tensor | None):
