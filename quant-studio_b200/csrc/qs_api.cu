@@ -461,7 +461,8 @@ MmPlan mm_plan(int type, int64_t n, int64_t k, int64_t slots, int64_t groups, in
     p.planes = 1 + (has_min(type) ? (type == qs::QS_Q2_K ? 2 : 1) : 0);
     p.splits = 1;
     const int64_t avg = (slots + groups - 1) / groups;
-    p.few = groups == 1 ? slots <= 8 : avg <= 4;
+    // rows that the small kernel can not hold go to the tiles whatever their number
+    p.few = (groups == 1 ? slots <= qs::FEW_SLOTS : avg <= 4) && (int64_t)p.units * qs::FEW_SLOTS * qs::FEW_UNIT_MAX <= qs::FEW_SMEM_MAX;
     if (!p.few) {
         p.bn = avg <= 32 ? 32 : avg <= 64 ? 64 : 128;
         const int64_t chunks = groups == 1 ? (slots + p.bn - 1) / p.bn : slots / p.bn + (groups < slots ? groups : slots) / 2 + 1;

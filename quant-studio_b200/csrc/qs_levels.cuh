@@ -3,9 +3,11 @@
 // levels, one scale per 32 values) are then sums of exact integer dot products.
 //
 // Unit: 32 consecutive values of a row, aligned to 32 (one Q8_0 block of the activations).
-// Lv<T>::unit gives its levels as 8 words (4 levels each, value order) and dl, ml of its two
-// halves of 16 values; G16: the halves' scales differ; HASMIN: ml is not always zero. dl and
-// ml are exact: a float16 times a few scale bits.
+// Lv<T>::load brings what unit j of a block needs into WORDS registers, Lv<T>::levels makes of
+// them its levels as 8 words (4 levels each, value order) and dl, ml of its two halves of 16
+// values; two steps, so that loads can run ahead. G16: the halves' scales differ; HASMIN: ml is
+// not always zero; SIGNED: levels are int8 (else 0 .. 31). dl and ml are exact: a float16
+// times a few scale bits. |weight| <= BD |d| + BM |m| with the float16 d at byte D, m at M.
 #pragma once
 
 #include "qs_kernels.h"
@@ -60,122 +62,154 @@ template <int T> struct Lv;
 
 template <> struct Lv<QS_Q4_0> {
     static constexpr int QK = 32, BB = 18, MAXAL = 2;
-    static constexpr bool G16 = false, HASMIN = false;
+    static constexpr bool G16 = false, HASMIN = false, SIGNED = true;
+    static constexpr int WORDS = 5, D = 0, M = 0;
+    static constexpr float BD = 8.0f, BM = 0.0f;
     template <int AL>
-    __device__ static void unit(const uint8_t* b, int, const uint16_t*, uint32_t* q, float* dl, float* ml) {
-        uint32_t w[4];
-        ld_words<4, 1>(b + 2, w);
-        dl[0] = dl[1] = h2f(ld_u16<AL>(b));
+    __device__ static void load(const uint8_t* b, int, uint32_t* r) {
+        ld_words<4, 1>(b + 2, r);
+        r[4] = ld_u16<AL>(b);
+    }
+    __device__ static void levels(const uint32_t* r, int, const uint16_t*, uint32_t* q, float* dl, float* ml) {
+        dl[0] = dl[1] = h2f(r[4]);
         ml[0] = ml[1] = 0.0f;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            q[i] = __vsub4(w[i] & 0x0F0F0F0Fu, 0x08080808u);
-            q[4 + i] = __vsub4((w[i] >> 4) & 0x0F0F0F0Fu, 0x08080808u);
+            q[i] = __vsub4(r[i] & 0x0F0F0F0Fu, 0x08080808u);
+            q[4 + i] = __vsub4((r[i] >> 4) & 0x0F0F0F0Fu, 0x08080808u);
         }
     }
 };
 
 template <> struct Lv<QS_Q4_1> {
     static constexpr int QK = 32, BB = 20, MAXAL = 4;
-    static constexpr bool G16 = false, HASMIN = true;
+    static constexpr bool G16 = false, HASMIN = true, SIGNED = false;
+    static constexpr int WORDS = 5, D = 0, M = 2;
+    static constexpr float BD = 15.0f, BM = 1.0f;
     template <int AL>
-    __device__ static void unit(const uint8_t* b, int, const uint16_t*, uint32_t* q, float* dl, float* ml) {
-        uint32_t w[5];
-        ld_words<5, AL>(b, w);
-        dl[0] = dl[1] = h2f(w[0] & 0xFFFFu);
-        ml[0] = ml[1] = -h2f(w[0] >> 16);
+    __device__ static void load(const uint8_t* b, int, uint32_t* r) {
+        ld_words<5, AL>(b, r);
+    }
+    __device__ static void levels(const uint32_t* r, int, const uint16_t*, uint32_t* q, float* dl, float* ml) {
+        dl[0] = dl[1] = h2f(r[0] & 0xFFFFu);
+        ml[0] = ml[1] = -h2f(r[0] >> 16);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            q[i] = w[1 + i] & 0x0F0F0F0Fu;
-            q[4 + i] = (w[1 + i] >> 4) & 0x0F0F0F0Fu;
+            q[i] = r[1 + i] & 0x0F0F0F0Fu;
+            q[4 + i] = (r[1 + i] >> 4) & 0x0F0F0F0Fu;
         }
     }
 };
 
 template <> struct Lv<QS_Q5_0> {
     static constexpr int QK = 32, BB = 22, MAXAL = 2;
-    static constexpr bool G16 = false, HASMIN = false;
+    static constexpr bool G16 = false, HASMIN = false, SIGNED = true;
+    static constexpr int WORDS = 6, D = 0, M = 0;
+    static constexpr float BD = 16.0f, BM = 0.0f;
     template <int AL>
-    __device__ static void unit(const uint8_t* b, int, const uint16_t*, uint32_t* q, float* dl, float* ml) {
-        uint32_t w[5];
-        ld_words<5, 1>(b + 2, w);
-        dl[0] = dl[1] = h2f(ld_u16<AL>(b));
+    __device__ static void load(const uint8_t* b, int, uint32_t* r) {
+        ld_words<5, 1>(b + 2, r);
+        r[5] = ld_u16<AL>(b);
+    }
+    __device__ static void levels(const uint32_t* r, int, const uint16_t*, uint32_t* q, float* dl, float* ml) {
+        dl[0] = dl[1] = h2f(r[5]);
         ml[0] = ml[1] = 0.0f;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            q[i] = __vsub4((w[1 + i] & 0x0F0F0F0Fu) | (bits_to_bytes(w[0] >> (4 * i)) << 4), 0x10101010u);
-            q[4 + i] = __vsub4(((w[1 + i] >> 4) & 0x0F0F0F0Fu) | (bits_to_bytes(w[0] >> (16 + 4 * i)) << 4), 0x10101010u);
+            q[i] = __vsub4((r[1 + i] & 0x0F0F0F0Fu) | (bits_to_bytes(r[0] >> (4 * i)) << 4), 0x10101010u);
+            q[4 + i] = __vsub4(((r[1 + i] >> 4) & 0x0F0F0F0Fu) | (bits_to_bytes(r[0] >> (16 + 4 * i)) << 4), 0x10101010u);
         }
     }
 };
 
 template <> struct Lv<QS_Q5_1> {
     static constexpr int QK = 32, BB = 24, MAXAL = 8;
-    static constexpr bool G16 = false, HASMIN = true;
+    static constexpr bool G16 = false, HASMIN = true, SIGNED = false;
+    static constexpr int WORDS = 6, D = 0, M = 2;
+    static constexpr float BD = 31.0f, BM = 1.0f;
     template <int AL>
-    __device__ static void unit(const uint8_t* b, int, const uint16_t*, uint32_t* q, float* dl, float* ml) {
-        uint32_t w[6];
-        ld_words<6, AL>(b, w);
-        dl[0] = dl[1] = h2f(w[0] & 0xFFFFu);
-        ml[0] = ml[1] = -h2f(w[0] >> 16);
+    __device__ static void load(const uint8_t* b, int, uint32_t* r) {
+        ld_words<6, AL>(b, r);
+    }
+    __device__ static void levels(const uint32_t* r, int, const uint16_t*, uint32_t* q, float* dl, float* ml) {
+        dl[0] = dl[1] = h2f(r[0] & 0xFFFFu);
+        ml[0] = ml[1] = -h2f(r[0] >> 16);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            q[i] = (w[2 + i] & 0x0F0F0F0Fu) | (bits_to_bytes(w[1] >> (4 * i)) << 4);
-            q[4 + i] = ((w[2 + i] >> 4) & 0x0F0F0F0Fu) | (bits_to_bytes(w[1] >> (16 + 4 * i)) << 4);
+            q[i] = (r[2 + i] & 0x0F0F0F0Fu) | (bits_to_bytes(r[1] >> (4 * i)) << 4);
+            q[4 + i] = ((r[2 + i] >> 4) & 0x0F0F0F0Fu) | (bits_to_bytes(r[1] >> (16 + 4 * i)) << 4);
         }
     }
 };
 
 template <> struct Lv<QS_Q8_0> {
     static constexpr int QK = 32, BB = 34, MAXAL = 2;
-    static constexpr bool G16 = false, HASMIN = false;
+    static constexpr bool G16 = false, HASMIN = false, SIGNED = true;
+    static constexpr int WORDS = 9, D = 0, M = 0;
+    static constexpr float BD = 128.0f, BM = 0.0f;
     template <int AL>
-    __device__ static void unit(const uint8_t* b, int, const uint16_t*, uint32_t* q, float* dl, float* ml) {
-        ld_words<8, 1>(b + 2, q);
-        dl[0] = dl[1] = h2f(ld_u16<AL>(b));
+    __device__ static void load(const uint8_t* b, int, uint32_t* r) {
+        ld_words<8, 1>(b + 2, r);
+        r[8] = ld_u16<AL>(b);
+    }
+    __device__ static void levels(const uint32_t* r, int, const uint16_t*, uint32_t* q, float* dl, float* ml) {
+        dl[0] = dl[1] = h2f(r[8]);
         ml[0] = ml[1] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) q[i] = r[i];
     }
 };
 
 template <> struct Lv<QS_Q2_K> {
     static constexpr int QK = 256, BB = 84, MAXAL = 4;
-    static constexpr bool G16 = true, HASMIN = true;
+    static constexpr bool G16 = true, HASMIN = true, SIGNED = false;
+    static constexpr int WORDS = 10, D = 80, M = 82;
+    static constexpr float BD = 45.0f, BM = 15.0f;
     template <int AL>
-    __device__ static void unit(const uint8_t* b, int j, const uint16_t*, uint32_t* q, float* dl, float* ml) {
-        uint32_t d[1];
-        ld_words<1, AL>(b + 80, d);
-        ld_words<8, AL>(b + 16 + 32 * (j / 4), q);
-        const float dd = h2f(d[0] & 0xFFFFu), dm = h2f(d[0] >> 16);
+    __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
+        ld_words<8, AL>(b + 16 + 32 * (j / 4), r);
+        ld_words<1, AL>(b + 80, r + 8);
+        r[9] = ld_u16<AL>(b + 2 * j);
+    }
+    __device__ static void levels(const uint32_t* r, int j, const uint16_t*, uint32_t* q, float* dl, float* ml) {
+        const float dd = h2f(r[8] & 0xFFFFu), dm = h2f(r[8] >> 16);
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const int sc = __ldg(b + 2 * j + h);
-            dl[h] = dd * (float)(sc & 15);
-            ml[h] = dm * (float)(sc >> 4);
+            const uint32_t sc = r[9] >> (8 * h);
+            dl[h] = dd * (float)(sc & 15u);
+            ml[h] = dm * (float)((sc >> 4) & 15u);
         }
 #pragma unroll
-        for (int i = 0; i < 8; i++) q[i] = (q[i] >> (2 * (j & 3))) & 0x03030303u;
+        for (int i = 0; i < 8; i++) q[i] = (r[i] >> (2 * (j & 3))) & 0x03030303u;
     }
 };
 
 template <> struct Lv<QS_Q3_K> {
     static constexpr int QK = 256, BB = 110, MAXAL = 2;
-    static constexpr bool G16 = true, HASMIN = false;
+    static constexpr bool G16 = true, HASMIN = false, SIGNED = true;
+    static constexpr int WORDS = 20, D = 108, M = 0;
+    static constexpr float BD = 128.0f, BM = 0.0f;
     template <int AL>
-    __device__ static void unit(const uint8_t* b, int j, const uint16_t*, uint32_t* q, float* dl, float* ml) {
-        uint32_t hm[8];
-        ld_words<8, AL>(b + 32 + 32 * (j / 4), q);
-        ld_words<8, AL>(b, hm);
-        const float d = h2f(ld_u16<AL>(b + 108));
+    __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
+        ld_words<8, AL>(b + 32 + 32 * (j / 4), r);
+        ld_words<8, AL>(b, r + 8);
+        ld_words<3, 1>(b + 96, r + 16);
+        r[19] = ld_u16<AL>(b + 108);
+    }
+    __device__ static void levels(const uint32_t* r, int j, const uint16_t*, uint32_t* q, float* dl, float* ml) {
+        // scale g = 2 j + h: low 4 bits in nibble g / 8 of byte g % 8, high 2 bits of byte 8 + g % 4
+        const float d = h2f(r[19]);
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const int g = 2 * j + h;
-            const int ls = (__ldg(b + 96 + g % 8) >> (4 * (g / 8))) & 0xF, hs = (__ldg(b + 104 + g % 4) >> (2 * (g / 4))) & 3;
-            dl[h] = d * (float)((ls | (hs << 4)) - 32);
+            const uint32_t ls = ((g & 4 ? r[17] : r[16]) >> (8 * (g & 3) + 4 * (g >> 3))) & 15u;
+            const uint32_t hs = (r[18] >> (8 * (g & 3) + 2 * (g >> 2))) & 3u;
+            dl[h] = d * (float)((int)(ls | (hs << 4)) - 32);
             ml[h] = 0.0f;
         }
 #pragma unroll
         for (int i = 0; i < 8; i++)
-            q[i] = __vsub4(((q[i] >> (2 * (j & 3))) & 0x03030303u) | (((hm[i] >> j) & 0x01010101u) << 2), 0x04040404u);
+            q[i] = __vsub4(((r[i] >> (2 * (j & 3))) & 0x03030303u) | (((r[8 + i] >> j) & 0x01010101u) << 2), 0x04040404u);
     }
 };
 
@@ -189,57 +223,67 @@ __device__ __forceinline__ void k4_scale_min(const uint32_t* s, int j, float& sc
 
 template <> struct Lv<QS_Q4_K> {
     static constexpr int QK = 256, BB = 144, MAXAL = 16;
-    static constexpr bool G16 = false, HASMIN = true;
+    static constexpr bool G16 = false, HASMIN = true, SIGNED = false;
+    static constexpr int WORDS = 12, D = 0, M = 2;
+    static constexpr float BD = 945.0f, BM = 63.0f;
     template <int AL>
-    __device__ static void unit(const uint8_t* b, int j, const uint16_t*, uint32_t* q, float* dl, float* ml) {
-        uint32_t h[4];
-        ld_words<4, AL>(b, h);
-        ld_words<8, AL>(b + 16 + 32 * (j / 2), q);
+    __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
+        ld_words<4, AL>(b, r + 8);
+        ld_words<8, AL>(b + 16 + 32 * (j / 2), r);
+    }
+    __device__ static void levels(const uint32_t* r, int j, const uint16_t*, uint32_t* q, float* dl, float* ml) {
         float sc, mn;
-        k4_scale_min(h + 1, j, sc, mn);
-        dl[0] = dl[1] = h2f(h[0] & 0xFFFFu) * sc;
-        ml[0] = ml[1] = h2f(h[0] >> 16) * mn;
+        k4_scale_min(r + 9, j, sc, mn);
+        dl[0] = dl[1] = h2f(r[8] & 0xFFFFu) * sc;
+        ml[0] = ml[1] = h2f(r[8] >> 16) * mn;
 #pragma unroll
-        for (int i = 0; i < 8; i++) q[i] = (q[i] >> (4 * (j & 1))) & 0x0F0F0F0Fu;
+        for (int i = 0; i < 8; i++) q[i] = (r[i] >> (4 * (j & 1))) & 0x0F0F0F0Fu;
     }
 };
 
 template <> struct Lv<QS_Q5_K> {
     static constexpr int QK = 256, BB = 176, MAXAL = 16;
-    static constexpr bool G16 = false, HASMIN = true;
+    static constexpr bool G16 = false, HASMIN = true, SIGNED = false;
+    static constexpr int WORDS = 20, D = 0, M = 2;
+    static constexpr float BD = 1953.0f, BM = 63.0f;
     template <int AL>
-    __device__ static void unit(const uint8_t* b, int j, const uint16_t*, uint32_t* q, float* dl, float* ml) {
-        uint32_t h[4], hi[8];
-        ld_words<4, AL>(b, h);
-        ld_words<8, AL>(b + 16, hi);
-        ld_words<8, AL>(b + 48 + 32 * (j / 2), q);
+    __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
+        ld_words<4, AL>(b, r + 8);
+        ld_words<8, AL>(b + 16, r + 12);
+        ld_words<8, AL>(b + 48 + 32 * (j / 2), r);
+    }
+    __device__ static void levels(const uint32_t* r, int j, const uint16_t*, uint32_t* q, float* dl, float* ml) {
         float sc, mn;
-        k4_scale_min(h + 1, j, sc, mn);
-        dl[0] = dl[1] = h2f(h[0] & 0xFFFFu) * sc;
-        ml[0] = ml[1] = h2f(h[0] >> 16) * mn;
+        k4_scale_min(r + 9, j, sc, mn);
+        dl[0] = dl[1] = h2f(r[8] & 0xFFFFu) * sc;
+        ml[0] = ml[1] = h2f(r[8] >> 16) * mn;
 #pragma unroll
         for (int i = 0; i < 8; i++)
-            q[i] = ((q[i] >> (4 * (j & 1))) & 0x0F0F0F0Fu) | (((hi[i] >> j) & 0x01010101u) << 4);
+            q[i] = ((r[i] >> (4 * (j & 1))) & 0x0F0F0F0Fu) | (((r[12 + i] >> j) & 0x01010101u) << 4);
     }
 };
 
 template <> struct Lv<QS_Q6_K> {
     static constexpr int QK = 256, BB = 210, MAXAL = 2;
-    static constexpr bool G16 = true, HASMIN = false;
+    static constexpr bool G16 = true, HASMIN = false, SIGNED = true;
+    static constexpr int WORDS = 18, D = 208, M = 0;
+    static constexpr float BD = 4096.0f, BM = 0.0f;
     template <int AL>
-    __device__ static void unit(const uint8_t* b, int j, const uint16_t*, uint32_t* q, float* dl, float* ml) {
+    __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
+        ld_words<8, AL>(b + 64 * (j / 4) + 32 * (j & 1), r);
+        ld_words<8, AL>(b + 128 + 32 * (j / 4), r + 8);
+        r[16] = ld_u16<AL>(b + 208);
+        r[17] = ld_u16<AL>(b + 192 + 2 * j);
+    }
+    __device__ static void levels(const uint32_t* r, int j, const uint16_t*, uint32_t* q, float* dl, float* ml) {
         // unit j: half c = j / 4, low nibbles of ql at 32 (j & 1) for j & 3 < 2, high ones for the rest
-        uint32_t hi[8];
-        ld_words<8, AL>(b + 64 * (j / 4) + 32 * (j & 1), q);
-        ld_words<8, AL>(b + 128 + 32 * (j / 4), hi);
-        const float d = h2f(ld_u16<AL>(b + 208));
-        const uint32_t s = ld_u16<AL>(b + 192 + 2 * j);
-        dl[0] = d * (float)(int8_t)(s & 0xFFu);
-        dl[1] = d * (float)(int8_t)(s >> 8);
+        const float d = h2f(r[16]);
+        dl[0] = d * (float)(int8_t)(r[17] & 0xFFu);
+        dl[1] = d * (float)(int8_t)(r[17] >> 8);
         ml[0] = ml[1] = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; i++)
-            q[i] = __vsub4(((q[i] >> (4 * ((j >> 1) & 1))) & 0x0F0F0F0Fu) | (((hi[i] >> (2 * (j & 3))) & 0x03030303u) << 4), 0x20202020u);
+            q[i] = __vsub4(((r[i] >> (4 * ((j >> 1) & 1))) & 0x0F0F0F0Fu) | (((r[8 + i] >> (2 * (j & 3))) & 0x03030303u) << 4), 0x20202020u);
     }
 };
 
@@ -259,34 +303,42 @@ __device__ __forceinline__ uint32_t sign8(uint32_t i) { return i | ((__popc(i) &
 
 template <> struct Lv<QS_IQ2_XXS> {
     static constexpr int QK = 256, BB = 66, MAXAL = 2;
-    static constexpr bool G16 = false, HASMIN = false;
+    static constexpr bool G16 = false, HASMIN = false, SIGNED = true;
+    static constexpr int WORDS = 3, D = 0, M = 0;
+    static constexpr float BD = 167.0f, BM = 0.0f;
     template <int AL>
-    __device__ static void unit(const uint8_t* b, int j, const uint16_t* kgrid, uint32_t* q, float* dl, float* ml) {
-        uint32_t w[2];
-        ld_words<2, 1>(b + 2 + 8 * j, w);
-        dl[0] = dl[1] = (h2f(ld_u16<AL>(b)) * (0.5f + (float)(w[1] >> 28))) * 0.25f;
+    __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
+        ld_words<2, 1>(b + 2 + 8 * j, r);
+        r[2] = ld_u16<AL>(b);
+    }
+    __device__ static void levels(const uint32_t* r, int, const uint16_t* kgrid, uint32_t* q, float* dl, float* ml) {
+        dl[0] = dl[1] = (h2f(r[2]) * (0.5f + (float)(r[1] >> 28))) * 0.25f;
         ml[0] = ml[1] = 0.0f;
 #pragma unroll
         for (int s = 0; s < 4; s++)
-            iq2_signed(__ldg(kgrid + ((w[0] >> (8 * s)) & 0xFFu)), sign8((w[1] >> (7 * s)) & 127u), q + 2 * s);
+            iq2_signed(__ldg(kgrid + ((r[0] >> (8 * s)) & 0xFFu)), sign8((r[1] >> (7 * s)) & 127u), q + 2 * s);
     }
 };
 
 template <> struct Lv<QS_IQ2_XS> {
     static constexpr int QK = 256, BB = 74, MAXAL = 2;
-    static constexpr bool G16 = true, HASMIN = false;
+    static constexpr bool G16 = true, HASMIN = false, SIGNED = true;
+    static constexpr int WORDS = 4, D = 0, M = 0;
+    static constexpr float BD = 167.0f, BM = 0.0f;
     template <int AL>
-    __device__ static void unit(const uint8_t* b, int j, const uint16_t* kgrid, uint32_t* q, float* dl, float* ml) {
-        uint32_t w[2];
-        ld_words<2, 1>(b + 2 + 8 * j, w);
-        const float d = h2f(ld_u16<AL>(b));
-        const int sc = __ldg(b + 66 + j);
-        dl[0] = (d * (0.5f + (float)(sc & 15))) * 0.25f;
-        dl[1] = (d * (0.5f + (float)(sc >> 4))) * 0.25f;
+    __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
+        ld_words<2, 1>(b + 2 + 8 * j, r);
+        r[2] = ld_u16<AL>(b);
+        r[3] = __ldg(b + 66 + j);
+    }
+    __device__ static void levels(const uint32_t* r, int, const uint16_t* kgrid, uint32_t* q, float* dl, float* ml) {
+        const float d = h2f(r[2]);
+        dl[0] = (d * (0.5f + (float)(r[3] & 15u))) * 0.25f;
+        dl[1] = (d * (0.5f + (float)(r[3] >> 4))) * 0.25f;
         ml[0] = ml[1] = 0.0f;
 #pragma unroll
         for (int s = 0; s < 4; s++) {
-            const uint32_t c = (w[s / 2] >> (16 * (s & 1))) & 0xFFFFu;
+            const uint32_t c = (r[s / 2] >> (16 * (s & 1))) & 0xFFFFu;
             iq2_signed(__ldg(kgrid + (c & 511u)), sign8(c >> 9), q + 2 * s);
         }
     }
@@ -294,21 +346,25 @@ template <> struct Lv<QS_IQ2_XS> {
 
 template <> struct Lv<QS_IQ2_S> {
     static constexpr int QK = 256, BB = 82, MAXAL = 2;
-    static constexpr bool G16 = true, HASMIN = false;
+    static constexpr bool G16 = true, HASMIN = false, SIGNED = true;
+    static constexpr int WORDS = 5, D = 0, M = 0;
+    static constexpr float BD = 167.0f, BM = 0.0f;
     template <int AL>
-    __device__ static void unit(const uint8_t* b, int j, const uint16_t* kgrid, uint32_t* q, float* dl, float* ml) {
-        uint32_t idx[1], sg[1];
-        ld_words<1, 1>(b + 2 + 4 * j, idx);
-        ld_words<1, 1>(b + 34 + 4 * j, sg);
-        const float d = h2f(ld_u16<AL>(b));
-        const int sc = __ldg(b + 74 + j);
-        const uint32_t qh = __ldg(b + 66 + j);
-        dl[0] = (d * (0.5f + (float)(sc & 15))) * 0.25f;
-        dl[1] = (d * (0.5f + (float)(sc >> 4))) * 0.25f;
+    __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
+        ld_words<1, 1>(b + 2 + 4 * j, r);
+        ld_words<1, 1>(b + 34 + 4 * j, r + 1);
+        r[2] = ld_u16<AL>(b);
+        r[3] = __ldg(b + 74 + j);
+        r[4] = __ldg(b + 66 + j);
+    }
+    __device__ static void levels(const uint32_t* r, int, const uint16_t* kgrid, uint32_t* q, float* dl, float* ml) {
+        const float d = h2f(r[2]);
+        dl[0] = (d * (0.5f + (float)(r[3] & 15u))) * 0.25f;
+        dl[1] = (d * (0.5f + (float)(r[3] >> 4))) * 0.25f;
         ml[0] = ml[1] = 0.0f;
 #pragma unroll
         for (int s = 0; s < 4; s++)
-            iq2_signed(__ldg(kgrid + (((idx[0] >> (8 * s)) & 0xFFu) | (((qh >> (2 * s)) & 3u) << 8))), (sg[0] >> (8 * s)) & 0xFFu, q + 2 * s);
+            iq2_signed(__ldg(kgrid + (((r[0] >> (8 * s)) & 0xFFu) | (((r[4] >> (2 * s)) & 3u) << 8))), (r[1] >> (8 * s)) & 0xFFu, q + 2 * s);
     }
 };
 
@@ -319,44 +375,54 @@ __device__ __forceinline__ uint32_t iq3_bytes(uint32_t c, uint32_t lo, uint32_t 
 
 template <> struct Lv<QS_IQ3_XXS> {
     static constexpr int QK = 256, BB = 98, MAXAL = 2;
-    static constexpr bool G16 = false, HASMIN = false;
+    static constexpr bool G16 = false, HASMIN = false, SIGNED = true;
+    static constexpr int WORDS = 4, D = 0, M = 0;
+    static constexpr float BD = 481.0f, BM = 0.0f;
     template <int AL>
-    __device__ static void unit(const uint8_t* b, int j, const uint16_t* kgrid, uint32_t* q, float* dl, float* ml) {
-        uint32_t idx[2], w[1];
-        ld_words<2, 1>(b + 2 + 8 * j, idx);
-        ld_words<1, 1>(b + 66 + 4 * j, w);
-        dl[0] = dl[1] = (h2f(ld_u16<AL>(b)) * (0.5f + (float)(w[0] >> 28))) * 0.5f;
+    __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
+        ld_words<2, 1>(b + 2 + 8 * j, r);
+        ld_words<1, 1>(b + 66 + 4 * j, r + 2);
+        r[3] = ld_u16<AL>(b);
+    }
+    __device__ static void levels(const uint32_t* r, int, const uint16_t* kgrid, uint32_t* q, float* dl, float* ml) {
+        dl[0] = dl[1] = (h2f(r[3]) * (0.5f + (float)(r[2] >> 28))) * 0.5f;
         ml[0] = ml[1] = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; i++) {  // levels 4, 12, ... 52, 62
-            const uint32_t sg = sign8((w[0] >> (7 * (i / 2))) & 127u) >> (4 * (i & 1));
-            q[i] = neg_bytes(iq3_bytes(__ldg(kgrid + ((idx[i / 4] >> (8 * (i & 3))) & 0xFFu)), 0x1C140C04u, 0x3E342C24u), bits_to_bytes(sg));
+            const uint32_t sg = sign8((r[2] >> (7 * (i / 2))) & 127u) >> (4 * (i & 1));
+            q[i] = neg_bytes(iq3_bytes(__ldg(kgrid + ((r[i / 4] >> (8 * (i & 3))) & 0xFFu)), 0x1C140C04u, 0x3E342C24u), bits_to_bytes(sg));
         }
     }
 };
 
 template <> struct Lv<QS_IQ3_S> {
     static constexpr int QK = 256, BB = 110, MAXAL = 2;
-    static constexpr bool G16 = false, HASMIN = false;
+    static constexpr bool G16 = false, HASMIN = false, SIGNED = true;
+    static constexpr int WORDS = 6, D = 0, M = 0;
+    static constexpr float BD = 465.0f, BM = 0.0f;
     template <int AL>
-    __device__ static void unit(const uint8_t* b, int j, const uint16_t* kgrid, uint32_t* q, float* dl, float* ml) {
-        uint32_t idx[2], sg[1];
-        ld_words<2, 1>(b + 2 + 8 * j, idx);
-        ld_words<1, 1>(b + 74 + 4 * j, sg);
-        const uint32_t qh = __ldg(b + 66 + j);
-        const int sc = (__ldg(b + 106 + j / 2) >> (4 * (j & 1))) & 15;
-        dl[0] = dl[1] = h2f(ld_u16<AL>(b)) * (float)(1 + 2 * sc);
+    __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
+        ld_words<2, 1>(b + 2 + 8 * j, r);
+        ld_words<1, 1>(b + 74 + 4 * j, r + 2);
+        r[3] = ld_u16<AL>(b);
+        r[4] = __ldg(b + 66 + j);
+        r[5] = __ldg(b + 106 + j / 2);
+    }
+    __device__ static void levels(const uint32_t* r, int j, const uint16_t* kgrid, uint32_t* q, float* dl, float* ml) {
+        dl[0] = dl[1] = h2f(r[3]) * (float)(1u + 2u * ((r[5] >> (4 * (j & 1))) & 15u));
         ml[0] = ml[1] = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; i++)  // levels 1, 3, ... 15
-            q[i] = neg_bytes(iq3_bytes(__ldg(kgrid + (((idx[i / 4] >> (8 * (i & 3))) & 0xFFu) | (((qh >> i) & 1u) << 8))), 0x07050301u, 0x0F0D0B09u),
-                             bits_to_bytes(sg[0] >> (4 * i)));
+            q[i] = neg_bytes(iq3_bytes(__ldg(kgrid + (((r[i / 4] >> (8 * (i & 3))) & 0xFFu) | (((r[4] >> i) & 1u) << 8))), 0x07050301u, 0x0F0D0B09u),
+                             bits_to_bytes(r[2] >> (4 * i)));
     }
 };
 
 template <> struct Lv<QS_IQ4_XS> {
     static constexpr int QK = 256, BB = 136, MAXAL = 8;
-    static constexpr bool G16 = false, HASMIN = false;
+    static constexpr bool G16 = false, HASMIN = false, SIGNED = true;
+    static constexpr int WORDS = 6, D = 0, M = 0;
+    static constexpr float BD = 4064.0f, BM = 0.0f;
     // the 16 level values, 4 to a word: -127 -104 -83 -65 | -49 -35 -22 -10 | 1 13 25 38 | 53 69 89 113
     __device__ static uint32_t value4(uint32_t n) {  // 4 nibbles (one per byte) -> their bytes
         const uint32_t lo = (n & 0x07u) | ((n & 0x0700u) >> 4) | ((n & 0x070000u) >> 8) | ((n & 0x07000000u) >> 12);
@@ -365,17 +431,18 @@ template <> struct Lv<QS_IQ4_XS> {
         return (a & ~m) | (c & m);
     }
     template <int AL>
-    __device__ static void unit(const uint8_t* b, int j, const uint16_t*, uint32_t* q, float* dl, float* ml) {
-        uint32_t h[2], w[4];
-        ld_words<2, AL>(b, h);
-        ld_words<4, AL>(b + 8 + 16 * j, w);
-        const int ls = (h[1] >> (4 * j)) & 15, hs = (h[0] >> (16 + 2 * j)) & 3;
-        dl[0] = dl[1] = h2f(h[0] & 0xFFFFu) * (float)((ls | (hs << 4)) - 32);
+    __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
+        ld_words<2, AL>(b, r + 4);
+        ld_words<4, AL>(b + 8 + 16 * j, r);
+    }
+    __device__ static void levels(const uint32_t* r, int j, const uint16_t*, uint32_t* q, float* dl, float* ml) {
+        const uint32_t ls = (r[5] >> (4 * j)) & 15u, hs = (r[4] >> (16 + 2 * j)) & 3u;
+        dl[0] = dl[1] = h2f(r[4] & 0xFFFFu) * (float)((int)(ls | (hs << 4)) - 32);
         ml[0] = ml[1] = 0.0f;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            q[i] = value4(w[i] & 0x0F0F0F0Fu);
-            q[4 + i] = value4((w[i] >> 4) & 0x0F0F0F0Fu);
+            q[i] = value4(r[i] & 0x0F0F0F0Fu);
+            q[4 + i] = value4((r[i] >> 4) & 0x0F0F0F0Fu);
         }
     }
 };

@@ -91,7 +91,7 @@ __device__ __forceinline__ Chunk find_chunk(const MmArgs& a, int c) {
 inline int64_t max_chunks(const MmArgs& a, int c) {
     if (!a.order) return ((int64_t)a.slots + c - 1) / c;
     const int64_t groups = a.n_exp + 1 < a.slots ? a.n_exp + 1 : a.slots;
-    return a.slots / c + groups;
+    return c == 1 ? a.slots : a.slots / c + groups;
 }
 
 __device__ __forceinline__ void store_val(void* p, int64_t i, int type, float v) {
@@ -111,6 +111,9 @@ __device__ __forceinline__ int sum16(const uint4& v) {
     return __dp4a((int)v.x, one, __dp4a((int)v.y, one, __dp4a((int)v.z, one, __dp4a((int)v.w, one, 0))));
 }
 
+// shared memory that the kernel for few slots may use: (32 levels, a scale, up to 2 sums) per unit
+// and slot, for up to 8 slots
+constexpr int FEW_SMEM_MAX = 200 * 1024, FEW_SLOTS = 8, FEW_UNIT_MAX = 44;
 cudaError_t launch_mm_few(int type, const MmArgs& a, const LaunchCtx& ctx);
 cudaError_t launch_mm_tile(int type, const MmArgs& a, int bn, const LaunchCtx& ctx);
 // activations into a.xq / a.xd (rows of the activations, not slots)

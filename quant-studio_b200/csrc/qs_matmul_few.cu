@@ -2,107 +2,137 @@
 //
 // The weights' bytes are the work: each is read once, a warp takes whole weight rows, lane l the
 // units l, l + 32, ... of a row, and the levels meet those of up to NT slots in 4-way integer
-// dot products (dp4a). The slots' Q8_0 rows are staged in shared memory once per CTA, in
-// slices of 128 units.
+// dot products (dp4a). The slots' Q8_0 rows are staged in shared memory once per CTA. A
+// warp's (row, unit) steps form one sequence over its rows, loaded PF steps ahead, so that
+// loads are in flight across row ends too.
+#include <algorithm>
+
 #include "qs_matmul.cuh"
 
 namespace qs {
 
 namespace {
 
-constexpr int FEW_WARPS = 8, FEW_ROWS = 2, SLICE = 128;  // warps, weight rows per warp, units per slice
-
 template <int T, int NT>
-struct FewSmem {
-    static constexpr int SUMS = !Lv<T>::HASMIN ? 0 : Lv<T>::G16 ? 2 : 1;
-    uint4 q[NT][2][SLICE];  // halves of 16 levels: adjacent lanes read adjacent 16 bytes
-    float d[NT][SLICE];
-    float s[SUMS ? SUMS : 1][NT][SUMS ? SLICE : 1];  // scale * sum of levels (of a half)
+struct FewCfg {
+    using L = Lv<T>;
+    static constexpr int SUMS = !L::HASMIN ? 0 : L::G16 ? 2 : 1;
+    static constexpr int PF = L::WORDS <= 6 ? 4 : 2;  // steps loaded ahead
+    // bytes per unit of a slot: levels as two planes of 16 bytes, scale, scale * sums of levels
+    static constexpr int UNIT = 32 + 4 + 4 * SUMS;
+    static int bytes(int units) { return NT * units * UNIT; }
 };
 
 template <int T, int NT>
-__global__ void __launch_bounds__(32 * FEW_WARPS) few_kernel(MmArgs a) {
+__global__ void __launch_bounds__(512) few_kernel(MmArgs a, int rows_per_warp) {
     using L = Lv<T>;
-    constexpr int UPB = L::QK / 32, SUMS = FewSmem<T, NT>::SUMS;
-    __shared__ FewSmem<T, NT> sm;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    using C = FewCfg<T, NT>;
+    constexpr int UPB = L::QK / 32, SUMS = C::SUMS, PF = C::PF;
+    extern __shared__ __align__(16) uint8_t smem[];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, units = a.units;
+    uint4* const xq = reinterpret_cast<uint4*>(smem);                         // [slot][half][unit]
+    float* const xd = reinterpret_cast<float*>(smem + NT * units * 32);       // [slot][unit]
+    float* const xs = xd + NT * units;                                        // [half][slot][unit]
     const Chunk ch = find_chunk<NT>(a, blockIdx.y);
     if (ch.group < 0) return;
-    const int n0 = (blockIdx.x * FEW_WARPS + warp) * FEW_ROWS, cnt = ch.hi - ch.lo;
-    float acc[FEW_ROWS][NT];
+    const int n0 = (blockIdx.x * (blockDim.x >> 5) + warp) * rows_per_warp, cnt = ch.hi - ch.lo;
+    const int rows = min(rows_per_warp, a.n - n0), iters = (units + 31) >> 5;  // rows may be <= 0
+    auto put = [&](int r, int t, float v) {
+        const int64_t slot = a.order ? __ldg(a.order + ch.lo + t) : ch.lo + t;
+        if (a.part) a.part[slot * a.n + n0 + r] = v;
+        else store_val(a.out, slot * a.out_stride + n0 + r, a.out_type, v);
+    };
+    if (a.order && ch.group == a.n_exp) {  // slots without an expert
+        for (int i = lane; i < rows * cnt; i += 32) put(i / cnt, i % cnt, 0.0f);
+        return;
+    }
+    // unit lane + 32 i of a row is unit j of its block for every i: UPB divides 32
+    const int j = lane % UPB, full = units >> 5;
+    constexpr int HOP = 32 / UPB * L::BB;  // bytes between a lane's blocks
+    const bool tail = lane < (units & 31);
+    const uint8_t* row_at = a.w + ch.group * a.w_exp + (int64_t)n0 * a.w_row + (lane / UPB) * L::BB;
+    const uint8_t* at = row_at;
+    uint32_t raw[PF][L::WORDS];
+    int lr = 0, li = 0;  // row and step of the next load
+    auto load = [&](uint32_t* r) {
+        if (lr < rows && (li < full || tail)) L::template load<L::MAXAL>(at, j, r);
+        at += HOP;
+        if (++li == iters) {
+            li = 0;
+            lr++;
+            at = row_at += a.w_row;
+        }
+    };
 #pragma unroll
-    for (int r = 0; r < FEW_ROWS; r++)
-#pragma unroll
-        for (int t = 0; t < NT; t++) acc[r][t] = 0.0f;
-    if (!a.order || ch.group < a.n_exp) {
-        const uint8_t* w = a.w + ch.group * a.w_exp;
-        for (int u0 = 0; u0 < a.units; u0 += SLICE) {
-            const int nu = min(SLICE, a.units - u0);
-            if (u0) __syncthreads();
-            for (int i = tid; i < NT * 2 * SLICE; i += 32 * FEW_WARPS) {
-                const int t = i / (2 * SLICE), u = (i / 2) % SLICE, h = i & 1;
-                uint4 q = make_uint4(0, 0, 0, 0);
-                float d = 0.0f;
-                if (t < cnt && u < nu) {
-                    const int slot = a.order ? __ldg(a.order + ch.lo + t) : ch.lo + t;
-                    const uint8_t* b = a.x + (slot / a.x_div) * a.x_row + (int64_t)(u0 + u) * 34;
-                    q = ld_16b(b + 2 + 16 * h);
-                    d = h2f(ld_u16<1>(b));
-                }
-                sm.q[t][h][u] = q;
-                if (h == 0) sm.d[t][u] = d;
-                if constexpr (SUMS == 2) sm.s[h][t][u] = d * (float)sum16(q);
-                if constexpr (SUMS == 1) {
-                    const int s = sum16(q), o = __shfl_xor_sync(0xffffffffu, s, 1);
-                    if (h == 0) sm.s[0][t][u] = d * (float)(s + o);
-                }
-            }
-            __syncthreads();
-#pragma unroll
-            for (int r = 0; r < FEW_ROWS; r++) {
-                if (n0 + r >= a.n) break;
-                const uint8_t* wr = w + (n0 + r) * a.w_row;
-#pragma unroll
-                for (int i = 0; i < SLICE / 32; i++) {
-                    const int u = lane + 32 * i;
-                    if (u >= nu) break;
-                    uint32_t q[8];
-                    float dl[2], ml[2];
-                    L::template unit<L::MAXAL>(wr + (int64_t)((u0 + u) / UPB) * L::BB, (u0 + u) % UPB, a.kgrid, q, dl, ml);
-#pragma unroll
-                    for (int t = 0; t < NT; t++) {
-                        const uint4 xa = sm.q[t][0][u], xb = sm.q[t][1][u];
-                        const float d = sm.d[t][u];
-                        int s0 = __dp4a((int)q[0], (int)xa.x, 0), s1 = 0;
-                        s0 = __dp4a((int)q[1], (int)xa.y, s0);
-                        s0 = __dp4a((int)q[2], (int)xa.z, s0);
-                        s0 = __dp4a((int)q[3], (int)xa.w, s0);
-                        if (!L::G16) s1 = s0;
-                        s1 = __dp4a((int)q[4], (int)xb.x, s1);
-                        s1 = __dp4a((int)q[5], (int)xb.y, s1);
-                        s1 = __dp4a((int)q[6], (int)xb.z, s1);
-                        s1 = __dp4a((int)q[7], (int)xb.w, s1);
-                        if (L::G16) acc[r][t] = __fmaf_rn(dl[0] * d, (float)s0, acc[r][t]);
-                        acc[r][t] = __fmaf_rn(dl[1] * d, (float)s1, acc[r][t]);
-                        if constexpr (SUMS >= 1) acc[r][t] = __fmaf_rn(-ml[0], sm.s[0][t][u], acc[r][t]);
-                        if constexpr (SUMS == 2) acc[r][t] = __fmaf_rn(-ml[1], sm.s[1][t][u], acc[r][t]);
-                    }
-                }
-            }
+    for (int p = 0; p < PF; p++) load(raw[p]);
+
+    for (int i = tid; i < NT * 2 * units; i += blockDim.x) {
+        const int h = i & 1, k = i >> 1, t = k / units, u = k - t * units;
+        uint4 q = make_uint4(0, 0, 0, 0);
+        float d = 0.0f;
+        if (t < cnt) {
+            const int slot = a.order ? __ldg(a.order + ch.lo + t) : ch.lo + t;
+            const uint8_t* b = a.x + (slot / a.x_div) * a.x_row + (int64_t)u * 34;
+            q = ld_16b(b + 2 + 16 * h);
+            d = h2f(ld_u16<1>(b));
+        }
+        xq[(t * 2 + h) * units + u] = q;
+        if (h == 0) xd[t * units + u] = d;
+        if constexpr (SUMS == 2) xs[(h * NT + t) * units + u] = d * (float)sum16(q);
+        if constexpr (SUMS == 1) {
+            // the other half's sum, computed again rather than exchanged: lanes may have left the loop
+            const int o = t < cnt ? sum16(ld_16b(a.x + ((a.order ? __ldg(a.order + ch.lo + t) : ch.lo + t) / a.x_div) * a.x_row + (int64_t)u * 34 + 2 + 16 * (h ^ 1))) : 0;
+            if (h == 0) xs[t * units + u] = d * (float)(sum16(q) + o);
         }
     }
+    __syncthreads();
+
+    float acc[NT];
 #pragma unroll
-    for (int r = 0; r < FEW_ROWS; r++) {
-        if (n0 + r >= a.n) break;
+    for (int t = 0; t < NT; t++) acc[t] = 0.0f;
+    int cr = 0, ci = 0;  // row and step at hand
+    const int steps = rows > 0 ? rows * iters : 0;
+    for (int s = 0; s < steps; s += PF) {
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
-            float v = acc[r][t];
+        for (int p = 0; p < PF; p++) {
+            if (s + p >= steps) break;
+            uint32_t q[8];
+            float dl[2], ml[2];
+            const bool live = ci < full || tail;
+            const int cu = ci * 32 + lane;
+            if (live) L::levels(raw[p], j, a.kgrid, q, dl, ml);
+            load(raw[p]);
+            if (live) {
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-            if (lane == 0 && t < cnt) {
-                const int64_t slot = a.order ? __ldg(a.order + ch.lo + t) : ch.lo + t;
-                if (a.part) a.part[slot * a.n + n0 + r] = v;
-                else store_val(a.out, slot * a.out_stride + n0 + r, a.out_type, v);
+                for (int t = 0; t < NT; t++) {
+                    const uint4 xa = xq[(2 * t) * units + cu], xb = xq[(2 * t + 1) * units + cu];
+                    const float d = xd[t * units + cu];
+                    int s0 = __dp4a((int)q[0], (int)xa.x, 0), s1 = 0;
+                    s0 = __dp4a((int)q[1], (int)xa.y, s0);
+                    s0 = __dp4a((int)q[2], (int)xa.z, s0);
+                    s0 = __dp4a((int)q[3], (int)xa.w, s0);
+                    if (!L::G16) s1 = s0;
+                    s1 = __dp4a((int)q[4], (int)xb.x, s1);
+                    s1 = __dp4a((int)q[5], (int)xb.y, s1);
+                    s1 = __dp4a((int)q[6], (int)xb.z, s1);
+                    s1 = __dp4a((int)q[7], (int)xb.w, s1);
+                    if (L::G16) acc[t] = __fmaf_rn(dl[0] * d, (float)s0, acc[t]);
+                    acc[t] = __fmaf_rn(dl[1] * d, (float)s1, acc[t]);
+                    if constexpr (SUMS >= 1) acc[t] = __fmaf_rn(-ml[0], xs[t * units + cu], acc[t]);
+                    if constexpr (SUMS == 2) acc[t] = __fmaf_rn(-ml[1], xs[(NT + t) * units + cu], acc[t]);
+                }
+            }
+            if (++ci == iters) {  // the row's end
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    float v = acc[t];
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+                    if (lane == 0 && t < cnt) put(cr, t, v);
+                    acc[t] = 0.0f;
+                }
+                ci = 0;
+                cr++;
             }
         }
     }
@@ -111,9 +141,22 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) few_kernel(MmArgs a) {
 template <int T, int NT>
 cudaError_t launch_few_t(const MmArgs& a, const LaunchCtx& ctx) {
     const int64_t chunks = max_chunks(a, NT);
-    if (chunks > 65535) return cudaErrorInvalidConfiguration;
-    const dim3 grid((unsigned)((a.n + FEW_WARPS * FEW_ROWS - 1) / (FEW_WARPS * FEW_ROWS)), (unsigned)chunks);
-    few_kernel<T, NT><<<grid, 32 * FEW_WARPS, 0, ctx.stream>>>(a);
+    const int bytes = FewCfg<T, NT>::bytes(a.units);
+    if (chunks > 65535 || bytes > FEW_SMEM_MAX) return cudaErrorInvalidConfiguration;
+    cudaError_t e = cudaFuncSetAttribute(few_kernel<T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_SMEM_MAX);
+    if (e != cudaSuccess) return e;
+    // Activations beyond a quarter of an SM's shared memory: fewer CTAs fit, with 16 warps each.
+    const int warps = bytes <= 48 * 1024 ? 8 : 16;
+    // Rows per warp such that the CTAs of all chunks fit the SMs at once: one wave of equal shares.
+    static const int regs = [] {
+        cudaFuncAttributes f;
+        return cudaFuncGetAttributes(&f, few_kernel<T, NT>) == cudaSuccess ? (f.numRegs + 7) / 8 * 8 : 128;
+    }();
+    const int per_sm = std::max(1, std::min({65536 / (regs * 32 * warps), 64 / warps, 227 * 1024 / (bytes + 1024)}));
+    const int64_t ctas = std::max<int64_t>(1, (int64_t)per_sm * ctx.num_sms / chunks);
+    const int64_t rpw = std::min<int64_t>(16, (a.n + ctas * warps - 1) / (ctas * warps));
+    const dim3 grid((unsigned)((a.n + warps * rpw - 1) / (warps * rpw)), (unsigned)chunks);
+    few_kernel<T, NT><<<grid, 32 * warps, bytes, ctx.stream>>>(a, (int)rpw);
     return cudaGetLastError();
 }
 

@@ -69,7 +69,7 @@ struct TileCfg {
 __device__ __forceinline__ int scale_pos(int row) { return (row & ~15) | ((row & 7) << 1) | ((row >> 3) & 1); }
 
 template <int T, int BN>
-__global__ void __launch_bounds__(TILE_THREADS, 2) tile_kernel(MmArgs a) {
+__global__ void __launch_bounds__(TILE_THREADS, BN == 128 ? 1 : 2) tile_kernel(MmArgs a) {
     using L = Lv<T>;
     using C = TileCfg<T, BN>;
     constexpr int UPB = L::QK / 32, H = C::H, SUMS = C::SUMS, MT = C::MT, NT = C::NT;
@@ -97,34 +97,34 @@ __global__ void __launch_bounds__(TILE_THREADS, 2) tile_kernel(MmArgs a) {
 #pragma unroll
         for (int j = 0; j < NT; j++) acc[i][j][0] = acc[i][j][1] = 0ull;
 
-    // weight items of a step: (row, unit), 2 per thread; 4 adjacent lanes one row
-    uint32_t wq[2][8];
-    float wdl[2][2], wml[2][2];
-    auto fetch_w = [&](int step) {
+    // weight items of a step: (row, unit), 2 per thread; 4 adjacent lanes one row. The block
+    // bytes are loaded a step ahead and unpacked behind the products that cover their latency.
+    uint32_t raw[2][L::WORDS];
+    auto load_w = [&](int step) {
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             const int item = tid + i * TILE_THREADS, row = item >> 2, u = step * TU + (item & 3);
-            if (n0 + row < a.n && u < a.units) {
-                L::template unit<L::MAXAL>(w + (int64_t)(n0 + row) * a.w_row + (int64_t)(u / UPB) * L::BB, u % UPB, a.kgrid, wq[i], wdl[i], wml[i]);
-            } else {
+            if (n0 + row < a.n && u < a.units)
+                L::template load<L::MAXAL>(w + (int64_t)(n0 + row) * a.w_row + (int64_t)(u / UPB) * L::BB, u % UPB, raw[i]);
+            else
 #pragma unroll
-                for (int j = 0; j < 8; j++) wq[i][j] = 0;
-                wdl[i][0] = wdl[i][1] = wml[i][0] = wml[i][1] = 0.0f;
-            }
+                for (int j = 0; j < L::WORDS; j++) raw[i][j] = 0;  // zero scales
         }
     };
-    auto put_w = [&](uint8_t* st) {
+    auto put_w = [&](int step, uint8_t* st) {
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             const int item = tid + i * TILE_THREADS, row = item >> 2, u = item & 3;
+            uint32_t q[8];
+            float dl[2], ml[2];
+            L::levels(raw[i], (step * TU + u) % UPB, a.kgrid, q, dl, ml);
 #pragma unroll
             for (int h = 0; h < 2; h++)
-                *reinterpret_cast<uint4*>(st + row * 128 + (((2 * u + h) ^ (row & 7)) << 4)) =
-                    make_uint4(wq[i][4 * h], wq[i][4 * h + 1], wq[i][4 * h + 2], wq[i][4 * h + 3]);
+                *reinterpret_cast<uint4*>(st + row * 128 + (((2 * u + h) ^ (row & 7)) << 4)) = make_uint4(q[4 * h], q[4 * h + 1], q[4 * h + 2], q[4 * h + 3]);
 #pragma unroll
             for (int h = 0; h < H; h++) {
-                reinterpret_cast<f32x2*>(st + C::OFF_DL)[(u * H + h) * TM + scale_pos(row)] = f2_splat(wdl[i][h]);
-                if constexpr (SUMS > 0) reinterpret_cast<f32x2*>(st + C::OFF_ML)[(u * H + h) * TM + scale_pos(row)] = f2_splat(-wml[i][h]);
+                reinterpret_cast<f32x2*>(st + C::OFF_DL)[(u * H + h) * TM + scale_pos(row)] = f2_splat(dl[h]);
+                if constexpr (SUMS > 0) reinterpret_cast<f32x2*>(st + C::OFF_ML)[(u * H + h) * TM + scale_pos(row)] = f2_splat(-ml[h]);
             }
         }
     };
@@ -156,8 +156,8 @@ __global__ void __launch_bounds__(TILE_THREADS, 2) tile_kernel(MmArgs a) {
 
     if (real && k0 < k1) {
         copy_x(k0, smem);
-        fetch_w(k0);
-        put_w(smem);
+        load_w(k0);
+        put_w(k0, smem);
         cp_wait_all();
         __syncthreads();
         const f32x2 nmagic = f2_splat(-12582912.0f);
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 2) tile_kernel(MmArgs a) {
             const bool more = k + 1 < k1;
             if (more) {
                 copy_x(k + 1, nx);
-                fetch_w(k + 1);
+                load_w(k + 1);
             }
             const uint32_t base = smem_u32(st);
 #pragma unroll
@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 2) tile_kernel(MmArgs a) {
                         }
                 }
             }
-            if (more) put_w(nx);
+            if (more) put_w(k + 1, nx);
             cp_wait_all();
             __syncthreads();
         }
