@@ -439,52 +439,34 @@ int block_align(int type) {
     }
 }
 
-bool has_min(int type) {
-    return type == qs::QS_Q4_1 || type == qs::QS_Q5_1 || type == qs::QS_Q2_K || type == qs::QS_Q4_K || type == qs::QS_Q5_K;
-}
-
-// How a product runs: which kernel, its tile, how often the row is split, and the workspace.
+// How a product runs: which kernel, its tile, over how many CTAs a tile's rows are split.
 struct MmPlan {
     bool few;
-    int bn, splits, units, units_pad, planes;
-    int64_t xq_off, xd_off, part_off, bytes;
-    bool part;
+    int bn, splits;
+    int64_t bytes;  // workspace
 };
 
-// slots: output rows before a weighted sum; groups: weight matrices that share them; x_rows:
-// activation rows. SMs: the tile kernel keeps two CTAs on each of a B200's 148.
-MmPlan mm_plan(int type, int64_t n, int64_t k, int64_t slots, int64_t groups, int64_t x_rows, bool sum) {
+// slots: output rows before a weighted sum; groups: weight matrices that share them. The tile
+// kernel keeps one CTA on each of a B200's 148 SMs.
+MmPlan mm_plan(int64_t n, int64_t k, int64_t slots, int64_t groups, bool sum) {
     MmPlan p;
-    memset(&p, 0, sizeof(p));
-    p.units = (int)(k / 32);
-    p.units_pad = (p.units + 3) / 4 * 4;
-    p.planes = 1 + (has_min(type) ? (type == qs::QS_Q2_K ? 2 : 1) : 0);
-    p.splits = 1;
-    const int64_t avg = (slots + groups - 1) / groups;
+    const int64_t avg = (slots + groups - 1) / groups, steps = (k + 255) / 256;
     // rows that the small kernel can not hold go to the tiles whatever their number
-    p.few = (groups == 1 ? slots <= qs::FEW_SLOTS : avg <= 4) && (int64_t)p.units * qs::FEW_SLOTS * qs::FEW_UNIT_MAX <= qs::FEW_SMEM_MAX;
-    if (!p.few) {
-        p.bn = avg <= 32 ? 32 : avg <= 64 ? 64 : 128;
-        const int64_t chunks = groups == 1 ? (slots + p.bn - 1) / p.bn : slots / p.bn + (groups < slots ? groups : slots) / 2 + 1;
-        const int64_t tiles = (n + 127) / 128 * chunks, steps = p.units_pad / 4;
-        if (tiles < 2 * 148) {
-            int64_t s = (2 * 148 + tiles - 1) / tiles;
-            if (s > steps / 4) s = steps / 4;  // 4 steps at least: shorter ones cost more to join than they gain
-            if (s > 1) {
-                const int64_t per = (steps + s - 1) / s;
-                p.splits = (int)((steps + per - 1) / per);
-            }
+    p.few = (groups == 1 ? slots <= qs::FEW_SLOTS : avg <= 4) && k / 32 * qs::FEW_SLOTS * qs::FEW_UNIT_MAX <= qs::FEW_SMEM_MAX;
+    p.bn = avg <= 32 ? 32 : avg <= 64 ? 64 : 128;
+    p.splits = 1;
+    const int64_t chunks = groups == 1 ? (slots + p.bn - 1) / p.bn : slots / p.bn + (groups < slots ? groups : slots) / 2 + 1;
+    const int64_t tiles = (n + 127) / 128 * chunks;
+    if (tiles > 0 && tiles < 148) {
+        int64_t s = 148 / tiles;
+        if (s > 8) s = 8;                  // a cluster
+        if (s > steps / 2) s = steps / 2;  // two steps each at least
+        if (s > 1) {
+            const int64_t per = (steps + s - 1) / s;
+            p.splits = (int)((steps + per - 1) / per);
         }
     }
-    p.part = sum || p.splits > 1;
-    int64_t at = 0;
-    auto take = [&](int64_t b) { const int64_t o = at; at += (b + 255) / 256 * 256; return o; };
-    if (!p.few) {
-        p.xq_off = take(x_rows * p.units_pad * 32);
-        p.xd_off = take(x_rows * p.units_pad * 4 * p.planes);
-    }
-    if (p.part) p.part_off = take((int64_t)p.splits * slots * n * 4);
-    p.bytes = at;
+    p.bytes = sum ? slots * n * 4 : 0;
     return p;
 }
 
@@ -517,27 +499,13 @@ int check_mm_operands(const TypeInfo* ti, const void* w, int64_t w_row_bytes, in
     return QS_OK;
 }
 
-// Fill the kernel call from the plan and run it.
-int run_mm(int ggml_type, const MmPlan& p, qs::MmArgs& a, int64_t x_rows, int per_out, const float* weights, const int* ids, void* workspace,
+int run_mm(int ggml_type, const MmPlan& p, qs::MmArgs& a, int64_t k, int top_k, const float* weights, const int* ids, void* workspace,
            const qs::LaunchCtx& ctx) {
-    uint8_t* ws = static_cast<uint8_t*>(workspace);
-    a.units = p.units;
-    a.units_pad = p.units_pad;
+    a.units = (int)(k / 32);
     a.splits = p.splits;
-    a.part = p.part ? reinterpret_cast<float*>(ws + p.part_off) : nullptr;
-    a.x_plane = x_rows * p.units_pad;
-    cudaError_t e;
-    if (p.few) {
-        e = qs::launch_mm_few(ggml_type, a, ctx);
-    } else {
-        int8_t* xq = reinterpret_cast<int8_t*>(ws + p.xq_off);
-        float* xd = reinterpret_cast<float*>(ws + p.xd_off);
-        a.xq = xq;
-        a.xd = xd;
-        e = qs::launch_mm_pack(a, (int)x_rows, xq, xd, p.planes, ctx);
-        if (e == cudaSuccess) e = qs::launch_mm_tile(ggml_type, a, p.bn, ctx);
-    }
-    if (e == cudaSuccess && p.part) e = qs::launch_mm_finish(a, per_out, weights, ids, ctx);
+    a.part = weights ? static_cast<float*>(workspace) : nullptr;
+    cudaError_t e = p.few ? qs::launch_mm_few(ggml_type, a, ctx) : qs::launch_mm_tile(ggml_type, a, p.bn, ctx);
+    if (e == cudaSuccess && weights) e = qs::launch_mm_sum(a, top_k, weights, ids, ctx);
     return e == cudaSuccess ? QS_OK : cuda_fail(e, "matmul launch");
 }
 
@@ -654,7 +622,7 @@ QS_API int qs_expert_plan(const int32_t* ids, int64_t n_slots, int n_experts, in
 QS_API int qs_matmul_workspace(int ggml_type, int64_t n, int64_t k, int64_t n_rows, int64_t* bytes) {
     const TypeInfo* ti;
     if (int rc = check_mm(ggml_type, n, k, n_rows, 1, &ti)) return rc;
-    if (bytes) *bytes = n_rows ? mm_plan(ggml_type, n, k, n_rows, 1, n_rows, false).bytes : 0;
+    if (bytes) *bytes = mm_plan(n, k, n_rows, 1, false).bytes;
     return QS_OK;
 }
 
@@ -665,7 +633,7 @@ QS_API int qs_matmul(int ggml_type, const void* w, int64_t w_row_bytes, int64_t 
     if (rc) return rc;
     if (n_rows == 0) return QS_OK;
     if ((rc = check_mm_operands(ti, w, w_row_bytes, k, x, x_row_bytes, out, out_type, out_row_stride, n))) return rc;
-    const MmPlan p = mm_plan(ggml_type, n, k, n_rows, 1, n_rows, false);
+    const MmPlan p = mm_plan(n, k, n_rows, 1, false);
     if ((rc = check_workspace(workspace, workspace_bytes, p.bytes))) return rc;
     CurrentContextGuard keep;
     int device;
@@ -687,7 +655,7 @@ QS_API int qs_matmul(int ggml_type, const void* w, int64_t w_row_bytes, int64_t 
     a.out_stride = out_row_stride;
     a.out_type = out_type;
     a.kgrid = qs::iq_kgrid(d->iq, ggml_type);
-    return run_mm(ggml_type, p, a, n_rows, 1, nullptr, nullptr, workspace, qs::LaunchCtx{static_cast<cudaStream_t>(stream), device, d->num_sms});
+    return run_mm(ggml_type, p, a, k, 1, nullptr, nullptr, workspace, qs::LaunchCtx{static_cast<cudaStream_t>(stream), device, d->num_sms});
 }
 
 QS_API int qs_matmul_experts_workspace(int ggml_type, int n_experts, int64_t n, int64_t k, int64_t n_tokens, int top_k, int x_per_slot, int sum,
@@ -696,7 +664,7 @@ QS_API int qs_matmul_experts_workspace(int ggml_type, int n_experts, int64_t n, 
     if (n_experts < 1 || n_experts > QS_MAX_EXPERTS) return fail(QS_EINVAL, "%d experts are not in 1 .. %d", n_experts, QS_MAX_EXPERTS);
     if (top_k < 1 || top_k > QS_MAX_EXPERTS) return fail(QS_EINVAL, "%d experts per token are not in 1 .. %d", top_k, QS_MAX_EXPERTS);
     if (int rc = check_mm(ggml_type, n, k, n_tokens, top_k, &ti)) return rc;
-    if (bytes) *bytes = n_tokens ? mm_plan(ggml_type, n, k, n_tokens * top_k, n_experts, x_per_slot ? n_tokens * top_k : n_tokens, sum != 0).bytes : 0;
+    if (bytes) *bytes = mm_plan(n, k, n_tokens * top_k, n_experts, sum != 0).bytes;
     return QS_OK;
 }
 
@@ -716,8 +684,8 @@ QS_API int qs_matmul_experts(int ggml_type, const void* w, int64_t w_row_bytes, 
     if (!ids || !order || !offsets) return fail(QS_EINVAL, "null ids, order or offsets");
     if (!aligned(ids, 4) || !aligned(order, 4) || !aligned(offsets, 4) || (weights && !aligned(weights, 4)))
         return fail(QS_EINVAL, "a pointer is not aligned to its elements");
-    const int64_t slots = n_tokens * top_k, x_rows = x_per_slot ? slots : n_tokens;
-    const MmPlan p = mm_plan(ggml_type, n, k, slots, n_experts, x_rows, weights != nullptr);
+    const int64_t slots = n_tokens * top_k;
+    const MmPlan p = mm_plan(n, k, slots, n_experts, weights != nullptr);
     if ((rc = check_workspace(workspace, workspace_bytes, p.bytes))) return rc;
     CurrentContextGuard keep;
     int device;
@@ -744,7 +712,7 @@ QS_API int qs_matmul_experts(int ggml_type, const void* w, int64_t w_row_bytes, 
     a.out_stride = out_row_stride;
     a.out_type = out_type;
     a.kgrid = qs::iq_kgrid(d->iq, ggml_type);
-    return run_mm(ggml_type, p, a, x_rows, weights ? top_k : 1, weights, weights ? ids : nullptr, workspace,
+    return run_mm(ggml_type, p, a, k, top_k, weights, ids, workspace,
                   qs::LaunchCtx{static_cast<cudaStream_t>(stream), device, d->num_sms});
 }
 

@@ -14,49 +14,56 @@
 
 namespace qs {
 
+// Global memory through the read-only path, shared memory (SM) plainly.
+template <bool SM, class V>
+__device__ __forceinline__ V ld_v(const V* p) {
+    if constexpr (SM) return *p;
+    else return __ldg(p);
+}
+
 // N words at any address, little-endian. AL: the alignment that is known; below 4 the aligned
 // words that hold the bytes are loaded and shifted (none of them lies wholly outside the bytes).
-template <int N, int AL>
+template <int N, int AL, bool SM = false>
 __device__ __forceinline__ void ld_words(const uint8_t* p, uint32_t* w) {
     if constexpr (AL >= 16 && N % 4 == 0) {
 #pragma unroll
         for (int i = 0; i < N / 4; i++) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i);
+            const uint4 v = ld_v<SM>(reinterpret_cast<const uint4*>(p) + i);
             w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
         }
     } else if constexpr (AL >= 8 && N % 2 == 0) {
 #pragma unroll
         for (int i = 0; i < N / 2; i++) {
-            const uint2 v = __ldg(reinterpret_cast<const uint2*>(p) + i);
+            const uint2 v = ld_v<SM>(reinterpret_cast<const uint2*>(p) + i);
             w[2 * i] = v.x; w[2 * i + 1] = v.y;
         }
     } else if constexpr (AL >= 4) {
 #pragma unroll
-        for (int i = 0; i < N; i++) w[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
+        for (int i = 0; i < N; i++) w[i] = ld_v<SM>(reinterpret_cast<const uint32_t*>(p) + i);
     } else {
         const uint32_t off = (uint32_t)(uintptr_t)p & 3, sh = 8 * off;
         const uint32_t* a = reinterpret_cast<const uint32_t*>(p - off);
         uint32_t v[N + 1];
 #pragma unroll
-        for (int i = 0; i < N; i++) v[i] = __ldg(a + i);
-        v[N] = off ? __ldg(a + N) : 0u;
+        for (int i = 0; i < N; i++) v[i] = ld_v<SM>(a + i);
+        v[N] = off ? ld_v<SM>(a + N) : 0u;
 #pragma unroll
         for (int i = 0; i < N; i++) w[i] = __funnelshift_r(v[i], v[i + 1], sh);
     }
 }
-template <int AL>
+template <int AL, bool SM = false>
 __device__ __forceinline__ uint32_t ld_u16(const uint8_t* p) {
-    if constexpr (AL >= 2) return __ldg(reinterpret_cast<const unsigned short*>(p));
-    else return (uint32_t)__ldg(p) | ((uint32_t)__ldg(p + 1) << 8);
+    if constexpr (AL >= 2) return ld_v<SM>(reinterpret_cast<const unsigned short*>(p));
+    else return (uint32_t)ld_v<SM>(p) | ((uint32_t)ld_v<SM>(p + 1) << 8);
 }
 __device__ __forceinline__ float h2f(uint32_t bits) { return f16_val((uint16_t)bits); }
 // 4 bits -> 4 bytes of 0 / 1 (bit i -> byte i)
 __device__ __forceinline__ uint32_t bits_to_bytes(uint32_t b) { return ((b & 0xFu) * 0x00204081u) & 0x01010101u; }
-// bytes of w negated where the byte of m (0 / 1) is 1
-__device__ __forceinline__ uint32_t neg_bytes(uint32_t w, uint32_t m) {
-    const uint32_t full = m * 0xFFu;
-    return __vadd4(w ^ full, m);
-}
+// bytes of w (1 .. 127) negated where the byte of m (0 / 1) is 1: no byte carries into the next
+__device__ __forceinline__ uint32_t neg_bytes(uint32_t w, uint32_t m) { return (w ^ (m * 0xFFu)) + m; }
+// bytes (below 128) minus the bytes of b (up to 128) as int8: bit 7 set keeps every difference from
+// borrowing, and is then taken back
+__device__ __forceinline__ uint32_t sub_bytes(uint32_t w, uint32_t b) { return ((w | 0x80808080u) - b) ^ 0x80808080u; }
 
 template <int T> struct Lv;
 
@@ -65,18 +72,18 @@ template <> struct Lv<QS_Q4_0> {
     static constexpr bool G16 = false, HASMIN = false, SIGNED = true;
     static constexpr int WORDS = 5, D = 0, M = 0;
     static constexpr float BD = 8.0f, BM = 0.0f;
-    template <int AL>
+    template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int, uint32_t* r) {
-        ld_words<4, 1>(b + 2, r);
-        r[4] = ld_u16<AL>(b);
+        ld_words<4, 1, SM>(b + 2, r);
+        r[4] = ld_u16<AL, SM>(b);
     }
     __device__ static void levels(const uint32_t* r, int, const uint16_t*, uint32_t* q, float* dl, float* ml) {
         dl[0] = dl[1] = h2f(r[4]);
         ml[0] = ml[1] = 0.0f;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            q[i] = __vsub4(r[i] & 0x0F0F0F0Fu, 0x08080808u);
-            q[4 + i] = __vsub4((r[i] >> 4) & 0x0F0F0F0Fu, 0x08080808u);
+            q[i] = sub_bytes(r[i] & 0x0F0F0F0Fu, 0x08080808u);
+            q[4 + i] = sub_bytes((r[i] >> 4) & 0x0F0F0F0Fu, 0x08080808u);
         }
     }
 };
@@ -86,9 +93,9 @@ template <> struct Lv<QS_Q4_1> {
     static constexpr bool G16 = false, HASMIN = true, SIGNED = false;
     static constexpr int WORDS = 5, D = 0, M = 2;
     static constexpr float BD = 15.0f, BM = 1.0f;
-    template <int AL>
+    template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int, uint32_t* r) {
-        ld_words<5, AL>(b, r);
+        ld_words<5, AL, SM>(b, r);
     }
     __device__ static void levels(const uint32_t* r, int, const uint16_t*, uint32_t* q, float* dl, float* ml) {
         dl[0] = dl[1] = h2f(r[0] & 0xFFFFu);
@@ -106,18 +113,18 @@ template <> struct Lv<QS_Q5_0> {
     static constexpr bool G16 = false, HASMIN = false, SIGNED = true;
     static constexpr int WORDS = 6, D = 0, M = 0;
     static constexpr float BD = 16.0f, BM = 0.0f;
-    template <int AL>
+    template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int, uint32_t* r) {
-        ld_words<5, 1>(b + 2, r);
-        r[5] = ld_u16<AL>(b);
+        ld_words<5, 1, SM>(b + 2, r);
+        r[5] = ld_u16<AL, SM>(b);
     }
     __device__ static void levels(const uint32_t* r, int, const uint16_t*, uint32_t* q, float* dl, float* ml) {
         dl[0] = dl[1] = h2f(r[5]);
         ml[0] = ml[1] = 0.0f;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            q[i] = __vsub4((r[1 + i] & 0x0F0F0F0Fu) | (bits_to_bytes(r[0] >> (4 * i)) << 4), 0x10101010u);
-            q[4 + i] = __vsub4(((r[1 + i] >> 4) & 0x0F0F0F0Fu) | (bits_to_bytes(r[0] >> (16 + 4 * i)) << 4), 0x10101010u);
+            q[i] = sub_bytes((r[1 + i] & 0x0F0F0F0Fu) | (bits_to_bytes(r[0] >> (4 * i)) << 4), 0x10101010u);
+            q[4 + i] = sub_bytes(((r[1 + i] >> 4) & 0x0F0F0F0Fu) | (bits_to_bytes(r[0] >> (16 + 4 * i)) << 4), 0x10101010u);
         }
     }
 };
@@ -127,9 +134,9 @@ template <> struct Lv<QS_Q5_1> {
     static constexpr bool G16 = false, HASMIN = true, SIGNED = false;
     static constexpr int WORDS = 6, D = 0, M = 2;
     static constexpr float BD = 31.0f, BM = 1.0f;
-    template <int AL>
+    template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int, uint32_t* r) {
-        ld_words<6, AL>(b, r);
+        ld_words<6, AL, SM>(b, r);
     }
     __device__ static void levels(const uint32_t* r, int, const uint16_t*, uint32_t* q, float* dl, float* ml) {
         dl[0] = dl[1] = h2f(r[0] & 0xFFFFu);
@@ -147,10 +154,10 @@ template <> struct Lv<QS_Q8_0> {
     static constexpr bool G16 = false, HASMIN = false, SIGNED = true;
     static constexpr int WORDS = 9, D = 0, M = 0;
     static constexpr float BD = 128.0f, BM = 0.0f;
-    template <int AL>
+    template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int, uint32_t* r) {
-        ld_words<8, 1>(b + 2, r);
-        r[8] = ld_u16<AL>(b);
+        ld_words<8, 1, SM>(b + 2, r);
+        r[8] = ld_u16<AL, SM>(b);
     }
     __device__ static void levels(const uint32_t* r, int, const uint16_t*, uint32_t* q, float* dl, float* ml) {
         dl[0] = dl[1] = h2f(r[8]);
@@ -165,11 +172,11 @@ template <> struct Lv<QS_Q2_K> {
     static constexpr bool G16 = true, HASMIN = true, SIGNED = false;
     static constexpr int WORDS = 10, D = 80, M = 82;
     static constexpr float BD = 45.0f, BM = 15.0f;
-    template <int AL>
+    template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
-        ld_words<8, AL>(b + 16 + 32 * (j / 4), r);
-        ld_words<1, AL>(b + 80, r + 8);
-        r[9] = ld_u16<AL>(b + 2 * j);
+        ld_words<8, AL, SM>(b + 16 + 32 * (j / 4), r);
+        ld_words<1, AL, SM>(b + 80, r + 8);
+        r[9] = ld_u16<AL, SM>(b + 2 * j);
     }
     __device__ static void levels(const uint32_t* r, int j, const uint16_t*, uint32_t* q, float* dl, float* ml) {
         const float dd = h2f(r[8] & 0xFFFFu), dm = h2f(r[8] >> 16);
@@ -189,12 +196,12 @@ template <> struct Lv<QS_Q3_K> {
     static constexpr bool G16 = true, HASMIN = false, SIGNED = true;
     static constexpr int WORDS = 20, D = 108, M = 0;
     static constexpr float BD = 128.0f, BM = 0.0f;
-    template <int AL>
+    template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
-        ld_words<8, AL>(b + 32 + 32 * (j / 4), r);
-        ld_words<8, AL>(b, r + 8);
-        ld_words<3, 1>(b + 96, r + 16);
-        r[19] = ld_u16<AL>(b + 108);
+        ld_words<8, AL, SM>(b + 32 + 32 * (j / 4), r);
+        ld_words<8, AL, SM>(b, r + 8);
+        ld_words<3, 1, SM>(b + 96, r + 16);
+        r[19] = ld_u16<AL, SM>(b + 108);
     }
     __device__ static void levels(const uint32_t* r, int j, const uint16_t*, uint32_t* q, float* dl, float* ml) {
         // scale g = 2 j + h: low 4 bits in nibble g / 8 of byte g % 8, high 2 bits of byte 8 + g % 4
@@ -209,7 +216,7 @@ template <> struct Lv<QS_Q3_K> {
         }
 #pragma unroll
         for (int i = 0; i < 8; i++)
-            q[i] = __vsub4(((r[i] >> (2 * (j & 3))) & 0x03030303u) | (((r[8 + i] >> j) & 0x01010101u) << 2), 0x04040404u);
+            q[i] = sub_bytes(((r[i] >> (2 * (j & 3))) & 0x03030303u) | (((r[8 + i] >> j) & 0x01010101u) << 2), 0x04040404u);
     }
 };
 
@@ -226,10 +233,10 @@ template <> struct Lv<QS_Q4_K> {
     static constexpr bool G16 = false, HASMIN = true, SIGNED = false;
     static constexpr int WORDS = 12, D = 0, M = 2;
     static constexpr float BD = 945.0f, BM = 63.0f;
-    template <int AL>
+    template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
-        ld_words<4, AL>(b, r + 8);
-        ld_words<8, AL>(b + 16 + 32 * (j / 2), r);
+        ld_words<4, AL, SM>(b, r + 8);
+        ld_words<8, AL, SM>(b + 16 + 32 * (j / 2), r);
     }
     __device__ static void levels(const uint32_t* r, int j, const uint16_t*, uint32_t* q, float* dl, float* ml) {
         float sc, mn;
@@ -246,11 +253,11 @@ template <> struct Lv<QS_Q5_K> {
     static constexpr bool G16 = false, HASMIN = true, SIGNED = false;
     static constexpr int WORDS = 20, D = 0, M = 2;
     static constexpr float BD = 1953.0f, BM = 63.0f;
-    template <int AL>
+    template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
-        ld_words<4, AL>(b, r + 8);
-        ld_words<8, AL>(b + 16, r + 12);
-        ld_words<8, AL>(b + 48 + 32 * (j / 2), r);
+        ld_words<4, AL, SM>(b, r + 8);
+        ld_words<8, AL, SM>(b + 16, r + 12);
+        ld_words<8, AL, SM>(b + 48 + 32 * (j / 2), r);
     }
     __device__ static void levels(const uint32_t* r, int j, const uint16_t*, uint32_t* q, float* dl, float* ml) {
         float sc, mn;
@@ -268,12 +275,12 @@ template <> struct Lv<QS_Q6_K> {
     static constexpr bool G16 = true, HASMIN = false, SIGNED = true;
     static constexpr int WORDS = 18, D = 208, M = 0;
     static constexpr float BD = 4096.0f, BM = 0.0f;
-    template <int AL>
+    template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
-        ld_words<8, AL>(b + 64 * (j / 4) + 32 * (j & 1), r);
-        ld_words<8, AL>(b + 128 + 32 * (j / 4), r + 8);
-        r[16] = ld_u16<AL>(b + 208);
-        r[17] = ld_u16<AL>(b + 192 + 2 * j);
+        ld_words<8, AL, SM>(b + 64 * (j / 4) + 32 * (j & 1), r);
+        ld_words<8, AL, SM>(b + 128 + 32 * (j / 4), r + 8);
+        r[16] = ld_u16<AL, SM>(b + 208);
+        r[17] = ld_u16<AL, SM>(b + 192 + 2 * j);
     }
     __device__ static void levels(const uint32_t* r, int j, const uint16_t*, uint32_t* q, float* dl, float* ml) {
         // unit j: half c = j / 4, low nibbles of ql at 32 (j & 1) for j & 3 < 2, high ones for the rest
@@ -283,7 +290,7 @@ template <> struct Lv<QS_Q6_K> {
         ml[0] = ml[1] = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; i++)
-            q[i] = __vsub4(((r[i] >> (4 * ((j >> 1) & 1))) & 0x0F0F0F0Fu) | (((r[8 + i] >> (2 * (j & 3))) & 0x03030303u) << 4), 0x20202020u);
+            q[i] = sub_bytes(((r[i] >> (4 * ((j >> 1) & 1))) & 0x0F0F0F0Fu) | (((r[8 + i] >> (2 * (j & 3))) & 0x03030303u) << 4), 0x20202020u);
     }
 };
 
@@ -306,10 +313,10 @@ template <> struct Lv<QS_IQ2_XXS> {
     static constexpr bool G16 = false, HASMIN = false, SIGNED = true;
     static constexpr int WORDS = 3, D = 0, M = 0;
     static constexpr float BD = 167.0f, BM = 0.0f;
-    template <int AL>
+    template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
-        ld_words<2, 1>(b + 2 + 8 * j, r);
-        r[2] = ld_u16<AL>(b);
+        ld_words<2, 1, SM>(b + 2 + 8 * j, r);
+        r[2] = ld_u16<AL, SM>(b);
     }
     __device__ static void levels(const uint32_t* r, int, const uint16_t* kgrid, uint32_t* q, float* dl, float* ml) {
         dl[0] = dl[1] = (h2f(r[2]) * (0.5f + (float)(r[1] >> 28))) * 0.25f;
@@ -325,11 +332,11 @@ template <> struct Lv<QS_IQ2_XS> {
     static constexpr bool G16 = true, HASMIN = false, SIGNED = true;
     static constexpr int WORDS = 4, D = 0, M = 0;
     static constexpr float BD = 167.0f, BM = 0.0f;
-    template <int AL>
+    template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
-        ld_words<2, 1>(b + 2 + 8 * j, r);
-        r[2] = ld_u16<AL>(b);
-        r[3] = __ldg(b + 66 + j);
+        ld_words<2, 1, SM>(b + 2 + 8 * j, r);
+        r[2] = ld_u16<AL, SM>(b);
+        r[3] = ld_v<SM>(b + 66 + j);
     }
     __device__ static void levels(const uint32_t* r, int, const uint16_t* kgrid, uint32_t* q, float* dl, float* ml) {
         const float d = h2f(r[2]);
@@ -349,13 +356,13 @@ template <> struct Lv<QS_IQ2_S> {
     static constexpr bool G16 = true, HASMIN = false, SIGNED = true;
     static constexpr int WORDS = 5, D = 0, M = 0;
     static constexpr float BD = 167.0f, BM = 0.0f;
-    template <int AL>
+    template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
-        ld_words<1, 1>(b + 2 + 4 * j, r);
-        ld_words<1, 1>(b + 34 + 4 * j, r + 1);
-        r[2] = ld_u16<AL>(b);
-        r[3] = __ldg(b + 74 + j);
-        r[4] = __ldg(b + 66 + j);
+        ld_words<1, 1, SM>(b + 2 + 4 * j, r);
+        ld_words<1, 1, SM>(b + 34 + 4 * j, r + 1);
+        r[2] = ld_u16<AL, SM>(b);
+        r[3] = ld_v<SM>(b + 74 + j);
+        r[4] = ld_v<SM>(b + 66 + j);
     }
     __device__ static void levels(const uint32_t* r, int, const uint16_t* kgrid, uint32_t* q, float* dl, float* ml) {
         const float d = h2f(r[2]);
@@ -378,11 +385,11 @@ template <> struct Lv<QS_IQ3_XXS> {
     static constexpr bool G16 = false, HASMIN = false, SIGNED = true;
     static constexpr int WORDS = 4, D = 0, M = 0;
     static constexpr float BD = 481.0f, BM = 0.0f;
-    template <int AL>
+    template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
-        ld_words<2, 1>(b + 2 + 8 * j, r);
-        ld_words<1, 1>(b + 66 + 4 * j, r + 2);
-        r[3] = ld_u16<AL>(b);
+        ld_words<2, 1, SM>(b + 2 + 8 * j, r);
+        ld_words<1, 1, SM>(b + 66 + 4 * j, r + 2);
+        r[3] = ld_u16<AL, SM>(b);
     }
     __device__ static void levels(const uint32_t* r, int, const uint16_t* kgrid, uint32_t* q, float* dl, float* ml) {
         dl[0] = dl[1] = (h2f(r[3]) * (0.5f + (float)(r[2] >> 28))) * 0.5f;
@@ -400,13 +407,13 @@ template <> struct Lv<QS_IQ3_S> {
     static constexpr bool G16 = false, HASMIN = false, SIGNED = true;
     static constexpr int WORDS = 6, D = 0, M = 0;
     static constexpr float BD = 465.0f, BM = 0.0f;
-    template <int AL>
+    template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
-        ld_words<2, 1>(b + 2 + 8 * j, r);
-        ld_words<1, 1>(b + 74 + 4 * j, r + 2);
-        r[3] = ld_u16<AL>(b);
-        r[4] = __ldg(b + 66 + j);
-        r[5] = __ldg(b + 106 + j / 2);
+        ld_words<2, 1, SM>(b + 2 + 8 * j, r);
+        ld_words<1, 1, SM>(b + 74 + 4 * j, r + 2);
+        r[3] = ld_u16<AL, SM>(b);
+        r[4] = ld_v<SM>(b + 66 + j);
+        r[5] = ld_v<SM>(b + 106 + j / 2);
     }
     __device__ static void levels(const uint32_t* r, int j, const uint16_t* kgrid, uint32_t* q, float* dl, float* ml) {
         dl[0] = dl[1] = h2f(r[3]) * (float)(1u + 2u * ((r[5] >> (4 * (j & 1))) & 15u));
@@ -430,10 +437,10 @@ template <> struct Lv<QS_IQ4_XS> {
         const uint32_t m = ((n >> 3) & 0x01010101u) * 0xFFu;
         return (a & ~m) | (c & m);
     }
-    template <int AL>
+    template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
-        ld_words<2, AL>(b, r + 4);
-        ld_words<4, AL>(b + 8 + 16 * j, r);
+        ld_words<2, AL, SM>(b, r + 4);
+        ld_words<4, AL, SM>(b + 8 + 16 * j, r);
     }
     __device__ static void levels(const uint32_t* r, int j, const uint16_t*, uint32_t* q, float* dl, float* ml) {
         const uint32_t ls = (r[5] >> (4 * j)) & 15u, hs = (r[4] >> (16 + 2 * j)) & 3u;

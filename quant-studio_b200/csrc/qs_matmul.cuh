@@ -31,14 +31,9 @@ struct MmArgs {
     void* out;             // slot s, column c at s * out_stride + c
     int64_t out_stride;
     int out_type;
-    float* part;           // partial sums [split][slot][n] instead of out, or null
-    int splits;
+    float* part;           // float32 results [slot][n] instead of out, or null
+    int splits;            // CTAs that share a tile's rows (tiles only)
     const uint16_t* kgrid;
-    // activations laid out for the tiles (qs_matmul_tile.cu), rows of units_pad * 32 levels
-    const int8_t* xq;
-    const float* xd;       // [plane][row][units_pad]: scale, scale * sum of (half) levels
-    int64_t x_plane;       // elements between planes
-    int units_pad;         // a multiple of 4
 };
 
 struct Chunk {
@@ -116,10 +111,8 @@ __device__ __forceinline__ int sum16(const uint4& v) {
 constexpr int FEW_SMEM_MAX = 200 * 1024, FEW_SLOTS = 8, FEW_UNIT_MAX = 44;
 cudaError_t launch_mm_few(int type, const MmArgs& a, const LaunchCtx& ctx);
 cudaError_t launch_mm_tile(int type, const MmArgs& a, int bn, const LaunchCtx& ctx);
-// activations into a.xq / a.xd (rows of the activations, not slots)
-cudaError_t launch_mm_pack(const MmArgs& a, int rows, int8_t* xq, float* xd, int planes, const LaunchCtx& ctx);
-// out[token] = sum over the slots (ids >= 0) of weight * sum over the splits of the partials
-cudaError_t launch_mm_finish(const MmArgs& a, int per_out, const float* weights, const int* ids, const LaunchCtx& ctx);
+// out[token] = sum over its per_out slots that have an expert of weight * part
+cudaError_t launch_mm_sum(const MmArgs& a, int per_out, const float* weights, const int* ids, const LaunchCtx& ctx);
 
 #define QS_FOR_TYPES(X)                                                                                     \
     X(QS_Q4_0) X(QS_Q4_1) X(QS_Q5_0) X(QS_Q5_1) X(QS_Q8_0) X(QS_Q2_K) X(QS_Q3_K) X(QS_Q4_K) X(QS_Q5_K)      \

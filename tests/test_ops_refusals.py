@@ -58,8 +58,7 @@ def matmul(t=12, w=A, wr=144, n=8, k=256, x=A, xr=272, rows=2, out=A, ot=0, os=8
 
 @pytest.mark.parametrize("bad", [dict(k=0), dict(k=128), dict(k=1 << 31), dict(n=0), dict(n=1 << 31), dict(rows=-1), dict(rows=(1 << 20) + 1),
                                  dict(rows=1 << 20, n=1 << 19, os=1 << 19), dict(w=None), dict(x=None), dict(out=None), dict(ot=2),
-                                 dict(wr=128), dict(wr=152), dict(xr=271), dict(os=7), dict(w=A + 8), dict(out=A + 2),
-                                 dict(rows=9), dict(rows=9, ws=A, wb=100), dict(rows=9, ws=A + 8, wb=1 << 20), dict(rows=9, ws=None, wb=1 << 20)])
+                                 dict(wr=128), dict(wr=152), dict(xr=271), dict(os=7), dict(w=A + 8), dict(out=A + 2)])
 def test_matmul(bad):
     assert matmul(**bad) == E
 
@@ -70,7 +69,9 @@ def test_matmul_type():
     assert lib().qs_matmul_workspace(20, 8, 256, 1, ctypes.byref(n)) == _native.QS_ENOTSUP
     assert lib().qs_matmul_workspace(12, 8, 100, 1, ctypes.byref(n)) == E
     assert lib().qs_matmul_workspace(12, 8, 256, 1, ctypes.byref(n)) == OK and n.value == 0
-    assert lib().qs_matmul_workspace(12, 8, 256, 9, ctypes.byref(n)) == OK and n.value > 0
+    assert lib().qs_matmul_workspace(12, 8, 256, 0, ctypes.byref(n)) == OK and n.value == 0
+    assert lib().qs_matmul_experts_workspace(12, 4, 8, 256, 2, 2, 0, 0, ctypes.byref(n)) == OK and n.value == 0
+    assert lib().qs_matmul_experts_workspace(12, 4, 8, 256, 2, 2, 0, 1, ctypes.byref(n)) == OK and n.value == 2 * 2 * 8 * 4
 
 
 @pytest.mark.parametrize("t,al", [(12, 16), (13, 16), (7, 8), (23, 8), (3, 4), (10, 4), (2, 2), (14, 2), (18, 2)])
@@ -87,7 +88,7 @@ def experts(t=12, w=A, wr=144, we=144 * 8, e=4, n=8, k=256, x=A, xr=272, per=0, 
 
 @pytest.mark.parametrize("bad", [dict(e=0), dict(e=1025), dict(top=0), dict(top=1025), dict(tokens=-1), dict(tokens=1 << 20), dict(we=144 * 7),
                                  dict(we=144 * 8 + 8), dict(ids=None), dict(order=None), dict(off=None), dict(ids=A + 2), dict(wt=A + 2),
-                                 dict(wt=A), dict(wr=143), dict(xr=200), dict(os=4), dict(k=32), dict(ot=7)])
+                                 dict(wt=A), dict(wt=A, ws=A, wb=127), dict(wt=A, ws=A + 8, wb=128), dict(wt=A, wb=128), dict(wr=143), dict(xr=200), dict(os=4), dict(k=32), dict(ot=7)])
 def test_experts(bad):
     assert experts(**bad) == E
 
