@@ -54,6 +54,7 @@ struct DeviceState {
     bool ready = false;
     int num_sms = 0;
     qs::IqTables* iq = nullptr;
+    unsigned int* fault = nullptr;  // the fault word
     cudaMemPool_t pool = nullptr;  // scratch of qs_tensor_error; keeps its memory between calls
 };
 
@@ -70,6 +71,7 @@ int ensure_device(int device, DeviceState** out) {
         if (e != cudaSuccess) return cuda_fail(e, "cudaDeviceGetAttribute");
         e = qs::iq_tables_create(&d.iq);
         if (e != cudaSuccess) return cuda_fail(e, "uploading the lattice codebooks");
+        if ((e = qs::fault_word(&d.fault)) != cudaSuccess) return cuda_fail(e, "the fault word's address");
         cudaMemPoolProps props;
         memset(&props, 0, sizeof(props));
         props.allocType = cudaMemAllocationTypePinned;
@@ -439,34 +441,44 @@ int block_align(int type) {
     }
 }
 
+bool has_min(int type) {
+    return type == qs::QS_Q4_1 || type == qs::QS_Q5_1 || type == qs::QS_Q2_K || type == qs::QS_Q4_K || type == qs::QS_Q5_K;
+}
+
 // How a product runs: which kernel, its tile, over how many CTAs a tile's rows are split.
 struct MmPlan {
     bool few;
     int bn, splits;
-    int64_t bytes;  // workspace
+    int64_t part_off, bytes;  // workspace: laid-out activations, then the slots' results before a sum
 };
 
 // slots: output rows before a weighted sum; groups: weight matrices that share them. The tile
 // kernel keeps one CTA on each of a B200's 148 SMs.
-MmPlan mm_plan(int64_t n, int64_t k, int64_t slots, int64_t groups, bool sum) {
+MmPlan mm_plan(int type, int64_t n, int64_t k, int64_t slots, int64_t groups, bool experts, bool sum) {
     MmPlan p;
-    const int64_t avg = (slots + groups - 1) / groups, steps = (k + 255) / 256;
+    const int64_t avg = (slots + groups - 1) / groups, units = k / 32, stages = (units + 1) / 2;
     // rows that the small kernel can not hold go to the tiles whatever their number
-    p.few = (groups == 1 ? slots <= qs::FEW_SLOTS : avg <= 4) && k / 32 * qs::FEW_SLOTS * qs::FEW_UNIT_MAX <= qs::FEW_SMEM_MAX;
-    p.bn = avg <= 32 ? 32 : avg <= 64 ? 64 : 128;
+    p.few = (groups == 1 ? slots <= qs::FEW_SLOTS : avg <= 4) && units * qs::FEW_SLOTS * qs::FEW_UNIT_MAX <= qs::FEW_SMEM_MAX;
+    p.bn = avg <= 32 ? 32 : avg <= 64 ? 64 : avg <= 128 ? 128 : 256;
     p.splits = 1;
     const int64_t chunks = groups == 1 ? (slots + p.bn - 1) / p.bn : slots / p.bn + (groups < slots ? groups : slots) / 2 + 1;
     const int64_t tiles = (n + 127) / 128 * chunks;
     if (tiles > 0 && tiles < 148) {
         int64_t s = 148 / tiles;
-        if (s > 8) s = 8;                  // a cluster
-        if (s > steps / 2) s = steps / 2;  // two steps each at least
+        if (s > 8) s = 8;                    // a cluster
+        if (s > stages / 8) s = stages / 8;  // 8 stages each at least
         if (s > 1) {
-            const int64_t per = (steps + s - 1) / s;
-            p.splits = (int)((steps + per - 1) / per);
+            const int64_t per = (stages + s - 1) / s;
+            p.splits = (int)((stages + per - 1) / per);
         }
     }
-    p.bytes = sum ? slots * n * 4 : 0;
+    int64_t xp = 0;
+    if (!p.few) {
+        const int planes = !has_min(type) ? 1 : type == qs::QS_Q2_K ? 3 : 2;
+        xp = (qs::mm_tc_workspace(units, qs::max_chunks(experts, slots, groups, p.bn), p.bn, planes) + 255) / 256 * 256;
+    }
+    p.part_off = xp;
+    p.bytes = xp + (sum ? slots * n * 4 : 0);
     return p;
 }
 
@@ -503,8 +515,8 @@ int run_mm(int ggml_type, const MmPlan& p, qs::MmArgs& a, int64_t k, int top_k, 
            const qs::LaunchCtx& ctx) {
     a.units = (int)(k / 32);
     a.splits = p.splits;
-    a.part = weights ? static_cast<float*>(workspace) : nullptr;
-    cudaError_t e = p.few ? qs::launch_mm_few(ggml_type, a, ctx) : qs::launch_mm_tile(ggml_type, a, p.bn, ctx);
+    a.part = weights ? reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + p.part_off) : nullptr;
+    cudaError_t e = p.few ? qs::launch_mm_few(ggml_type, a, ctx) : qs::launch_mm_tc(ggml_type, a, p.bn, workspace, ctx);
     if (e == cudaSuccess && weights) e = qs::launch_mm_sum(a, top_k, weights, ids, ctx);
     return e == cudaSuccess ? QS_OK : cuda_fail(e, "matmul launch");
 }
@@ -622,7 +634,7 @@ QS_API int qs_expert_plan(const int32_t* ids, int64_t n_slots, int n_experts, in
 QS_API int qs_matmul_workspace(int ggml_type, int64_t n, int64_t k, int64_t n_rows, int64_t* bytes) {
     const TypeInfo* ti;
     if (int rc = check_mm(ggml_type, n, k, n_rows, 1, &ti)) return rc;
-    if (bytes) *bytes = mm_plan(n, k, n_rows, 1, false).bytes;
+    if (bytes) *bytes = mm_plan(ggml_type, n, k, n_rows, 1, false, false).bytes;
     return QS_OK;
 }
 
@@ -633,7 +645,7 @@ QS_API int qs_matmul(int ggml_type, const void* w, int64_t w_row_bytes, int64_t 
     if (rc) return rc;
     if (n_rows == 0) return QS_OK;
     if ((rc = check_mm_operands(ti, w, w_row_bytes, k, x, x_row_bytes, out, out_type, out_row_stride, n))) return rc;
-    const MmPlan p = mm_plan(n, k, n_rows, 1, false);
+    const MmPlan p = mm_plan(ggml_type, n, k, n_rows, 1, false, false);
     if ((rc = check_workspace(workspace, workspace_bytes, p.bytes))) return rc;
     CurrentContextGuard keep;
     int device;
@@ -655,6 +667,7 @@ QS_API int qs_matmul(int ggml_type, const void* w, int64_t w_row_bytes, int64_t 
     a.out_stride = out_row_stride;
     a.out_type = out_type;
     a.kgrid = qs::iq_kgrid(d->iq, ggml_type);
+    a.fault = d->fault;
     return run_mm(ggml_type, p, a, k, 1, nullptr, nullptr, workspace, qs::LaunchCtx{static_cast<cudaStream_t>(stream), device, d->num_sms});
 }
 
@@ -664,7 +677,7 @@ QS_API int qs_matmul_experts_workspace(int ggml_type, int n_experts, int64_t n, 
     if (n_experts < 1 || n_experts > QS_MAX_EXPERTS) return fail(QS_EINVAL, "%d experts are not in 1 .. %d", n_experts, QS_MAX_EXPERTS);
     if (top_k < 1 || top_k > QS_MAX_EXPERTS) return fail(QS_EINVAL, "%d experts per token are not in 1 .. %d", top_k, QS_MAX_EXPERTS);
     if (int rc = check_mm(ggml_type, n, k, n_tokens, top_k, &ti)) return rc;
-    if (bytes) *bytes = mm_plan(n, k, n_tokens * top_k, n_experts, sum != 0).bytes;
+    if (bytes) *bytes = mm_plan(ggml_type, n, k, n_tokens * top_k, n_experts, true, sum != 0).bytes;
     return QS_OK;
 }
 
@@ -685,7 +698,7 @@ QS_API int qs_matmul_experts(int ggml_type, const void* w, int64_t w_row_bytes, 
     if (!aligned(ids, 4) || !aligned(order, 4) || !aligned(offsets, 4) || (weights && !aligned(weights, 4)))
         return fail(QS_EINVAL, "a pointer is not aligned to its elements");
     const int64_t slots = n_tokens * top_k;
-    const MmPlan p = mm_plan(n, k, slots, n_experts, weights != nullptr);
+    const MmPlan p = mm_plan(ggml_type, n, k, slots, n_experts, true, weights != nullptr);
     if ((rc = check_workspace(workspace, workspace_bytes, p.bytes))) return rc;
     CurrentContextGuard keep;
     int device;
@@ -712,6 +725,7 @@ QS_API int qs_matmul_experts(int ggml_type, const void* w, int64_t w_row_bytes, 
     a.out_stride = out_row_stride;
     a.out_type = out_type;
     a.kgrid = qs::iq_kgrid(d->iq, ggml_type);
+    a.fault = d->fault;
     return run_mm(ggml_type, p, a, k, top_k, weights, ids, workspace,
                   qs::LaunchCtx{static_cast<cudaStream_t>(stream), device, d->num_sms});
 }

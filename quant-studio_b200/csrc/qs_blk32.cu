@@ -616,6 +616,13 @@ cudaError_t launch_blk32(int type, const QuantArgs& a, const LaunchCtx& ctx) {
     }
 }
 
+cudaError_t fault_word(unsigned int** out) {
+    void* p = nullptr;
+    const cudaError_t e = cudaGetSymbolAddress(&p, g_qs_fault_bits);
+    *out = static_cast<unsigned int*>(p);
+    return e;
+}
+
 cudaError_t read_fault_bits(unsigned int* bits, bool clear) {
     cudaError_t e = cudaMemcpyFromSymbol(bits, g_qs_fault_bits, sizeof(unsigned int));
     if (e != cudaSuccess || !clear || *bits == 0) return e;

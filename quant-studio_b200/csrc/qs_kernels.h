@@ -39,6 +39,8 @@ cudaError_t launch_blk32(int type, const QuantArgs& a, const LaunchCtx& ctx);
 // Fault word of the current device: bit 0 = a kernel gave up waiting for a bulk copy.
 // Synchronous; clears the word when `clear` and it is non-zero.
 cudaError_t read_fault_bits(unsigned int* bits, bool clear);
+// Address of that word on the current device.
+cudaError_t fault_word(unsigned int** out);
 cudaError_t launch_iq(int type, const QuantArgs& a, const LaunchCtx& ctx, const IqTables* t);
 cudaError_t iq_tables_create(IqTables** out);  // uploads the codebooks to the current device
 cudaError_t iq_tables_ensure(IqTables* t, int type);  // neighbour tables of type's grid, once

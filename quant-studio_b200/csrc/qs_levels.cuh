@@ -6,8 +6,9 @@
 // Lv<T>::load brings what unit j of a block needs into WORDS registers, Lv<T>::levels makes of
 // them its levels as 8 words (4 levels each, value order) and dl, ml of its two halves of 16
 // values; two steps, so that loads can run ahead. G16: the halves' scales differ; HASMIN: ml is
-// not always zero; SIGNED: levels are int8 (else 0 .. 31). dl and ml are exact: a float16
-// times a few scale bits. |weight| <= BD |d| + BM |m| with the float16 d at byte D, m at M.
+// not always zero; G16 formats also give d and the integer factors of its halves (base, subs:
+// dl[h] = base * sub[h]). SIGNED: levels are int8 (else 0 .. 31). dl and ml are exact: a float16
+// times a few scale bits.
 #pragma once
 
 #include "qs_kernels.h"
@@ -70,8 +71,7 @@ template <int T> struct Lv;
 template <> struct Lv<QS_Q4_0> {
     static constexpr int QK = 32, BB = 18, MAXAL = 2;
     static constexpr bool G16 = false, HASMIN = false, SIGNED = true;
-    static constexpr int WORDS = 5, D = 0, M = 0;
-    static constexpr float BD = 8.0f, BM = 0.0f;
+    static constexpr int WORDS = 5;
     template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int, uint32_t* r) {
         ld_words<4, 1, SM>(b + 2, r);
@@ -91,8 +91,7 @@ template <> struct Lv<QS_Q4_0> {
 template <> struct Lv<QS_Q4_1> {
     static constexpr int QK = 32, BB = 20, MAXAL = 4;
     static constexpr bool G16 = false, HASMIN = true, SIGNED = false;
-    static constexpr int WORDS = 5, D = 0, M = 2;
-    static constexpr float BD = 15.0f, BM = 1.0f;
+    static constexpr int WORDS = 5;
     template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int, uint32_t* r) {
         ld_words<5, AL, SM>(b, r);
@@ -111,8 +110,7 @@ template <> struct Lv<QS_Q4_1> {
 template <> struct Lv<QS_Q5_0> {
     static constexpr int QK = 32, BB = 22, MAXAL = 2;
     static constexpr bool G16 = false, HASMIN = false, SIGNED = true;
-    static constexpr int WORDS = 6, D = 0, M = 0;
-    static constexpr float BD = 16.0f, BM = 0.0f;
+    static constexpr int WORDS = 6;
     template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int, uint32_t* r) {
         ld_words<5, 1, SM>(b + 2, r);
@@ -132,8 +130,7 @@ template <> struct Lv<QS_Q5_0> {
 template <> struct Lv<QS_Q5_1> {
     static constexpr int QK = 32, BB = 24, MAXAL = 8;
     static constexpr bool G16 = false, HASMIN = true, SIGNED = false;
-    static constexpr int WORDS = 6, D = 0, M = 2;
-    static constexpr float BD = 31.0f, BM = 1.0f;
+    static constexpr int WORDS = 6;
     template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int, uint32_t* r) {
         ld_words<6, AL, SM>(b, r);
@@ -152,8 +149,7 @@ template <> struct Lv<QS_Q5_1> {
 template <> struct Lv<QS_Q8_0> {
     static constexpr int QK = 32, BB = 34, MAXAL = 2;
     static constexpr bool G16 = false, HASMIN = false, SIGNED = true;
-    static constexpr int WORDS = 9, D = 0, M = 0;
-    static constexpr float BD = 128.0f, BM = 0.0f;
+    static constexpr int WORDS = 9;
     template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int, uint32_t* r) {
         ld_words<8, 1, SM>(b + 2, r);
@@ -170,8 +166,7 @@ template <> struct Lv<QS_Q8_0> {
 template <> struct Lv<QS_Q2_K> {
     static constexpr int QK = 256, BB = 84, MAXAL = 4;
     static constexpr bool G16 = true, HASMIN = true, SIGNED = false;
-    static constexpr int WORDS = 10, D = 80, M = 82;
-    static constexpr float BD = 45.0f, BM = 15.0f;
+    static constexpr int WORDS = 10;
     template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
         ld_words<8, AL, SM>(b + 16 + 32 * (j / 4), r);
@@ -189,13 +184,14 @@ template <> struct Lv<QS_Q2_K> {
 #pragma unroll
         for (int i = 0; i < 8; i++) q[i] = (r[i] >> (2 * (j & 3))) & 0x03030303u;
     }
+    __device__ static float base(const uint32_t* r) { return h2f(r[8] & 0xFFFFu); }
+    __device__ static int sub(const uint32_t* r, int, int h) { return (int)((r[9] >> (8 * h)) & 15u); }
 };
 
 template <> struct Lv<QS_Q3_K> {
     static constexpr int QK = 256, BB = 110, MAXAL = 2;
     static constexpr bool G16 = true, HASMIN = false, SIGNED = true;
-    static constexpr int WORDS = 20, D = 108, M = 0;
-    static constexpr float BD = 128.0f, BM = 0.0f;
+    static constexpr int WORDS = 20;
     template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
         ld_words<8, AL, SM>(b + 32 + 32 * (j / 4), r);
@@ -204,19 +200,21 @@ template <> struct Lv<QS_Q3_K> {
         r[19] = ld_u16<AL, SM>(b + 108);
     }
     __device__ static void levels(const uint32_t* r, int j, const uint16_t*, uint32_t* q, float* dl, float* ml) {
-        // scale g = 2 j + h: low 4 bits in nibble g / 8 of byte g % 8, high 2 bits of byte 8 + g % 4
-        const float d = h2f(r[19]);
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const int g = 2 * j + h;
-            const uint32_t ls = ((g & 4 ? r[17] : r[16]) >> (8 * (g & 3) + 4 * (g >> 3))) & 15u;
-            const uint32_t hs = (r[18] >> (8 * (g & 3) + 2 * (g >> 2))) & 3u;
-            dl[h] = d * (float)((int)(ls | (hs << 4)) - 32);
+            dl[h] = base(r) * (float)sub(r, j, h);
             ml[h] = 0.0f;
         }
 #pragma unroll
         for (int i = 0; i < 8; i++)
             q[i] = sub_bytes(((r[i] >> (2 * (j & 3))) & 0x03030303u) | (((r[8 + i] >> j) & 0x01010101u) << 2), 0x04040404u);
+    }
+    __device__ static float base(const uint32_t* r) { return h2f(r[19]); }
+    __device__ static int sub(const uint32_t* r, int j, int h) {
+        // scale g = 2 j + h: low 4 bits in nibble g / 8 of byte g % 8, high 2 bits of byte 8 + g % 4
+        const int g = 2 * j + h;
+        const uint32_t ls = ((g & 4 ? r[17] : r[16]) >> (8 * (g & 3) + 4 * (g >> 3))) & 15u;
+        return (int)(ls | (((r[18] >> (8 * (g & 3) + 2 * (g >> 2))) & 3u) << 4)) - 32;
     }
 };
 
@@ -231,8 +229,7 @@ __device__ __forceinline__ void k4_scale_min(const uint32_t* s, int j, float& sc
 template <> struct Lv<QS_Q4_K> {
     static constexpr int QK = 256, BB = 144, MAXAL = 16;
     static constexpr bool G16 = false, HASMIN = true, SIGNED = false;
-    static constexpr int WORDS = 12, D = 0, M = 2;
-    static constexpr float BD = 945.0f, BM = 63.0f;
+    static constexpr int WORDS = 12;
     template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
         ld_words<4, AL, SM>(b, r + 8);
@@ -251,8 +248,7 @@ template <> struct Lv<QS_Q4_K> {
 template <> struct Lv<QS_Q5_K> {
     static constexpr int QK = 256, BB = 176, MAXAL = 16;
     static constexpr bool G16 = false, HASMIN = true, SIGNED = false;
-    static constexpr int WORDS = 20, D = 0, M = 2;
-    static constexpr float BD = 1953.0f, BM = 63.0f;
+    static constexpr int WORDS = 20;
     template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
         ld_words<4, AL, SM>(b, r + 8);
@@ -273,8 +269,7 @@ template <> struct Lv<QS_Q5_K> {
 template <> struct Lv<QS_Q6_K> {
     static constexpr int QK = 256, BB = 210, MAXAL = 2;
     static constexpr bool G16 = true, HASMIN = false, SIGNED = true;
-    static constexpr int WORDS = 18, D = 208, M = 0;
-    static constexpr float BD = 4096.0f, BM = 0.0f;
+    static constexpr int WORDS = 18;
     template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
         ld_words<8, AL, SM>(b + 64 * (j / 4) + 32 * (j & 1), r);
@@ -292,6 +287,8 @@ template <> struct Lv<QS_Q6_K> {
         for (int i = 0; i < 8; i++)
             q[i] = sub_bytes(((r[i] >> (4 * ((j >> 1) & 1))) & 0x0F0F0F0Fu) | (((r[8 + i] >> (2 * (j & 3))) & 0x03030303u) << 4), 0x20202020u);
     }
+    __device__ static float base(const uint32_t* r) { return h2f(r[16]); }
+    __device__ static int sub(const uint32_t* r, int, int h) { return (int)(int8_t)(r[17] >> (8 * h)); }
 };
 
 // four levels of an IQ2 code (2 bits each: 8, 25, 43) as bytes
@@ -311,8 +308,7 @@ __device__ __forceinline__ uint32_t sign8(uint32_t i) { return i | ((__popc(i) &
 template <> struct Lv<QS_IQ2_XXS> {
     static constexpr int QK = 256, BB = 66, MAXAL = 2;
     static constexpr bool G16 = false, HASMIN = false, SIGNED = true;
-    static constexpr int WORDS = 3, D = 0, M = 0;
-    static constexpr float BD = 167.0f, BM = 0.0f;
+    static constexpr int WORDS = 3;
     template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
         ld_words<2, 1, SM>(b + 2 + 8 * j, r);
@@ -330,8 +326,7 @@ template <> struct Lv<QS_IQ2_XXS> {
 template <> struct Lv<QS_IQ2_XS> {
     static constexpr int QK = 256, BB = 74, MAXAL = 2;
     static constexpr bool G16 = true, HASMIN = false, SIGNED = true;
-    static constexpr int WORDS = 4, D = 0, M = 0;
-    static constexpr float BD = 167.0f, BM = 0.0f;
+    static constexpr int WORDS = 4;
     template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
         ld_words<2, 1, SM>(b + 2 + 8 * j, r);
@@ -349,13 +344,14 @@ template <> struct Lv<QS_IQ2_XS> {
             iq2_signed(__ldg(kgrid + (c & 511u)), sign8(c >> 9), q + 2 * s);
         }
     }
+    __device__ static float base(const uint32_t* r) { return h2f(r[2]) * 0.125f; }
+    __device__ static int sub(const uint32_t* r, int, int h) { return 1 + 2 * (int)((r[3] >> (4 * h)) & 15u); }
 };
 
 template <> struct Lv<QS_IQ2_S> {
     static constexpr int QK = 256, BB = 82, MAXAL = 2;
     static constexpr bool G16 = true, HASMIN = false, SIGNED = true;
-    static constexpr int WORDS = 5, D = 0, M = 0;
-    static constexpr float BD = 167.0f, BM = 0.0f;
+    static constexpr int WORDS = 5;
     template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
         ld_words<1, 1, SM>(b + 2 + 4 * j, r);
@@ -373,6 +369,8 @@ template <> struct Lv<QS_IQ2_S> {
         for (int s = 0; s < 4; s++)
             iq2_signed(__ldg(kgrid + (((r[0] >> (8 * s)) & 0xFFu) | (((r[4] >> (2 * s)) & 3u) << 8))), (r[1] >> (8 * s)) & 0xFFu, q + 2 * s);
     }
+    __device__ static float base(const uint32_t* r) { return h2f(r[2]) * 0.125f; }
+    __device__ static int sub(const uint32_t* r, int, int h) { return 1 + 2 * (int)((r[3] >> (4 * h)) & 15u); }
 };
 
 // four levels of an IQ3 code (3 bits each): byte table lo (levels 0..3), hi (levels 4..7)
@@ -383,8 +381,7 @@ __device__ __forceinline__ uint32_t iq3_bytes(uint32_t c, uint32_t lo, uint32_t 
 template <> struct Lv<QS_IQ3_XXS> {
     static constexpr int QK = 256, BB = 98, MAXAL = 2;
     static constexpr bool G16 = false, HASMIN = false, SIGNED = true;
-    static constexpr int WORDS = 4, D = 0, M = 0;
-    static constexpr float BD = 481.0f, BM = 0.0f;
+    static constexpr int WORDS = 4;
     template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
         ld_words<2, 1, SM>(b + 2 + 8 * j, r);
@@ -405,8 +402,7 @@ template <> struct Lv<QS_IQ3_XXS> {
 template <> struct Lv<QS_IQ3_S> {
     static constexpr int QK = 256, BB = 110, MAXAL = 2;
     static constexpr bool G16 = false, HASMIN = false, SIGNED = true;
-    static constexpr int WORDS = 6, D = 0, M = 0;
-    static constexpr float BD = 465.0f, BM = 0.0f;
+    static constexpr int WORDS = 6;
     template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
         ld_words<2, 1, SM>(b + 2 + 8 * j, r);
@@ -428,8 +424,7 @@ template <> struct Lv<QS_IQ3_S> {
 template <> struct Lv<QS_IQ4_XS> {
     static constexpr int QK = 256, BB = 136, MAXAL = 8;
     static constexpr bool G16 = false, HASMIN = false, SIGNED = true;
-    static constexpr int WORDS = 6, D = 0, M = 0;
-    static constexpr float BD = 4064.0f, BM = 0.0f;
+    static constexpr int WORDS = 6;
     // the 16 level values, 4 to a word: -127 -104 -83 -65 | -49 -35 -22 -10 | 1 13 25 38 | 53 69 89 113
     __device__ static uint32_t value4(uint32_t n) {  // 4 nibbles (one per byte) -> their bytes
         const uint32_t lo = (n & 0x07u) | ((n & 0x0700u) >> 4) | ((n & 0x070000u) >> 8) | ((n & 0x07000000u) >> 12);

@@ -34,6 +34,7 @@ struct MmArgs {
     float* part;           // float32 results [slot][n] instead of out, or null
     int splits;            // CTAs that share a tile's rows (tiles only)
     const uint16_t* kgrid;
+    unsigned int* fault;   // the device's fault word
 };
 
 struct Chunk {
@@ -83,16 +84,39 @@ __device__ __forceinline__ Chunk find_chunk(const MmArgs& a, int c) {
 }
 
 // the number of chunks is at most this (it depends on the offsets, which the host does not read)
-inline int64_t max_chunks(const MmArgs& a, int c) {
-    if (!a.order) return ((int64_t)a.slots + c - 1) / c;
-    const int64_t groups = a.n_exp + 1 < a.slots ? a.n_exp + 1 : a.slots;
-    return c == 1 ? a.slots : a.slots / c + groups;
+inline int64_t max_chunks(bool ordered, int64_t slots, int64_t n_exp, int c) {
+    if (!ordered) return (slots + c - 1) / c;
+    const int64_t groups = n_exp + 1 < slots ? n_exp + 1 : slots;
+    return c == 1 ? slots : slots / c + groups;
 }
+inline int64_t max_chunks(const MmArgs& a, int c) { return max_chunks(a.order != nullptr, a.slots, a.n_exp, c); }
 
 __device__ __forceinline__ void store_val(void* p, int64_t i, int type, float v) {
     if (type == SRC_F32) static_cast<float*>(p)[i] = v;
     else if (type == SRC_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);
     else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+}
+
+// A slot's 128 columns from n0 on, 4 per lane, to element `at` of out; vec: all exist, 4-element aligned.
+__device__ __forceinline__ void store_row4(void* out, int64_t at, int type, float4 v, int lane, int n0, int n, bool vec) {
+    if (vec) {
+        if (type == SRC_F32) {
+            reinterpret_cast<float4*>(static_cast<float*>(out) + at)[lane] = v;
+        } else if (type == SRC_F16) {
+            const __half2 p = __floats2half2_rn(v.x, v.y), q = __floats2half2_rn(v.z, v.w);
+            reinterpret_cast<uint2*>(static_cast<__half*>(out) + at)[lane] =
+                make_uint2(*reinterpret_cast<const uint32_t*>(&p), *reinterpret_cast<const uint32_t*>(&q));
+        } else {
+            const __nv_bfloat162 p = __floats2bfloat162_rn(v.x, v.y), q = __floats2bfloat162_rn(v.z, v.w);
+            reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(out) + at)[lane] =
+                make_uint2(*reinterpret_cast<const uint32_t*>(&p), *reinterpret_cast<const uint32_t*>(&q));
+        }
+    } else {
+        const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+            if (n0 + 4 * lane + c < n) store_val(out, at + 4 * lane + c, type, e[c]);
+    }
 }
 
 // 16 bytes at any address
@@ -111,6 +135,10 @@ __device__ __forceinline__ int sum16(const uint4& v) {
 constexpr int FEW_SMEM_MAX = 200 * 1024, FEW_SLOTS = 8, FEW_UNIT_MAX = 44;
 cudaError_t launch_mm_few(int type, const MmArgs& a, const LaunchCtx& ctx);
 cudaError_t launch_mm_tile(int type, const MmArgs& a, int bn, const LaunchCtx& ctx);
+// tcgen05 tiles (qs_matmul_tc.cu): bytes of the laid-out activations at xp for `chunks` chunks of
+// bn slots; planes: 1, 2 with minima, 3 with minima per 16 values
+int64_t mm_tc_workspace(int64_t units, int64_t chunks, int bn, int planes);
+cudaError_t launch_mm_tc(int type, const MmArgs& a, int bn, void* xp, const LaunchCtx& ctx);
 // out[token] = sum over its per_out slots that have an expert of weight * part
 cudaError_t launch_mm_sum(const MmArgs& a, int per_out, const float* weights, const int* ids, const LaunchCtx& ctx);
 

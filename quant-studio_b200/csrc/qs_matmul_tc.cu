@@ -1,0 +1,456 @@
+// Packed products for many slots on the 5th-generation tensor cores (tcgen05), exact per unit.
+//
+// Integer levels are exact in float16: |level| <= 128, and with the sub-scale of a 16-value group
+// multiplied in (Q2_K, Q3_K, IQ2_XS, IQ2_S) at most 1333; Q6_K's factor of up to 4096 is split into
+// two exact float16 parts. A unit's 32 products are at most 2^24 in sum, so the float32 accumulator
+// in tensor memory holds the integer dot product itself, and no rounding happens before the scales:
+//   acc[n, t] += (dl[n, u] * dx[t, u]) * D_u[n, t]  -  ml[n, u] * (dx * sum lx)[t, u]
+// in float32 registers, two columns per packed instruction. Scales change with every unit in
+// both operands, so the accumulator is read once per unit: 128 x BN values against 2 * 128 * BN * 32
+// operations. Reading, scaling and adding is the bound (two packed operations per pair of values,
+// three for formats with minima), next to it the matrix product itself (half of that time).
+//
+// Roles in a CTA (one per SM, 16 warps):
+//   warps 0-7    own the tile's sums: lane = weight row, each warp half of the columns
+//   warps 8-11   unpack the weights: thread = row, two units per stage, block bytes loaded a stage ahead
+//   warp 12      issues the matrix products (and owns the tensor memory)
+//   warp 13      copies the activations' stage (one bulk copy: levels as the matrix unit reads
+//                them, then the scale planes), laid out beforehand by xpack_kernel
+// Stages are a ring in shared memory (full: unpacked + copied, empty: products done + planes
+// read); the accumulators are a ring in tensor memory. Every wait is bounded: one that runs out
+// records bit 0 of the fault word and its role leaves.
+// The order of the 32 values within a unit does not matter to the sum; both operands use the one
+// that unpacks cheapest (word_halves).
+#include <cooperative_groups.h>
+
+#include "qs_matmul.cuh"
+
+namespace qs {
+
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int TC_M = 128, TC_THREADS = 512;
+constexpr int TC_SMEM = 227 * 1024;
+
+template <int T, int BN>
+struct TcCfg {
+    using L = Lv<T>;
+    static constexpr bool FOLD = L::G16, SPLIT = T == QS_Q6_K;
+    static constexpr int SUMS = !L::HASMIN ? 0 : L::G16 ? 2 : 1, PLANES = 1 + SUMS;
+    static constexpr int A_BYTES = TC_M * 128, A_ALL = A_BYTES * (SPLIT ? 2 : 1), B_BYTES = BN * 128;
+    static constexpr int P_BYTES = 2 * PLANES * BN * 4, X_BYTES = B_BYTES + P_BYTES;  // one bulk copy
+    static constexpr int OFF_B = A_ALL, OFF_P = OFF_B + B_BYTES, OFF_D = OFF_P + P_BYTES;
+    static constexpr int STAGE = (OFF_D + 2 * PLANES * TC_M * 4 + 1023) / 1024 * 1024;
+    static constexpr int FIT = (TC_SMEM - 4096) / STAGE, NS = FIT > 6 ? 6 : FIT;
+    static constexpr int NB = BN == 256 ? 2 : 4;       // accumulators in tensor memory
+    static constexpr int COLS = NB * BN < 32 ? 32 : NB * BN;
+    // 256 columns need 128 registers a thread for the sums alone: registers move from the other
+    // warpgroups to the two with the sums (192, 192, 88, 40 a thread of the 128 at launch)
+    static constexpr bool MOVE = BN == 256;
+    static constexpr int OUT_PITCH = TC_M + 4;
+    static constexpr int BYTES = NS * STAGE + 1024;    // 1024 to align the ring
+    static_assert(NS >= 2, "two stages at least");
+    static_assert(BN * OUT_PITCH * 4 <= NS * STAGE, "the tile leaves through the same memory");
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+    asm volatile("{ .reg .b64 st; mbarrier.arrive.shared::cta.b64 st, [%0]; }" ::"r"(bar) : "memory");
+}
+// Completion of the phase of that parity; false (and the fault recorded) after a bounded number of
+// polls, seconds beyond anything a running product needs.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, unsigned int* fault) {
+    for (int it = 0; it < (1 << 20); it++) {
+        uint32_t ok;
+        asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        if (ok) return true;
+        if (it > 64) __nanosleep(64);
+    }
+    atomicOr(fault, 1u);
+    return false;
+}
+// `bytes` from global to shared memory, completing on the barrier
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile(
+        "{ .reg .b64 st; mbarrier.arrive.expect_tx.shared::cta.b64 st, [%3], %2; }\n"
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+        ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+// Shared-memory operand, K-major, rows of 128 bytes in the 128-byte swizzle: 8-row groups 1024
+// bytes apart
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr) {
+    return (uint64_t)((addr & 0x3FFFF) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{ .reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(addr) : "memory");
+}
+// the loads' registers pass through the wait, so that nothing reads them before it
+__device__ __forceinline__ void tmem_wait_ld(uint32_t* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                   "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :: "memory");
+}
+
+// 4 byte levels as 4 float16, in the order b0 b2 b1 b3: a byte behind 0x64 is 1024 + byte
+__device__ __forceinline__ void word_halves(uint32_t w, __half2 bias, __half2* h) {
+    const uint32_t a = (w & 0x00FF00FFu) | 0x64006400u, b = ((w >> 8) & 0x00FF00FFu) | 0x64006400u;
+    h[0] = __hsub2(*reinterpret_cast<const __half2*>(&a), bias);
+    h[1] = __hsub2(*reinterpret_cast<const __half2*>(&b), bias);
+}
+__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+
+// The slots' Q8_0 rows as the matrix unit reads them, [chunk][stage]: BN rows of 64 float16 levels
+// (two units) in the 128-byte swizzle, then [unit][plane][slot] floats (scale, scale * sum of levels of
+// the unit or of its halves). Rows without a slot are zero. One CTA per stage and chunk.
+template <int BN, int SUMS>
+__global__ void __launch_bounds__(256) xpack_kernel(MmArgs a, uint8_t* out) {
+    constexpr int X_BYTES = BN * 128 + 2 * (1 + SUMS) * BN * 4;
+    const Chunk ch = find_chunk<BN>(a, blockIdx.y);
+    if (ch.group < 0 || (a.order && ch.group == a.n_exp)) return;
+    const int stage = blockIdx.x;
+    uint8_t* o = out + ((int64_t)blockIdx.y * gridDim.x + stage) * X_BYTES;
+    for (int i = threadIdx.x; i < 2 * BN; i += 256) {
+        const int t = i >> 1, uu = i & 1, u = 2 * stage + uu;
+        uint32_t q[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        float d = 0.0f;
+        if (ch.lo + t < ch.hi && u < a.units) {
+            const int slot = a.order ? __ldg(a.order + ch.lo + t) : ch.lo + t;
+            const uint8_t* b = a.x + (int64_t)(slot / a.x_div) * a.x_row + (int64_t)u * 34;
+            ld_words<8, 1>(b + 2, q);
+            d = h2f(ld_u16<1>(b));
+        }
+        const __half2 bias = __float2half2_rn(1152.0f);
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            __half2 h[4];
+            word_halves(q[2 * c] ^ 0x80808080u, bias, h);
+            word_halves(q[2 * c + 1] ^ 0x80808080u, bias, h + 2);
+            *reinterpret_cast<uint4*>(o + t * 128 + (((4 * uu + c) ^ (t & 7)) << 4)) = make_uint4(h2_bits(h[0]), h2_bits(h[1]), h2_bits(h[2]), h2_bits(h[3]));
+        }
+        float* p = reinterpret_cast<float*>(o + BN * 128) + uu * (1 + SUMS) * BN + t;
+        p[0] = d;
+        const int s0 = sum16(make_uint4(q[0], q[1], q[2], q[3])), s1 = sum16(make_uint4(q[4], q[5], q[6], q[7]));
+        if constexpr (SUMS == 1) p[BN] = d * (float)(s0 + s1);
+        if constexpr (SUMS == 2) {
+            p[BN] = d * (float)s0;
+            p[2 * BN] = d * (float)s1;
+        }
+    }
+}
+
+template <int T, int BN>
+__global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8_t* xp) {
+    using L = Lv<T>;
+    using C = TcCfg<T, BN>;
+    constexpr int UPB = L::QK / 32, SUMS = C::SUMS, PLANES = C::PLANES, NS = C::NS, NB = C::NB;
+    constexpr int HALF = BN / 2;  // columns of a warp
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t bars[3 * NS + 2 * NB];
+    __shared__ uint32_t s_tmem;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const Chunk ch = find_chunk<BN>(a, blockIdx.y);
+    if (ch.group < 0) return;  // the CTAs of a cluster share the chunk
+    const uint32_t ring = (smem_u32(smem_raw) + 1023) & ~1023u;
+    uint8_t* const ring_p = smem_raw + (ring - smem_u32(smem_raw));
+    const uint32_t full_w = smem_u32(bars), full_x = full_w + 8 * NS, empty = full_x + 8 * NS, acc_full = empty + 8 * NS, acc_empty = acc_full + 8 * NB;
+    if (tid == 0) {
+        for (int s = 0; s < NS; s++) {
+            mbar_init(full_w + 8 * s, 4);
+            mbar_init(full_x + 8 * s, 1);
+            mbar_init(empty + 8 * s, 1 + 8);
+        }
+        for (int b = 0; b < NB; b++) {
+            mbar_init(acc_full + 8 * b, 1);
+            mbar_init(acc_empty + 8 * b, 8);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "n"(C::COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = s_tmem;
+
+    const int n0 = blockIdx.x * TC_M, cnt = ch.hi - ch.lo;
+    const int stages = (a.units + 1) / 2, per = (stages + a.splits - 1) / a.splits;
+    const bool real = !a.order || ch.group < a.n_exp;
+    const int k0 = blockIdx.z * per, k1 = real ? min(k0 + per, stages) : k0;
+
+    if (warp >= 12) {
+        if constexpr (C::MOVE) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        if (warp == 12) {
+            if (lane == 0) {
+                // D float32, A and B float16 K-major, N = BN, M = 128
+                constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(TC_M >> 4) << 24);
+                int unit = 0;
+                bool ok = true;
+                for (int k = k0; k < k1 && ok; k++) {
+                    const int i = k - k0, s = i % NS, ph = (i / NS) & 1;
+                    ok = mbar_wait(full_w + 8 * s, ph, a.fault) && mbar_wait(full_x + 8 * s, ph, a.fault);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t st = ring + s * C::STAGE;
+                    for (int uu = 0; uu < 2; uu++, unit++) {
+                        const int b = unit % NB;
+                        if (!(ok = mbar_wait(acc_empty + 8 * b, ((unit / NB) & 1) ^ 1, a.fault))) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                        for (int h = 0; h < (C::SPLIT ? 2 : 1); h++)
+#pragma unroll
+                            for (int kk = 0; kk < 2; kk++)
+                                mma_f16(tmem + b * BN, operand_desc(st + h * C::A_BYTES + uu * 64 + kk * 32), operand_desc(st + C::OFF_B + uu * 64 + kk * 32),
+                                        idesc, h + kk > 0);
+                        mma_commit(acc_full + 8 * b);
+                    }
+                    if (ok) mma_commit(empty + 8 * s);
+                }
+            }
+            __syncwarp();
+            asm volatile("bar.sync 1, 288;" ::: "memory");  // the sums' warps have read their last accumulator
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(C::COLS));
+        } else if (warp == 13 && lane == 0) {
+            const uint8_t* src = xp + (int64_t)blockIdx.y * stages * C::X_BYTES;
+            int k = k0;
+            for (; k < k1; k++) {
+                const int i = k - k0, s = i % NS;
+                if (!mbar_wait(empty + 8 * s, ((i / NS) & 1) ^ 1, a.fault)) break;
+                bulk_load(ring + s * C::STAGE + C::OFF_B, src + (int64_t)k * C::X_BYTES, C::X_BYTES, full_x + 8 * s);
+            }
+            // no copy outlives the CTA
+            for (int j = max(k0, k - NS); j < k; j++) mbar_wait(full_x + 8 * ((j - k0) % NS), ((j - k0) / NS) & 1, a.fault);
+        }
+    } else if (warp >= 8) {
+        if constexpr (C::MOVE) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        const int row = tid - 256;
+        const bool mine = n0 + row < a.n;
+        const uint8_t* w = a.w + (real ? ch.group * a.w_exp : 0) + (int64_t)(mine ? n0 + row : 0) * a.w_row;
+        uint32_t raw[2][L::WORDS];
+        auto load = [&](int k) {
+#pragma unroll
+            for (int uu = 0; uu < 2; uu++) {
+                const int u = 2 * k + uu;
+                if (mine && k < k1 && u < a.units) L::template load<L::MAXAL>(w + (int64_t)(u / UPB) * L::BB, u % UPB, raw[uu]);
+                else
+#pragma unroll
+                    for (int j = 0; j < L::WORDS; j++) raw[uu][j] = 0;  // zero scales
+            }
+        };
+        load(k0);
+        for (int k = k0; k < k1; k++) {
+            const int i = k - k0, s = i % NS;
+            uint8_t* st = ring_p + s * C::STAGE;
+            if (!mbar_wait(empty + 8 * s, ((i / NS) & 1) ^ 1, a.fault)) break;
+#pragma unroll
+            for (int uu = 0; uu < 2; uu++) {
+                const int j = (2 * k + uu) % UPB;
+                uint32_t q[8];
+                float dl[2], ml[2];
+                L::levels(raw[uu], j, a.kgrid, q, dl, ml);
+                const __half2 bias = __float2half2_rn(L::SIGNED ? 1152.0f : 1024.0f);
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    __half2 h[4];
+                    word_halves(L::SIGNED ? q[2 * c] ^ 0x80808080u : q[2 * c], bias, h);
+                    word_halves(L::SIGNED ? q[2 * c + 1] ^ 0x80808080u : q[2 * c + 1], bias, h + 2);
+                    uint8_t* o = st + row * 128 + (((4 * uu + c) ^ (row & 7)) << 4);
+                    if constexpr (C::FOLD) {
+                        const __half2 sc = __half2half2(__int2half_rn(L::sub(raw[uu], j, c >> 1)));
+                        __half2 p[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) p[e] = __hmul2(h[e], sc);
+                        if constexpr (C::SPLIT) {  // the product's rounding error, exact in float16
+#pragma unroll
+                            for (int e = 0; e < 4; e++) h[e] = __hfma2(h[e], sc, __hneg2(p[e]));
+                            *reinterpret_cast<uint4*>(o + C::A_BYTES) = make_uint4(h2_bits(h[0]), h2_bits(h[1]), h2_bits(h[2]), h2_bits(h[3]));
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; e++) h[e] = p[e];
+                    }
+                    *reinterpret_cast<uint4*>(o) = make_uint4(h2_bits(h[0]), h2_bits(h[1]), h2_bits(h[2]), h2_bits(h[3]));
+                }
+                float* d = reinterpret_cast<float*>(st + C::OFF_D) + uu * PLANES * TC_M + row;
+                if constexpr (C::FOLD) d[0] = L::base(raw[uu]);
+                else d[0] = dl[0];
+                if constexpr (SUMS >= 1) d[TC_M] = -ml[0];
+                if constexpr (SUMS == 2) d[2 * TC_M] = -ml[1];
+            }
+            load(k + 1);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full_w + 8 * s);
+        }
+    } else {
+        if constexpr (C::MOVE) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+        const int row = (warp & 3) * 32 + lane, c0 = (warp >> 2) * HALF;
+        constexpr int NBT = HALF / 16;
+        f32x2 acc[HALF / 2];
+#pragma unroll
+        for (int i = 0; i < HALF / 2; i++) acc[i] = 0ull;
+        int unit = 0;
+        bool ok = true;
+        for (int k = k0; k < k1 && ok; k++) {
+            const int i = k - k0, s = i % NS, ph = (i / NS) & 1;
+            ok = mbar_wait(full_w + 8 * s, ph, a.fault) && mbar_wait(full_x + 8 * s, ph, a.fault);
+            if (!ok) break;
+            const uint8_t* st = ring_p + s * C::STAGE;
+            for (int uu = 0; uu < 2; uu++, unit++) {
+                const int b = unit % NB;
+                const float* d = reinterpret_cast<const float*>(st + C::OFF_D) + uu * PLANES * TC_M + row;
+                const float4* x = reinterpret_cast<const float4*>(st + C::OFF_P + (uu * PLANES * BN + c0) * 4);
+                const f32x2 dl = f2_splat(d[0]);
+                f32x2 ml[SUMS ? SUMS : 1];
+#pragma unroll
+                for (int p = 0; p < SUMS; p++) ml[p] = f2_splat(d[(1 + p) * TC_M]);
+                if (!(ok = mbar_wait(acc_full + 8 * b, (unit / NB) & 1, a.fault))) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + b * BN + c0;
+                uint32_t v[2][16];
+                tmem_ld16(at, v[0]);
+                tmem_wait_ld(v[0]);
+#pragma unroll
+                for (int bt = 0; bt < NBT; bt++) {
+                    if (bt + 1 < NBT) tmem_ld16(at + 16 * (bt + 1), v[(bt + 1) & 1]);
+                    const uint32_t* r = v[bt & 1];
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        const float4 xv = x[bt * 4 + c];
+                        f32x2& a0 = acc[bt * 8 + 2 * c];
+                        f32x2& a1 = acc[bt * 8 + 2 * c + 1];
+                        a0 = f2_fma(f2_mul_z(dl, f2_pack(xv.x, xv.y)), f2_pack(__uint_as_float(r[4 * c]), __uint_as_float(r[4 * c + 1])), a0);
+                        a1 = f2_fma(f2_mul_z(dl, f2_pack(xv.z, xv.w)), f2_pack(__uint_as_float(r[4 * c + 2]), __uint_as_float(r[4 * c + 3])), a1);
+#pragma unroll
+                        for (int p = 0; p < SUMS; p++) {
+                            const float4 sv = x[(1 + p) * (BN / 4) + bt * 4 + c];
+                            a0 = f2_fma(ml[p], f2_pack(sv.x, sv.y), a0);
+                            a1 = f2_fma(ml[p], f2_pack(sv.z, sv.w), a1);
+                        }
+                    }
+                    if (bt + 1 < NBT) tmem_wait_ld(v[(bt + 1) & 1]);
+                    if (bt + 2 == NBT || NBT == 1) {  // the last loads are in registers
+                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(acc_empty + 8 * b);
+                    }
+                }
+            }
+            __syncwarp();
+            if (ok && lane == 0) mbar_arrive(empty + 8 * s);
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        asm volatile("bar.sync 1, 288;" ::: "memory");
+
+        // the tile through shared memory (all copies and products have been waited for), so that a
+        // slot's columns leave in whole rows
+        float* o = reinterpret_cast<float*>(ring_p);
+#pragma unroll
+        for (int i = 0; i < HALF / 2; i++) {
+            float x0, x1;
+            f2_unpack(acc[i], x0, x1);
+            o[(c0 + 2 * i) * C::OUT_PITCH + row] = x0;
+            o[(c0 + 2 * i + 1) * C::OUT_PITCH + row] = x1;
+        }
+        const int rank = blockIdx.z, ranks = a.splits;
+        if (ranks > 1) cg::this_cluster().sync();
+        else asm volatile("bar.sync 2, 256;" ::: "memory");
+        void* out = a.part ? (void*)a.part : a.out;
+        const int type = a.part ? (int)SRC_F32 : a.out_type;
+        const int64_t stride = a.part ? a.n : a.out_stride;
+        const bool vec = n0 + TC_M <= a.n && stride % 4 == 0 && ((uintptr_t)out & 15) == 0;
+        for (int t = warp * ranks + rank; t < cnt; t += 8 * ranks) {
+            const int64_t slot = a.order ? __ldg(a.order + ch.lo + t) : ch.lo + t;
+            const int64_t at = slot * stride + n0;
+            float4 v;
+            if (ranks > 1) {
+                v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                for (int r = 0; r < ranks; r++) {
+                    const float4 f = *reinterpret_cast<const float4*>(cg::this_cluster().map_shared_rank(o, r) + t * C::OUT_PITCH + 4 * lane);
+                    v.x += f.x; v.y += f.y; v.z += f.z; v.w += f.w;
+                }
+            } else {
+                v = *reinterpret_cast<const float4*>(o + t * C::OUT_PITCH + 4 * lane);
+            }
+            store_row4(out, at, type, v, lane, n0, a.n, vec);
+        }
+    }
+    __syncwarp();
+    if (a.splits > 1) {
+        if (warp >= 8) cg::this_cluster().sync();
+        cg::this_cluster().sync();  // the others may still read this tile
+    }
+}
+
+template <int T, int BN>
+cudaError_t launch_tc_t(const MmArgs& a, uint8_t* xp, const LaunchCtx& ctx) {
+    using C = TcCfg<T, BN>;
+    const int64_t chunks = max_chunks(a, BN);
+    if (chunks > 65535) return cudaErrorInvalidConfiguration;
+    xpack_kernel<BN, C::SUMS><<<dim3((a.units + 1) / 2, (unsigned)chunks), 256, 0, ctx.stream>>>(a, xp);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    e = cudaFuncSetAttribute(tc_kernel<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::BYTES);
+    if (e != cudaSuccess) return e;
+    if constexpr (C::MOVE) {  // the warpgroups' shares must be there at launch
+        static const int regs = [] {
+            cudaFuncAttributes f;
+            return cudaFuncGetAttributes(&f, tc_kernel<T, BN>) == cudaSuccess ? f.numRegs : 0;
+        }();
+        if (regs * TC_THREADS < 128 * (192 + 192 + 88 + 40)) return cudaErrorInvalidConfiguration;
+    }
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3((unsigned)((a.n + TC_M - 1) / TC_M), (unsigned)chunks, (unsigned)a.splits);
+    cfg.blockDim = dim3(TC_THREADS);
+    cfg.dynamicSmemBytes = C::BYTES;
+    cfg.stream = ctx.stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 1;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = (unsigned)a.splits;
+    cfg.attrs = at;
+    cfg.numAttrs = a.splits > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, tc_kernel<T, BN>, a, static_cast<const uint8_t*>(xp));
+}
+
+template <int T>
+cudaError_t launch_tc(const MmArgs& a, int bn, uint8_t* xp, const LaunchCtx& ctx) {
+    return bn == 32 ? launch_tc_t<T, 32>(a, xp, ctx) : bn == 64 ? launch_tc_t<T, 64>(a, xp, ctx) : bn == 128 ? launch_tc_t<T, 128>(a, xp, ctx) : launch_tc_t<T, 256>(a, xp, ctx);
+}
+
+}  // namespace
+
+int64_t mm_tc_workspace(int64_t units, int64_t chunks, int bn, int planes) {
+    return chunks * ((units + 1) / 2) * ((int64_t)bn * 128 + 2 * planes * bn * 4);
+}
+
+cudaError_t launch_mm_tc(int type, const MmArgs& a, int bn, void* xp, const LaunchCtx& ctx) {
+    switch (type) {
+#define X(T) case T: return launch_tc<T>(a, bn, static_cast<uint8_t*>(xp), ctx);
+        QS_FOR_TYPES(X)
+#undef X
+    default: return cudaErrorInvalidValue;
+    }
+}
+
+}  // namespace qs
