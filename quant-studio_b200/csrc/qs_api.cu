@@ -447,19 +447,20 @@ bool has_min(int type) {
 
 // How a product runs: which kernel, its tile, over how many CTAs a tile's rows are split.
 struct MmPlan {
-    bool few;
+    bool few, lo;
     int bn, splits;
     int64_t part_off, bytes;  // workspace: laid-out activations, then the slots' results before a sum
 };
 
 // slots: output rows before a weighted sum; groups: weight matrices that share them. The tile
 // kernel keeps one CTA on each of a B200's 148 SMs.
-MmPlan mm_plan(int type, int64_t n, int64_t k, int64_t slots, int64_t groups, bool experts, bool sum) {
+MmPlan mm_plan(int type, int64_t n, int64_t k, int64_t slots, int64_t groups, bool experts, bool sum, bool lo) {
     MmPlan p;
     const int64_t avg = (slots + groups - 1) / groups, units = k / 32, stages = (units + 1) / 2;
     // rows that the small kernel can not hold go to the tiles whatever their number
     p.few = (groups == 1 ? slots <= qs::FEW_SLOTS : avg <= 4) && units * qs::FEW_SLOTS * qs::FEW_UNIT_MAX <= qs::FEW_SMEM_MAX;
-    p.bn = avg <= 32 ? 32 : avg <= 64 ? 64 : avg <= 128 ? 128 : 256;
+    p.lo = lo;
+    p.bn = avg <= 32 ? 32 : avg <= 64 ? 64 : avg <= 128 || lo ? 128 : 256;
     p.splits = 1;
     const int64_t chunks = groups == 1 ? (slots + p.bn - 1) / p.bn : slots / p.bn + (groups < slots ? groups : slots) / 2 + 1;
     const int64_t tiles = (n + 127) / 128 * chunks;
@@ -468,14 +469,14 @@ MmPlan mm_plan(int type, int64_t n, int64_t k, int64_t slots, int64_t groups, bo
         if (s > 8) s = 8;                    // a cluster
         if (s > stages / 8) s = stages / 8;  // 8 stages each at least
         if (s > 1) {
-            const int64_t per = (stages + s - 1) / s;
+            const int64_t per = ((stages + s - 1) / s + 3) / 4 * 4;
             p.splits = (int)((stages + per - 1) / per);
         }
     }
     int64_t xp = 0;
     if (!p.few) {
-        const int planes = !has_min(type) ? 1 : type == qs::QS_Q2_K ? 3 : 2;
-        xp = (qs::mm_tc_workspace(units, qs::max_chunks(experts, slots, groups, p.bn), p.bn, planes) + 255) / 256 * 256;
+        const int sums = !has_min(type) ? 0 : type == qs::QS_Q2_K ? 2 : 1;
+        xp = (qs::mm_tc_workspace(units, qs::max_chunks(experts, slots, groups, p.bn), p.bn, lo, sums) + 255) / 256 * 256;
     }
     p.part_off = xp;
     p.bytes = xp + (sum ? slots * n * 4 : 0);
@@ -490,7 +491,7 @@ int check_mm(int ggml_type, int64_t n, int64_t k, int64_t rows, int64_t per_toke
     if (k > (int64_t)1 << 30) return fail(QS_EINVAL, "row length %lld is over 2^30", (long long)k);
     if (n <= 0 || n > (int64_t)1 << 30) return fail(QS_EINVAL, "weight row count %lld is not in 1 .. 2^30", (long long)n);
     if (rows < 0) return fail(QS_EINVAL, "negative row count");
-    // 65535 chunks of 32 slots, and the joining kernel's threads
+    // 65535 chunks of 32 slots, and the threads of a weighted sum
     if (rows > (1 << 20) / per_token || rows * per_token * n > (int64_t)1 << 38)
         return fail(QS_EINVAL, "%lld rows of %lld outputs are too many for one call", (long long)(rows * per_token), (long long)n);
     *out = ti;
@@ -516,7 +517,7 @@ int run_mm(int ggml_type, const MmPlan& p, qs::MmArgs& a, int64_t k, int top_k, 
     a.units = (int)(k / 32);
     a.splits = p.splits;
     a.part = weights ? reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + p.part_off) : nullptr;
-    cudaError_t e = p.few ? qs::launch_mm_few(ggml_type, a, ctx) : qs::launch_mm_tc(ggml_type, a, p.bn, workspace, ctx);
+    cudaError_t e = p.few ? qs::launch_mm_few(ggml_type, a, ctx) : qs::launch_mm_tc(ggml_type, a, p.bn, p.lo, workspace, ctx);
     if (e == cudaSuccess && weights) e = qs::launch_mm_sum(a, top_k, weights, ids, ctx);
     return e == cudaSuccess ? QS_OK : cuda_fail(e, "matmul launch");
 }
@@ -631,10 +632,11 @@ QS_API int qs_expert_plan(const int32_t* ids, int64_t n_slots, int n_experts, in
     return e == cudaSuccess ? QS_OK : cuda_fail(e, "expert plan launch");
 }
 
-QS_API int qs_matmul_workspace(int ggml_type, int64_t n, int64_t k, int64_t n_rows, int64_t* bytes) {
+QS_API int qs_matmul_workspace(int ggml_type, int64_t n, int64_t k, int64_t n_rows, int out_type, int64_t* bytes) {
     const TypeInfo* ti;
+    if (!is_src(out_type)) return fail(QS_EINVAL, "output type %d is not F32/F16/BF16", out_type);
     if (int rc = check_mm(ggml_type, n, k, n_rows, 1, &ti)) return rc;
-    if (bytes) *bytes = mm_plan(ggml_type, n, k, n_rows, 1, false, false).bytes;
+    if (bytes) *bytes = mm_plan(ggml_type, n, k, n_rows, 1, false, false, out_type != QS_SRC_BF16).bytes;
     return QS_OK;
 }
 
@@ -645,7 +647,7 @@ QS_API int qs_matmul(int ggml_type, const void* w, int64_t w_row_bytes, int64_t 
     if (rc) return rc;
     if (n_rows == 0) return QS_OK;
     if ((rc = check_mm_operands(ti, w, w_row_bytes, k, x, x_row_bytes, out, out_type, out_row_stride, n))) return rc;
-    const MmPlan p = mm_plan(ggml_type, n, k, n_rows, 1, false, false);
+    const MmPlan p = mm_plan(ggml_type, n, k, n_rows, 1, false, false, out_type != QS_SRC_BF16);
     if ((rc = check_workspace(workspace, workspace_bytes, p.bytes))) return rc;
     CurrentContextGuard keep;
     int device;
@@ -671,13 +673,14 @@ QS_API int qs_matmul(int ggml_type, const void* w, int64_t w_row_bytes, int64_t 
     return run_mm(ggml_type, p, a, k, 1, nullptr, nullptr, workspace, qs::LaunchCtx{static_cast<cudaStream_t>(stream), device, d->num_sms});
 }
 
-QS_API int qs_matmul_experts_workspace(int ggml_type, int n_experts, int64_t n, int64_t k, int64_t n_tokens, int top_k, int x_per_slot, int sum,
+QS_API int qs_matmul_experts_workspace(int ggml_type, int n_experts, int64_t n, int64_t k, int64_t n_tokens, int top_k, int sum, int out_type,
                                        int64_t* bytes) {
     const TypeInfo* ti;
+    if (!is_src(out_type)) return fail(QS_EINVAL, "output type %d is not F32/F16/BF16", out_type);
     if (n_experts < 1 || n_experts > QS_MAX_EXPERTS) return fail(QS_EINVAL, "%d experts are not in 1 .. %d", n_experts, QS_MAX_EXPERTS);
     if (top_k < 1 || top_k > QS_MAX_EXPERTS) return fail(QS_EINVAL, "%d experts per token are not in 1 .. %d", top_k, QS_MAX_EXPERTS);
     if (int rc = check_mm(ggml_type, n, k, n_tokens, top_k, &ti)) return rc;
-    if (bytes) *bytes = mm_plan(ggml_type, n, k, n_tokens * top_k, n_experts, true, sum != 0).bytes;
+    if (bytes) *bytes = mm_plan(ggml_type, n, k, n_tokens * top_k, n_experts, true, sum != 0, out_type != QS_SRC_BF16).bytes;
     return QS_OK;
 }
 
@@ -698,7 +701,7 @@ QS_API int qs_matmul_experts(int ggml_type, const void* w, int64_t w_row_bytes, 
     if (!aligned(ids, 4) || !aligned(order, 4) || !aligned(offsets, 4) || (weights && !aligned(weights, 4)))
         return fail(QS_EINVAL, "a pointer is not aligned to its elements");
     const int64_t slots = n_tokens * top_k;
-    const MmPlan p = mm_plan(ggml_type, n, k, slots, n_experts, true, weights != nullptr);
+    const MmPlan p = mm_plan(ggml_type, n, k, slots, n_experts, true, weights != nullptr, out_type != QS_SRC_BF16);
     if ((rc = check_workspace(workspace, workspace_bytes, p.bytes))) return rc;
     CurrentContextGuard keep;
     int device;

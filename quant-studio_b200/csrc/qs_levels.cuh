@@ -6,8 +6,9 @@
 // Lv<T>::load brings what unit j of a block needs into WORDS registers, Lv<T>::levels makes of
 // them its levels as 8 words (4 levels each, value order) and dl, ml of its two halves of 16
 // values; two steps, so that loads can run ahead. G16: the halves' scales differ; HASMIN: ml is
-// not always zero; G16 formats also give d and the integer factors of its halves (base, subs:
-// dl[h] = base * sub[h]). SIGNED: levels are int8 (else 0 .. 31). dl and ml are exact: a float16
+// not always zero; SIGNED: levels are int8 (else 0 .. 31). FOLD: a superblock has one scale, base, and
+// integer factors sub (dl[h] = base * sub(h)) whose products with the levels stay below 2048
+// (Q6_K: up to 4096). dl and ml are exact: a float16
 // times a few scale bits.
 #pragma once
 
@@ -70,7 +71,7 @@ template <int T> struct Lv;
 
 template <> struct Lv<QS_Q4_0> {
     static constexpr int QK = 32, BB = 18, MAXAL = 2;
-    static constexpr bool G16 = false, HASMIN = false, SIGNED = true;
+    static constexpr bool G16 = false, HASMIN = false, SIGNED = true, FOLD = false;
     static constexpr int WORDS = 5;
     template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int, uint32_t* r) {
@@ -90,7 +91,7 @@ template <> struct Lv<QS_Q4_0> {
 
 template <> struct Lv<QS_Q4_1> {
     static constexpr int QK = 32, BB = 20, MAXAL = 4;
-    static constexpr bool G16 = false, HASMIN = true, SIGNED = false;
+    static constexpr bool G16 = false, HASMIN = true, SIGNED = false, FOLD = false;
     static constexpr int WORDS = 5;
     template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int, uint32_t* r) {
@@ -109,7 +110,7 @@ template <> struct Lv<QS_Q4_1> {
 
 template <> struct Lv<QS_Q5_0> {
     static constexpr int QK = 32, BB = 22, MAXAL = 2;
-    static constexpr bool G16 = false, HASMIN = false, SIGNED = true;
+    static constexpr bool G16 = false, HASMIN = false, SIGNED = true, FOLD = false;
     static constexpr int WORDS = 6;
     template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int, uint32_t* r) {
@@ -129,7 +130,7 @@ template <> struct Lv<QS_Q5_0> {
 
 template <> struct Lv<QS_Q5_1> {
     static constexpr int QK = 32, BB = 24, MAXAL = 8;
-    static constexpr bool G16 = false, HASMIN = true, SIGNED = false;
+    static constexpr bool G16 = false, HASMIN = true, SIGNED = false, FOLD = false;
     static constexpr int WORDS = 6;
     template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int, uint32_t* r) {
@@ -148,7 +149,7 @@ template <> struct Lv<QS_Q5_1> {
 
 template <> struct Lv<QS_Q8_0> {
     static constexpr int QK = 32, BB = 34, MAXAL = 2;
-    static constexpr bool G16 = false, HASMIN = false, SIGNED = true;
+    static constexpr bool G16 = false, HASMIN = false, SIGNED = true, FOLD = false;
     static constexpr int WORDS = 9;
     template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int, uint32_t* r) {
@@ -165,7 +166,7 @@ template <> struct Lv<QS_Q8_0> {
 
 template <> struct Lv<QS_Q2_K> {
     static constexpr int QK = 256, BB = 84, MAXAL = 4;
-    static constexpr bool G16 = true, HASMIN = true, SIGNED = false;
+    static constexpr bool G16 = true, HASMIN = true, SIGNED = false, FOLD = true;
     static constexpr int WORDS = 10;
     template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
@@ -190,7 +191,7 @@ template <> struct Lv<QS_Q2_K> {
 
 template <> struct Lv<QS_Q3_K> {
     static constexpr int QK = 256, BB = 110, MAXAL = 2;
-    static constexpr bool G16 = true, HASMIN = false, SIGNED = true;
+    static constexpr bool G16 = true, HASMIN = false, SIGNED = true, FOLD = true;
     static constexpr int WORDS = 20;
     template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
@@ -228,7 +229,7 @@ __device__ __forceinline__ void k4_scale_min(const uint32_t* s, int j, float& sc
 
 template <> struct Lv<QS_Q4_K> {
     static constexpr int QK = 256, BB = 144, MAXAL = 16;
-    static constexpr bool G16 = false, HASMIN = true, SIGNED = false;
+    static constexpr bool G16 = false, HASMIN = true, SIGNED = false, FOLD = true;
     static constexpr int WORDS = 12;
     template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
@@ -243,11 +244,17 @@ template <> struct Lv<QS_Q4_K> {
 #pragma unroll
         for (int i = 0; i < 8; i++) q[i] = (r[i] >> (4 * (j & 1))) & 0x0F0F0F0Fu;
     }
+    __device__ static float base(const uint32_t* r) { return h2f(r[8] & 0xFFFFu); }
+    __device__ static int sub(const uint32_t* r, int j, int) {
+        float sc, mn;
+        k4_scale_min(r + 9, j, sc, mn);
+        return (int)sc;
+    }
 };
 
 template <> struct Lv<QS_Q5_K> {
     static constexpr int QK = 256, BB = 176, MAXAL = 16;
-    static constexpr bool G16 = false, HASMIN = true, SIGNED = false;
+    static constexpr bool G16 = false, HASMIN = true, SIGNED = false, FOLD = true;
     static constexpr int WORDS = 20;
     template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
@@ -264,11 +271,17 @@ template <> struct Lv<QS_Q5_K> {
         for (int i = 0; i < 8; i++)
             q[i] = ((r[i] >> (4 * (j & 1))) & 0x0F0F0F0Fu) | (((r[12 + i] >> j) & 0x01010101u) << 4);
     }
+    __device__ static float base(const uint32_t* r) { return h2f(r[8] & 0xFFFFu); }
+    __device__ static int sub(const uint32_t* r, int j, int) {
+        float sc, mn;
+        k4_scale_min(r + 9, j, sc, mn);
+        return (int)sc;
+    }
 };
 
 template <> struct Lv<QS_Q6_K> {
     static constexpr int QK = 256, BB = 210, MAXAL = 2;
-    static constexpr bool G16 = true, HASMIN = false, SIGNED = true;
+    static constexpr bool G16 = true, HASMIN = false, SIGNED = true, FOLD = true;
     static constexpr int WORDS = 18;
     template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
@@ -307,7 +320,7 @@ __device__ __forceinline__ uint32_t sign8(uint32_t i) { return i | ((__popc(i) &
 
 template <> struct Lv<QS_IQ2_XXS> {
     static constexpr int QK = 256, BB = 66, MAXAL = 2;
-    static constexpr bool G16 = false, HASMIN = false, SIGNED = true;
+    static constexpr bool G16 = false, HASMIN = false, SIGNED = true, FOLD = true;
     static constexpr int WORDS = 3;
     template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
@@ -321,11 +334,13 @@ template <> struct Lv<QS_IQ2_XXS> {
         for (int s = 0; s < 4; s++)
             iq2_signed(__ldg(kgrid + ((r[0] >> (8 * s)) & 0xFFu)), sign8((r[1] >> (7 * s)) & 127u), q + 2 * s);
     }
+    __device__ static float base(const uint32_t* r) { return h2f(r[2]) * 0.125f; }
+    __device__ static int sub(const uint32_t* r, int, int) { return 1 + 2 * (int)(r[1] >> 28); }
 };
 
 template <> struct Lv<QS_IQ2_XS> {
     static constexpr int QK = 256, BB = 74, MAXAL = 2;
-    static constexpr bool G16 = true, HASMIN = false, SIGNED = true;
+    static constexpr bool G16 = true, HASMIN = false, SIGNED = true, FOLD = true;
     static constexpr int WORDS = 4;
     template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
@@ -350,7 +365,7 @@ template <> struct Lv<QS_IQ2_XS> {
 
 template <> struct Lv<QS_IQ2_S> {
     static constexpr int QK = 256, BB = 82, MAXAL = 2;
-    static constexpr bool G16 = true, HASMIN = false, SIGNED = true;
+    static constexpr bool G16 = true, HASMIN = false, SIGNED = true, FOLD = true;
     static constexpr int WORDS = 5;
     template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
@@ -380,7 +395,7 @@ __device__ __forceinline__ uint32_t iq3_bytes(uint32_t c, uint32_t lo, uint32_t 
 
 template <> struct Lv<QS_IQ3_XXS> {
     static constexpr int QK = 256, BB = 98, MAXAL = 2;
-    static constexpr bool G16 = false, HASMIN = false, SIGNED = true;
+    static constexpr bool G16 = false, HASMIN = false, SIGNED = true, FOLD = true;
     static constexpr int WORDS = 4;
     template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
@@ -397,11 +412,13 @@ template <> struct Lv<QS_IQ3_XXS> {
             q[i] = neg_bytes(iq3_bytes(__ldg(kgrid + ((r[i / 4] >> (8 * (i & 3))) & 0xFFu)), 0x1C140C04u, 0x3E342C24u), bits_to_bytes(sg));
         }
     }
+    __device__ static float base(const uint32_t* r) { return h2f(r[3]) * 0.25f; }
+    __device__ static int sub(const uint32_t* r, int, int) { return 1 + 2 * (int)(r[2] >> 28); }
 };
 
 template <> struct Lv<QS_IQ3_S> {
     static constexpr int QK = 256, BB = 110, MAXAL = 2;
-    static constexpr bool G16 = false, HASMIN = false, SIGNED = true;
+    static constexpr bool G16 = false, HASMIN = false, SIGNED = true, FOLD = true;
     static constexpr int WORDS = 6;
     template <int AL, bool SM = false>
     __device__ static void load(const uint8_t* b, int j, uint32_t* r) {
@@ -419,11 +436,13 @@ template <> struct Lv<QS_IQ3_S> {
             q[i] = neg_bytes(iq3_bytes(__ldg(kgrid + (((r[i / 4] >> (8 * (i & 3))) & 0xFFu) | (((r[4] >> i) & 1u) << 8))), 0x07050301u, 0x0F0D0B09u),
                              bits_to_bytes(r[2] >> (4 * i)));
     }
+    __device__ static float base(const uint32_t* r) { return h2f(r[3]); }
+    __device__ static int sub(const uint32_t* r, int j, int) { return 1 + 2 * (int)((r[5] >> (4 * (j & 1))) & 15u); }
 };
 
 template <> struct Lv<QS_IQ4_XS> {
     static constexpr int QK = 256, BB = 136, MAXAL = 8;
-    static constexpr bool G16 = false, HASMIN = false, SIGNED = true;
+    static constexpr bool G16 = false, HASMIN = false, SIGNED = true, FOLD = false;
     static constexpr int WORDS = 6;
     // the 16 level values, 4 to a word: -127 -104 -83 -65 | -49 -35 -22 -10 | 1 13 25 38 | 53 69 89 113
     __device__ static uint32_t value4(uint32_t n) {  // 4 nibbles (one per byte) -> their bytes

@@ -134,11 +134,26 @@ __device__ __forceinline__ int sum16(const uint4& v) {
 // and slot, for up to 8 slots
 constexpr int FEW_SMEM_MAX = 200 * 1024, FEW_SLOTS = 8, FEW_UNIT_MAX = 44;
 cudaError_t launch_mm_few(int type, const MmArgs& a, const LaunchCtx& ctx);
-cudaError_t launch_mm_tile(int type, const MmArgs& a, int bn, const LaunchCtx& ctx);
-// tcgen05 tiles (qs_matmul_tc.cu): bytes of the laid-out activations at xp for `chunks` chunks of
-// bn slots; planes: 1, 2 with minima, 3 with minima per 16 values
-int64_t mm_tc_workspace(int64_t units, int64_t chunks, int bn, int planes);
-cudaError_t launch_mm_tc(int type, const MmArgs& a, int bn, void* xp, const LaunchCtx& ctx);
+// tcgen05 tiles (qs_matmul_tc.cuh): tiles of bn slots; lo: both float16 parts of the activations. ws:
+// mm_tc_workspace bytes for `chunks` chunks (the rows' powers of two lead); sums: level sums per unit
+// (1 with minima, 2 with minima per 16 values, else 0)
+inline int64_t xs_bytes(int64_t chunks, int bn) { return (chunks * bn * 4 + 255) / 256 * 256; }
+inline int64_t mm_tc_workspace(int64_t units, int64_t chunks, int bn, bool lo, int sums) {
+    return xs_bytes(chunks, bn) + chunks * ((units + 1) / 2) * ((int64_t)bn * 128 * (lo ? 2 : 1) + 2 * sums * bn * 4);
+}
+// by the file that holds the type
+cudaError_t launch_mm_tc_legacy(int type, const MmArgs& a, int bn, bool lo, void* ws, const LaunchCtx& ctx);
+cudaError_t launch_mm_tc_k(int type, const MmArgs& a, int bn, bool lo, void* ws, const LaunchCtx& ctx);
+cudaError_t launch_mm_tc_k2(int type, const MmArgs& a, int bn, bool lo, void* ws, const LaunchCtx& ctx);
+cudaError_t launch_mm_tc_iq(int type, const MmArgs& a, int bn, bool lo, void* ws, const LaunchCtx& ctx);
+inline cudaError_t launch_mm_tc(int type, const MmArgs& a, int bn, bool lo, void* ws, const LaunchCtx& ctx) {
+    switch (type) {
+    case QS_Q4_0: case QS_Q4_1: case QS_Q5_0: case QS_Q5_1: case QS_Q8_0: return launch_mm_tc_legacy(type, a, bn, lo, ws, ctx);
+    case QS_Q2_K: case QS_Q3_K: case QS_Q4_K: return launch_mm_tc_k(type, a, bn, lo, ws, ctx);
+    case QS_Q5_K: case QS_Q6_K: case QS_IQ4_XS: return launch_mm_tc_k2(type, a, bn, lo, ws, ctx);
+    default: return launch_mm_tc_iq(type, a, bn, lo, ws, ctx);
+    }
+}
 // out[token] = sum over its per_out slots that have an expert of weight * part
 cudaError_t launch_mm_sum(const MmArgs& a, int per_out, const float* weights, const int* ids, const LaunchCtx& ctx);
 

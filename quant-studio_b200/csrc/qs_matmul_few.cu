@@ -138,6 +138,44 @@ __global__ void __launch_bounds__(512) few_kernel(MmArgs a, int rows_per_warp) {
     }
 }
 
+// One thread per VEC columns of an output row: the slots in order.
+template <int VEC>
+__global__ void __launch_bounds__(256) sum_kernel(MmArgs a, int per_out, const float* weights, const int* ids, int n_vec) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, outs = a.slots / per_out;
+    if (i >= outs * n_vec) return;
+    const int64_t r = i / n_vec;
+    const int c = (int)(i - r * n_vec) * VEC;
+    float sum[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; v++) sum[v] = 0.0f;
+    constexpr int B = 4;  // slots whose loads are in flight together
+    for (int j0 = 0; j0 < per_out; j0 += B) {
+        float p[B][VEC], wt[B];
+        bool use[B];
+#pragma unroll
+        for (int b = 0; b < B; b++) {
+            const int64_t slot = r * per_out + j0 + b;
+            const bool in = j0 + b < per_out;
+            use[b] = in && (unsigned)__ldg(ids + (in ? slot : 0)) < (unsigned)a.n_exp;
+            wt[b] = in ? __ldg(weights + slot) : 0.0f;
+            const float* q = a.part + (in ? slot : 0) * a.n + c;
+            if constexpr (VEC == 4) {
+                const float4 f = __ldg(reinterpret_cast<const float4*>(q));
+                p[b][0] = f.x; p[b][1] = f.y; p[b][2] = f.z; p[b][3] = f.w;
+            } else {
+                p[b][0] = __ldg(q);
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < B; b++)
+#pragma unroll
+            for (int v = 0; v < VEC; v++)
+                if (use[b]) sum[v] = __fmaf_rn(wt[b], p[b][v], sum[v]);
+    }
+#pragma unroll
+    for (int v = 0; v < VEC; v++) store_val(a.out, r * a.out_stride + c + v, a.out_type, sum[v]);
+}
+
 template <int T, int NT>
 cudaError_t launch_few_t(const MmArgs& a, const LaunchCtx& ctx) {
     const int64_t chunks = max_chunks(a, NT);
@@ -177,6 +215,16 @@ cudaError_t launch_mm_few(int type, const MmArgs& a, const LaunchCtx& ctx) {
 #undef X
     default: return cudaErrorInvalidValue;
     }
+}
+
+cudaError_t launch_mm_sum(const MmArgs& a, int per_out, const float* weights, const int* ids, const LaunchCtx& ctx) {
+    const bool v4 = a.n % 4 == 0;
+    const int n_vec = v4 ? a.n / 4 : a.n;
+    const int64_t threads = (int64_t)(a.slots / per_out) * n_vec;
+    const unsigned blocks = (unsigned)((threads + 255) / 256);
+    if (v4) sum_kernel<4><<<blocks, 256, 0, ctx.stream>>>(a, per_out, weights, ids, n_vec);
+    else sum_kernel<1><<<blocks, 256, 0, ctx.stream>>>(a, per_out, weights, ids, n_vec);
+    return cudaGetLastError();
 }
 
 }  // namespace qs

@@ -1,26 +1,35 @@
-// Packed products for many slots on the 5th-generation tensor cores (tcgen05), exact per unit.
+// Packed products for many slots on the 5th-generation tensor cores (tcgen05, float16 operands,
+// float32 sums in tensor memory).
 //
-// Integer levels are exact in float16: |level| <= 128, and with the sub-scale of a 16-value group
-// multiplied in (Q2_K, Q3_K, IQ2_XS, IQ2_S) at most 1333; Q6_K's factor of up to 4096 is split into
-// two exact float16 parts. A unit's 32 products are at most 2^24 in sum, so the float32 accumulator
-// in tensor memory holds the integer dot product itself, and no rounding happens before the scales:
-//   acc[n, t] += (dl[n, u] * dx[t, u]) * D_u[n, t]  -  ml[n, u] * (dx * sum lx)[t, u]
-// in float32 registers, two columns per packed instruction. Scales change with every unit in
-// both operands, so the accumulator is read once per unit: 128 x BN values against 2 * 128 * BN * 32
-// operations. Reading, scaling and adding is the bound (two packed operations per pair of values,
-// three for formats with minima), next to it the matrix product itself (half of that time).
+// Weights: integer levels are exact in float16, and so is level * sub-scale of the formats with one
+// scale per superblock (at most 2048): for those D sums W' x over a superblock of 256 values, and
+//   acc[n, t] += d[n, superblock] * D[n, t]
+// in float32 registers. Formats with a scale per 32 values are scaled and added every 32. Q6_K's
+// level * sub-scale (up to 4096) is float16 hi + lo, exact together.
+// Activations: scale * level has 19 bits; times a power of two per row (so that the row's largest lies
+// below 2^15) it is float16 hi + lo, exact together down to 2^-39 of the row's largest. LO: the
+// products use both parts (Q6_K: hi hi, hi lo, lo hi), for float32 and float16 results. For
+// bfloat16 results hi alone is multiplied: its rounding, 2^-12 of a value, is 1/8 of the result's.
+// Minima are one more term, - ml[n, unit] * (scale * sum of levels)[t, unit], per 32 (16) values.
+//
+// A pass over K = 32 of a 128 x 256 tile is 271 cycles of the matrix unit (540 with LO). Scaling every 32
+// values by both operands' scales instead, with exact integers in D, was built first and took 1235 us
+// for 2048 slots of Q4_K 14336 x 4096: three float32 operations per value and unit are 768 cycles
+// (a packed f32x2 operation takes two), an SM has no more than 128 lanes.
 //
 // Roles in a CTA (one per SM, 16 warps):
 //   warps 0-7    own the tile's sums: lane = weight row, each warp half of the columns
 //   warps 8-11   unpack the weights: thread = row, two units per stage, block bytes loaded a stage ahead
 //   warp 12      issues the matrix products (and owns the tensor memory)
-//   warp 13      copies the activations' stage (one bulk copy: levels as the matrix unit reads
-//                them, then the scale planes), laid out beforehand by xpack_kernel
+//   warp 13      copies the activations' stage (one bulk copy: float16 rows as the matrix unit reads
+//                them, then the planes of scaled level sums), laid out beforehand by xpack_kernel
 // Stages are a ring in shared memory (full: unpacked + copied, empty: products done + planes
 // read); the accumulators are a ring in tensor memory. Every wait is bounded: one that runs out
 // records bit 0 of the fault word and its role leaves.
 // The order of the 32 values within a unit does not matter to the sum; both operands use the one
 // that unpacks cheapest (word_halves).
+#pragma once
+
 #include <cooperative_groups.h>
 
 #include "qs_matmul.cuh"
@@ -34,18 +43,20 @@ namespace cg = cooperative_groups;
 constexpr int TC_M = 128, TC_THREADS = 512;
 constexpr int TC_SMEM = 227 * 1024;
 
-template <int T, int BN>
+template <int T, int BN, bool LO>
 struct TcCfg {
     using L = Lv<T>;
-    static constexpr bool FOLD = L::G16, SPLIT = T == QS_Q6_K;
-    static constexpr int SUMS = !L::HASMIN ? 0 : L::G16 ? 2 : 1, PLANES = 1 + SUMS;
-    static constexpr int A_BYTES = TC_M * 128, A_ALL = A_BYTES * (SPLIT ? 2 : 1), B_BYTES = BN * 128;
-    static constexpr int P_BYTES = 2 * PLANES * BN * 4, X_BYTES = B_BYTES + P_BYTES;  // one bulk copy
-    static constexpr int OFF_B = A_ALL, OFF_P = OFF_B + B_BYTES, OFF_D = OFF_P + P_BYTES;
-    static constexpr int STAGE = (OFF_D + 2 * PLANES * TC_M * 4 + 1023) / 1024 * 1024;
-    static constexpr int FIT = (TC_SMEM - 4096) / STAGE, NS = FIT > 6 ? 6 : FIT;
+    static constexpr bool SPLIT = LO && T == QS_Q6_K;
+    static constexpr int SUMS = !L::HASMIN ? 0 : L::G16 ? 2 : 1;
+    static constexpr int GROUP = L::FOLD ? 4 : 0;  // stages that share an accumulator; 0: one per unit
+    static constexpr int A_BYTES = TC_M * 128, A_ALL = A_BYTES * (SPLIT ? 2 : 1), B_BYTES = BN * 128, B_ALL = B_BYTES * (LO ? 2 : 1);
+    static constexpr int P_BYTES = 2 * SUMS * BN * 4, X_BYTES = B_ALL + P_BYTES;  // one bulk copy
+    static constexpr int OFF_B = A_ALL, OFF_P = OFF_B + B_ALL, OFF_D = OFF_P + P_BYTES;
+    // weight scales [unit][128], then minima [unit][half][128]
+    static constexpr int STAGE = (OFF_D + 2 * (1 + SUMS) * TC_M * 4 + 1023) / 1024 * 1024;
+    static constexpr int FIT = (TC_SMEM - 4096) / STAGE, NS = FIT > 8 ? 8 : FIT;
     static constexpr int NB = BN == 256 ? 2 : 4;       // accumulators in tensor memory
-    static constexpr int COLS = NB * BN < 32 ? 32 : NB * BN;
+    static constexpr int COLS = NB * BN;
     // 256 columns need 128 registers a thread for the sums alone: registers move from the other
     // warpgroups to the two with the sums (192, 192, 88, 40 a thread of the 128 at launch)
     static constexpr bool MOVE = BN == 256;
@@ -116,50 +127,72 @@ __device__ __forceinline__ void word_halves(uint32_t w, __half2 bias, __half2* h
 }
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 
-// The slots' Q8_0 rows as the matrix unit reads them, [chunk][stage]: BN rows of 64 float16 levels
-// (two units) in the 128-byte swizzle, then [unit][plane][slot] floats (scale, scale * sum of levels of
-// the unit or of its halves). Rows without a slot are zero. One CTA per stage and chunk.
-template <int BN, int SUMS>
-__global__ void __launch_bounds__(256) xpack_kernel(MmArgs a, uint8_t* out) {
-    constexpr int X_BYTES = BN * 128 + 2 * (1 + SUMS) * BN * 4;
+// The slots' Q8_0 rows as the matrix unit reads them, [chunk][stage]: BN rows of 64 float16 values
+// (two units) in the 128-byte swizzle, with LO the rows' low parts behind them, then [unit][plane][slot]
+// floats (scale * sum of levels of the unit or of its halves); all times the row's power of two,
+// whose inverse goes to xs[chunk][slot]. Rows without a slot are zero. One warp per row: the largest
+// scale first, then lane l the units l, l + 32, ...
+template <int BN, int SUMS, bool LO>
+__global__ void __launch_bounds__(256) xpack_kernel(MmArgs a, uint8_t* out, float* xs) {
+    constexpr int B_BYTES = BN * 128, B_ALL = B_BYTES * (LO ? 2 : 1), X_BYTES = B_ALL + 2 * SUMS * BN * 4;
     const Chunk ch = find_chunk<BN>(a, blockIdx.y);
     if (ch.group < 0 || (a.order && ch.group == a.n_exp)) return;
-    const int stage = blockIdx.x;
-    uint8_t* o = out + ((int64_t)blockIdx.y * gridDim.x + stage) * X_BYTES;
-    for (int i = threadIdx.x; i < 2 * BN; i += 256) {
-        const int t = i >> 1, uu = i & 1, u = 2 * stage + uu;
+    const int lane = threadIdx.x & 31, t = blockIdx.x * 8 + (threadIdx.x >> 5), stages = (a.units + 1) / 2;
+    const bool live = ch.lo + t < ch.hi;
+    const int slot = live ? (a.order ? __ldg(a.order + ch.lo + t) : ch.lo + t) : 0;
+    const uint8_t* row = a.x + (int64_t)(slot / a.x_div) * a.x_row;
+    uint32_t top = 0;  // largest |scale| as float16 bits; above 0x7BFF: inf or NaN
+    if (live)
+        for (int u = lane; u < a.units; u += 32) top = max(top, ld_u16<1>(row + (int64_t)u * 34) & 0x7FFFu);
+    top = __reduce_max_sync(0xffffffffu, top);
+    // 2^(7 - exponent): scales below 2^8, values below 2^15
+    float up = 1.0f;
+    if (top > 0 && top <= 0x7BFFu) up = __uint_as_float((uint32_t)(127 + 7 + 127 - (int)(__float_as_uint(h2f(top)) >> 23)) << 23);
+    if (lane == 0) xs[(int64_t)blockIdx.y * BN + t] = 1.0f / up;
+    uint8_t* o = out + (int64_t)blockIdx.y * stages * X_BYTES;
+    for (int u = lane; u < 2 * stages; u += 32) {
         uint32_t q[8] = {0, 0, 0, 0, 0, 0, 0, 0};
         float d = 0.0f;
-        if (ch.lo + t < ch.hi && u < a.units) {
-            const int slot = a.order ? __ldg(a.order + ch.lo + t) : ch.lo + t;
-            const uint8_t* b = a.x + (int64_t)(slot / a.x_div) * a.x_row + (int64_t)u * 34;
-            ld_words<8, 1>(b + 2, q);
-            d = h2f(ld_u16<1>(b));
+        if (live && u < a.units) {
+            ld_words<8, 1>(row + (int64_t)u * 34 + 2, q);
+            d = h2f(ld_u16<1>(row + (int64_t)u * 34)) * up;
         }
-        const __half2 bias = __float2half2_rn(1152.0f);
+        uint8_t* st = o + (int64_t)(u >> 1) * X_BYTES;
+        const int uu = u & 1;
 #pragma unroll
         for (int c = 0; c < 4; c++) {
-            __half2 h[4];
-            word_halves(q[2 * c] ^ 0x80808080u, bias, h);
-            word_halves(q[2 * c + 1] ^ 0x80808080u, bias, h + 2);
-            *reinterpret_cast<uint4*>(o + t * 128 + (((4 * uu + c) ^ (t & 7)) << 4)) = make_uint4(h2_bits(h[0]), h2_bits(h[1]), h2_bits(h[2]), h2_bits(h[3]));
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                // halves of word 2 c + e / 2: bytes 0, 2 or 1, 3
+                const uint32_t w = q[2 * c + (e >> 1)] >> (8 * (e & 1));
+                const float v0 = d * (float)(int8_t)w, v1 = d * (float)(int8_t)(w >> 16);
+                const __half2 h = __floats2half2_rn(v0, v1);
+                const float2 f = __half22float2(h);
+                hi[e] = h2_bits(h);
+                if constexpr (LO) lo[e] = h2_bits(__floats2half2_rn(v0 - f.x, v1 - f.y));
+            }
+            uint8_t* p = st + t * 128 + (((4 * uu + c) ^ (t & 7)) << 4);
+            *reinterpret_cast<uint4*>(p) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            if constexpr (LO) *reinterpret_cast<uint4*>(p + B_BYTES) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
-        float* p = reinterpret_cast<float*>(o + BN * 128) + uu * (1 + SUMS) * BN + t;
-        p[0] = d;
-        const int s0 = sum16(make_uint4(q[0], q[1], q[2], q[3])), s1 = sum16(make_uint4(q[4], q[5], q[6], q[7]));
-        if constexpr (SUMS == 1) p[BN] = d * (float)(s0 + s1);
-        if constexpr (SUMS == 2) {
-            p[BN] = d * (float)s0;
-            p[2 * BN] = d * (float)s1;
+        if constexpr (SUMS > 0) {
+            float* p = reinterpret_cast<float*>(st + B_ALL) + uu * SUMS * BN + t;
+            const int s0 = sum16(make_uint4(q[0], q[1], q[2], q[3])), s1 = sum16(make_uint4(q[4], q[5], q[6], q[7]));
+            if constexpr (SUMS == 1) p[0] = d * (float)(s0 + s1);
+            else {
+                p[0] = d * (float)s0;
+                p[BN] = d * (float)s1;
+            }
         }
     }
 }
 
-template <int T, int BN>
-__global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8_t* xp) {
+template <int T, int BN, bool LO>
+__global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8_t* xp, const float* xs) {
     using L = Lv<T>;
-    using C = TcCfg<T, BN>;
-    constexpr int UPB = L::QK / 32, SUMS = C::SUMS, PLANES = C::PLANES, NS = C::NS, NB = C::NB;
+    using C = TcCfg<T, BN, LO>;
+    constexpr int UPB = L::QK / 32, SUMS = C::SUMS, NS = C::NS, NB = C::NB, GROUP = C::GROUP;
     constexpr int HALF = BN / 2;  // columns of a warp
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[3 * NS + 2 * NB];
@@ -192,7 +225,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
     const uint32_t tmem = s_tmem;
 
     const int n0 = blockIdx.x * TC_M, cnt = ch.hi - ch.lo;
-    const int stages = (a.units + 1) / 2, per = (stages + a.splits - 1) / a.splits;
+    const int stages = (a.units + 1) / 2, per = ((stages + a.splits - 1) / a.splits + 3) & ~3;  // whole superblocks
     const bool real = !a.order || ch.group < a.n_exp;
     const int k0 = blockIdx.z * per, k1 = real ? min(k0 + per, stages) : k0;
 
@@ -202,7 +235,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
             if (lane == 0) {
                 // D float32, A and B float16 K-major, N = BN, M = 128
                 constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(TC_M >> 4) << 24);
-                int unit = 0;
+                int n_acc = 0;  // accumulators begun
                 bool ok = true;
                 for (int k = k0; k < k1 && ok; k++) {
                     const int i = k - k0, s = i % NS, ph = (i / NS) & 1;
@@ -210,17 +243,25 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint32_t st = ring + s * C::STAGE;
-                    for (int uu = 0; uu < 2; uu++, unit++) {
-                        const int b = unit % NB;
-                        if (!(ok = mbar_wait(acc_empty + 8 * b, ((unit / NB) & 1) ^ 1, a.fault))) break;
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    for (int uu = 0; uu < 2; uu++) {
+                        const bool first = GROUP ? uu == 0 && i % GROUP == 0 : true;
+                        const bool last = GROUP ? uu == 1 && (i % GROUP == GROUP - 1 || k + 1 == k1) : true;
+                        const int b = n_acc % NB;
+                        if (first) {
+                            if (!(ok = mbar_wait(acc_empty + 8 * b, ((n_acc / NB) & 1) ^ 1, a.fault))) break;
+                            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        }
 #pragma unroll
-                        for (int h = 0; h < (C::SPLIT ? 2 : 1); h++)
-#pragma unroll
-                            for (int kk = 0; kk < 2; kk++)
-                                mma_f16(tmem + b * BN, operand_desc(st + h * C::A_BYTES + uu * 64 + kk * 32), operand_desc(st + C::OFF_B + uu * 64 + kk * 32),
-                                        idesc, h + kk > 0);
-                        mma_commit(acc_full + 8 * b);
+                        for (int kk = 0; kk < 2; kk++) {
+                            const uint32_t at = uu * 64 + kk * 32;
+                            mma_f16(tmem + b * BN, operand_desc(st + at), operand_desc(st + C::OFF_B + at), idesc, !first || kk > 0);
+                            if constexpr (LO) mma_f16(tmem + b * BN, operand_desc(st + at), operand_desc(st + C::OFF_B + C::B_BYTES + at), idesc, true);
+                            if constexpr (C::SPLIT) mma_f16(tmem + b * BN, operand_desc(st + C::A_BYTES + at), operand_desc(st + C::OFF_B + at), idesc, true);
+                        }
+                        if (last) {
+                            mma_commit(acc_full + 8 * b);
+                            n_acc++;
+                        }
                     }
                     if (ok) mma_commit(empty + 8 * s);
                 }
@@ -274,7 +315,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
                     word_halves(L::SIGNED ? q[2 * c] ^ 0x80808080u : q[2 * c], bias, h);
                     word_halves(L::SIGNED ? q[2 * c + 1] ^ 0x80808080u : q[2 * c + 1], bias, h + 2);
                     uint8_t* o = st + row * 128 + (((4 * uu + c) ^ (row & 7)) << 4);
-                    if constexpr (C::FOLD) {
+                    if constexpr (L::FOLD) {
                         const __half2 sc = __half2half2(__int2half_rn(L::sub(raw[uu], j, c >> 1)));
                         __half2 p[4];
 #pragma unroll
@@ -289,11 +330,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
                     }
                     *reinterpret_cast<uint4*>(o) = make_uint4(h2_bits(h[0]), h2_bits(h[1]), h2_bits(h[2]), h2_bits(h[3]));
                 }
-                float* d = reinterpret_cast<float*>(st + C::OFF_D) + uu * PLANES * TC_M + row;
-                if constexpr (C::FOLD) d[0] = L::base(raw[uu]);
-                else d[0] = dl[0];
-                if constexpr (SUMS >= 1) d[TC_M] = -ml[0];
-                if constexpr (SUMS == 2) d[2 * TC_M] = -ml[1];
+                float* d = reinterpret_cast<float*>(st + C::OFF_D) + row;
+                if constexpr (L::FOLD) d[uu * TC_M] = L::base(raw[uu]);
+                else d[uu * TC_M] = dl[0];
+#pragma unroll
+                for (int p = 0; p < SUMS; p++) d[(2 + uu * SUMS + p) * TC_M] = -ml[p];
             }
             load(k + 1);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -307,22 +348,33 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
         f32x2 acc[HALF / 2];
 #pragma unroll
         for (int i = 0; i < HALF / 2; i++) acc[i] = 0ull;
-        int unit = 0;
+        int n_acc = 0;  // accumulators read
         bool ok = true;
         for (int k = k0; k < k1 && ok; k++) {
             const int i = k - k0, s = i % NS, ph = (i / NS) & 1;
             ok = mbar_wait(full_w + 8 * s, ph, a.fault) && mbar_wait(full_x + 8 * s, ph, a.fault);
             if (!ok) break;
             const uint8_t* st = ring_p + s * C::STAGE;
-            for (int uu = 0; uu < 2; uu++, unit++) {
-                const int b = unit % NB;
-                const float* d = reinterpret_cast<const float*>(st + C::OFF_D) + uu * PLANES * TC_M + row;
-                const float4* x = reinterpret_cast<const float4*>(st + C::OFF_P + (uu * PLANES * BN + c0) * 4);
-                const f32x2 dl = f2_splat(d[0]);
-                f32x2 ml[SUMS ? SUMS : 1];
+            const float* d = reinterpret_cast<const float*>(st + C::OFF_D) + row;
+            // minima: the planes' values of 4 columns to all lanes at once
 #pragma unroll
-                for (int p = 0; p < SUMS; p++) ml[p] = f2_splat(d[(1 + p) * TC_M]);
-                if (!(ok = mbar_wait(acc_full + 8 * b, (unit / NB) & 1, a.fault))) break;
+            for (int p = 0; p < 2 * SUMS; p++) {
+                const f32x2 ml = f2_splat(d[(2 + p) * TC_M]);
+                const float4* x = reinterpret_cast<const float4*>(st + C::OFF_P + (p * BN + c0) * 4);
+#pragma unroll
+                for (int c = 0; c < HALF / 4; c++) {
+                    const float4 v = x[c];
+                    acc[2 * c] = f2_fma(ml, f2_pack(v.x, v.y), acc[2 * c]);
+                    acc[2 * c + 1] = f2_fma(ml, f2_pack(v.z, v.w), acc[2 * c + 1]);
+                }
+            }
+#pragma unroll
+            for (int uu = 0; uu < 2; uu++) {
+                if (GROUP && (uu == 0 || (i % (GROUP ? GROUP : 1) != GROUP - 1 && k + 1 < k1))) continue;
+                const int b = n_acc % NB;
+                const f32x2 dl = f2_splat(d[uu * TC_M]);
+                if (!(ok = mbar_wait(acc_full + 8 * b, (n_acc / NB) & 1, a.fault))) break;
+                n_acc++;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + b * BN + c0;
                 uint32_t v[2][16];
@@ -333,19 +385,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
                     if (bt + 1 < NBT) tmem_ld16(at + 16 * (bt + 1), v[(bt + 1) & 1]);
                     const uint32_t* r = v[bt & 1];
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        const float4 xv = x[bt * 4 + c];
-                        f32x2& a0 = acc[bt * 8 + 2 * c];
-                        f32x2& a1 = acc[bt * 8 + 2 * c + 1];
-                        a0 = f2_fma(f2_mul_z(dl, f2_pack(xv.x, xv.y)), f2_pack(__uint_as_float(r[4 * c]), __uint_as_float(r[4 * c + 1])), a0);
-                        a1 = f2_fma(f2_mul_z(dl, f2_pack(xv.z, xv.w)), f2_pack(__uint_as_float(r[4 * c + 2]), __uint_as_float(r[4 * c + 3])), a1);
-#pragma unroll
-                        for (int p = 0; p < SUMS; p++) {
-                            const float4 sv = x[(1 + p) * (BN / 4) + bt * 4 + c];
-                            a0 = f2_fma(ml[p], f2_pack(sv.x, sv.y), a0);
-                            a1 = f2_fma(ml[p], f2_pack(sv.z, sv.w), a1);
-                        }
-                    }
+                    for (int c = 0; c < 8; c++)
+                        acc[bt * 8 + c] = f2_fma(dl, f2_pack(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1])), acc[bt * 8 + c]);
                     if (bt + 1 < NBT) tmem_wait_ld(v[(bt + 1) & 1]);
                     if (bt + 2 == NBT || NBT == 1) {  // the last loads are in registers
                         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -390,6 +431,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
             } else {
                 v = *reinterpret_cast<const float4*>(o + t * C::OUT_PITCH + 4 * lane);
             }
+            const float sx = real ? __ldg(xs + (int64_t)blockIdx.y * BN + t) : 1.0f;
+            v = make_float4(v.x * sx, v.y * sx, v.z * sx, v.w * sx);
             store_row4(out, at, type, v, lane, n0, a.n, vec);
         }
     }
@@ -400,20 +443,22 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
     }
 }
 
-template <int T, int BN>
-cudaError_t launch_tc_t(const MmArgs& a, uint8_t* xp, const LaunchCtx& ctx) {
-    using C = TcCfg<T, BN>;
+template <int T, int BN, bool LO>
+cudaError_t launch_tc_t(const MmArgs& a, void* ws, const LaunchCtx& ctx) {
+    using C = TcCfg<T, BN, LO>;
     const int64_t chunks = max_chunks(a, BN);
     if (chunks > 65535) return cudaErrorInvalidConfiguration;
-    xpack_kernel<BN, C::SUMS><<<dim3((a.units + 1) / 2, (unsigned)chunks), 256, 0, ctx.stream>>>(a, xp);
+    float* xs = static_cast<float*>(ws);
+    uint8_t* xp = static_cast<uint8_t*>(ws) + xs_bytes(chunks, BN);
+    xpack_kernel<BN, C::SUMS, LO><<<dim3(BN / 8, (unsigned)chunks), 256, 0, ctx.stream>>>(a, xp, xs);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    e = cudaFuncSetAttribute(tc_kernel<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::BYTES);
-    if (e != cudaSuccess) return e;
+    auto kernel = tc_kernel<T, BN, LO>;
+    if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::BYTES)) != cudaSuccess) return e;
     if constexpr (C::MOVE) {  // the warpgroups' shares must be there at launch
         static const int regs = [] {
             cudaFuncAttributes f;
-            return cudaFuncGetAttributes(&f, tc_kernel<T, BN>) == cudaSuccess ? f.numRegs : 0;
+            return cudaFuncGetAttributes(&f, tc_kernel<T, BN, LO>) == cudaSuccess ? f.numRegs : 0;
         }();
         if (regs * TC_THREADS < 128 * (192 + 192 + 88 + 40)) return cudaErrorInvalidConfiguration;
     }
@@ -430,27 +475,17 @@ cudaError_t launch_tc_t(const MmArgs& a, uint8_t* xp, const LaunchCtx& ctx) {
     at[0].val.clusterDim.z = (unsigned)a.splits;
     cfg.attrs = at;
     cfg.numAttrs = a.splits > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, tc_kernel<T, BN>, a, static_cast<const uint8_t*>(xp));
+    return cudaLaunchKernelEx(&cfg, kernel, a, static_cast<const uint8_t*>(xp), static_cast<const float*>(xs));
 }
 
 template <int T>
-cudaError_t launch_tc(const MmArgs& a, int bn, uint8_t* xp, const LaunchCtx& ctx) {
-    return bn == 32 ? launch_tc_t<T, 32>(a, xp, ctx) : bn == 64 ? launch_tc_t<T, 64>(a, xp, ctx) : bn == 128 ? launch_tc_t<T, 128>(a, xp, ctx) : launch_tc_t<T, 256>(a, xp, ctx);
+cudaError_t launch_tc(const MmArgs& a, int bn, bool lo, void* ws, const LaunchCtx& ctx) {
+    if (lo) return bn == 32 ? launch_tc_t<T, 32, true>(a, ws, ctx) : bn == 64 ? launch_tc_t<T, 64, true>(a, ws, ctx) : launch_tc_t<T, 128, true>(a, ws, ctx);
+    return bn == 32   ? launch_tc_t<T, 32, false>(a, ws, ctx)
+           : bn == 64 ? launch_tc_t<T, 64, false>(a, ws, ctx)
+           : bn == 128 ? launch_tc_t<T, 128, false>(a, ws, ctx) : launch_tc_t<T, 256, false>(a, ws, ctx);
 }
 
 }  // namespace
-
-int64_t mm_tc_workspace(int64_t units, int64_t chunks, int bn, int planes) {
-    return chunks * ((units + 1) / 2) * ((int64_t)bn * 128 + 2 * planes * bn * 4);
-}
-
-cudaError_t launch_mm_tc(int type, const MmArgs& a, int bn, void* xp, const LaunchCtx& ctx) {
-    switch (type) {
-#define X(T) case T: return launch_tc<T>(a, bn, static_cast<uint8_t*>(xp), ctx);
-        QS_FOR_TYPES(X)
-#undef X
-    default: return cudaErrorInvalidValue;
-    }
-}
 
 }  // namespace qs

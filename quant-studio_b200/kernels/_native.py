@@ -69,7 +69,7 @@ def lib() -> ctypes.CDLL:
             L.qs_route.argtypes = [c_vp, c_i, c_i64, c_i64, c_i, c_i, c_i, c_vp, c_i, c_i, c_i, c_i, ctypes.c_float, c_vp, c_vp, c_vp]
             L.qs_expert_plan.argtypes = [c_vp, c_i64, c_i, c_vp, c_vp, c_vp]
             L.qs_matmul.argtypes = [c_i, c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_i, c_i64, c_vp, c_i64, c_vp]
-            L.qs_matmul_workspace.argtypes = [c_i, c_i64, c_i64, c_i64, p_i64]
+            L.qs_matmul_workspace.argtypes = [c_i, c_i64, c_i64, c_i64, c_i, p_i64]
             L.qs_matmul_experts.argtypes = [c_i, c_vp, c_i64, c_i64, c_i, c_i64, c_i64, c_vp, c_i64, c_i, c_vp, c_vp, c_vp, c_i64, c_i,
                                             c_vp, c_vp, c_i, c_i64, c_vp, c_i64, c_vp]
             L.qs_matmul_experts_workspace.argtypes = [c_i, c_i, c_i64, c_i64, c_i64, c_i, c_i, c_i, p_i64]

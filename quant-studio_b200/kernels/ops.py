@@ -206,7 +206,7 @@ def matmul(blocks: torch.Tensor, ggml_type: int, x_q8: torch.Tensor, out_dtype: 
     """
     dev, k = _packed_args(blocks, ggml_type, x_q8, 2, out_dtype)
     n, rows = blocks.shape[0], x_q8.shape[0]
-    size = _matmul_workspace(int(ggml_type), n, k, rows)
+    size = _matmul_workspace(int(ggml_type), n, k, rows, SRC_IDS[out_dtype])
     out = torch.empty((rows, n), dtype=out_dtype, device=blocks.device)
     ws = torch.empty(size, dtype=torch.uint8, device=blocks.device) if size else None
     check(lib().qs_matmul(int(ggml_type), blocks.data_ptr(), _row_stride(blocks), n, k, x_q8.data_ptr(), _row_stride(x_q8), rows,
@@ -242,7 +242,7 @@ def matmul_experts(blocks: torch.Tensor, ggml_type: int, x_q8: torch.Tensor, pla
     row = blocks.stride(1) if n > 1 else -(-blocks.shape[2] // 16) * 16  # a stride that nothing steps over fits any alignment
     expert = blocks.stride(0) if experts > 1 else n * row
     per_slot, summed = int(rows != tokens), int(weights is not None)
-    size = _experts_workspace(int(ggml_type), experts, n, k, tokens, top_k, per_slot, summed)
+    size = _experts_workspace(int(ggml_type), experts, n, k, tokens, top_k, summed, SRC_IDS[out_dtype])
     out = torch.empty(shape, dtype=out_dtype, device=blocks.device)
     ws = torch.empty(size, dtype=torch.uint8, device=blocks.device) if size else None
     order = plan.table.data_ptr()

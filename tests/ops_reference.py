@@ -33,14 +33,15 @@ def decode64(blocks, qtype):
     return dequantize(flat, GTYPE[qtype]).astype(np.float64).reshape(*blocks.shape[:-1], -1)
 
 
-def product(xq, w, qtype):
+def product(xq, w, qtype, out="float32"):
     """(y, bound): the 64-bit product and how far a float32 evaluation may be from it.
 
     Per unit of 32 values the integer sums are exact; a unit adds up to 4 terms (two halves, two
     minima), each with a rounded scale product and a rounded addition, and the terms of a row
     are added in any order: at most (8 units + 8) roundings, each of at most half a step of
     the sum of the terms' magnitudes. Minima are separate terms: |dl l| <= |w| + |ml|. gguf-py's
-    decode rounds each weight once more.
+    decode rounds each weight once more. For bfloat16 results the activations may be rounded to
+    float16 (half a step: 2^-11 of a value).
     """
     x, ww = decode64(xq, "q8_0"), decode64(w, qtype)
     mag = np.abs(ww)
@@ -50,8 +51,8 @@ def product(xq, w, qtype):
         z[..., lo:hi] = 0
         mag = mag + 2 * np.abs(decode64(z.reshape(w.shape), qtype))
     y = x @ np.swapaxes(ww, -1, -2)
-    units = x.shape[-1] // 32
-    return y, (8 * units + 8) * 2.0 ** -24 * (np.abs(x) @ np.swapaxes(mag, -1, -2))
+    steps = (8 * (x.shape[-1] // 32) + 8) * 2.0 ** -24 + (2.0 ** -11 if out == "bfloat16" else 0.0)
+    return y, steps * (np.abs(x) @ np.swapaxes(mag, -1, -2))
 
 
 def rounding(y, dtype):

@@ -197,7 +197,7 @@ def test_matmul_sizes(qtype, rows, n, k, dtype):
     w = ref.random_blocks(qtype, (n,), k, rng)
     x = ref.random_blocks("q8_0", (rows,), k, rng)
     got = ops.matmul(cuda(w), int(ref.GTYPE[qtype]), cuda(x), out_dtype=DT[dtype])
-    check_product(got, *ref.product(x, w, qtype))
+    check_product(got, *ref.product(x, w, qtype, dtype))
 
 
 @pytest.mark.parametrize("qtype", ["q8_0", "q4_k", "q6_k"])
@@ -219,7 +219,7 @@ def test_matmul_strides(qtype, rows):
     L = _native.lib()
     import ctypes
     size = ctypes.c_int64()
-    _native.check(L.qs_matmul_workspace(int(ref.GTYPE[qtype]), n, k, rows, ctypes.byref(size)))
+    _native.check(L.qs_matmul_workspace(int(ref.GTYPE[qtype]), n, k, rows, 0, ctypes.byref(size)))
     ws = torch.empty(max(size.value, 1), dtype=torch.uint8, device="cuda")
     out = torch.full((rows + 1, n + 5), 7.0, device="cuda")
     wc, xc = cuda(w), cuda(x)
@@ -247,7 +247,7 @@ def test_matmul_extremes(rows):
     assert not torch.isfinite(got[:, [3, 130]]).any() and torch.equal(got[:, keep], clean[:, keep])
 
 
-def experts_want(x, w, qtype, ids, weights, per_slot):
+def experts_want(x, w, qtype, ids, weights, per_slot, out="float32"):
     t, k = ids.shape
     n = w.shape[1]
     y, b = np.zeros((t, k, n)), np.zeros((t, k, n))
@@ -255,7 +255,7 @@ def experts_want(x, w, qtype, ids, weights, per_slot):
         for j in range(k):
             if 0 <= ids[i, j] < w.shape[0]:
                 r = i * k + j if per_slot else i
-                yy, bb = ref.product(x[r:r + 1], w[ids[i, j]], qtype)
+                yy, bb = ref.product(x[r:r + 1], w[ids[i, j]], qtype, out)
                 y[i, j], b[i, j] = yy[0], bb[0]
     if weights is None:
         return y, b
@@ -338,7 +338,7 @@ def test_layer(tokens):
     check_product(got_up, up, ub)
     act = _native.quantize(8, torch.relu(got_up).square().reshape(-1, 256), None).cpu().numpy()
     wts = (1.5 * pick / pick.sum(1, keepdims=True)).astype(np.float32)
-    y, b = experts_want(act, wd.cpu().numpy(), "q6_k", idn, wts, True)
+    y, b = experts_want(act, wd.cpu().numpy(), "q6_k", idn, wts, True, "bfloat16")
     # weights: the logits' error in the scores, twice (score and sum), and their rounding
     slack = (4 * zb.max() + 2.0 ** -22) * np.abs(experts_want(act, wd.cpu().numpy(), "q6_k", idn, None, True)[0]).sum(1) * 1.5
     check_product(out, y, b + slack)
