@@ -106,6 +106,9 @@ template <> struct Lv<QS_Q4_1> {
             q[4 + i] = (r[1 + i] >> 4) & 0x0F0F0F0Fu;
         }
     }
+    // the block's minima, one per unit (per 16 values for Q2_K)
+    template <int AL>
+    __device__ static void minima(const uint8_t* b, float* m) { m[0] = -h2f(ld_u16<AL>(b + 2)); }
 };
 
 template <> struct Lv<QS_Q5_0> {
@@ -145,6 +148,9 @@ template <> struct Lv<QS_Q5_1> {
             q[4 + i] = ((r[2 + i] >> 4) & 0x0F0F0F0Fu) | (bits_to_bytes(r[1] >> (16 + 4 * i)) << 4);
         }
     }
+    // the block's minima, one per unit (per 16 values for Q2_K)
+    template <int AL>
+    __device__ static void minima(const uint8_t* b, float* m) { m[0] = -h2f(ld_u16<AL>(b + 2)); }
 };
 
 template <> struct Lv<QS_Q8_0> {
@@ -187,6 +193,15 @@ template <> struct Lv<QS_Q2_K> {
     }
     __device__ static float base(const uint32_t* r) { return h2f(r[8] & 0xFFFFu); }
     __device__ static int sub(const uint32_t* r, int, int h) { return (int)((r[9] >> (8 * h)) & 15u); }
+    template <int AL>
+    __device__ static void minima(const uint8_t* b, float* m) {
+        uint32_t s[4], d[1];
+        ld_words<4, AL>(b, s);
+        ld_words<1, AL>(b + 80, d);
+        const float dm = h2f(d[0] >> 16);
+#pragma unroll
+        for (int i = 0; i < 16; i++) m[i] = dm * (float)((s[i / 4] >> (8 * (i & 3) + 4)) & 15u);
+    }
 };
 
 template <> struct Lv<QS_Q3_K> {
@@ -250,6 +265,18 @@ template <> struct Lv<QS_Q4_K> {
         k4_scale_min(r + 9, j, sc, mn);
         return (int)sc;
     }
+    template <int AL>
+    __device__ static void minima(const uint8_t* b, float* m) {
+        uint32_t h[4];
+        ld_words<4, AL>(b, h);
+        const float dm = h2f(h[0] >> 16);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            float sc, mn;
+            k4_scale_min(h + 1, j, sc, mn);
+            m[j] = dm * mn;
+        }
+    }
 };
 
 template <> struct Lv<QS_Q5_K> {
@@ -276,6 +303,18 @@ template <> struct Lv<QS_Q5_K> {
         float sc, mn;
         k4_scale_min(r + 9, j, sc, mn);
         return (int)sc;
+    }
+    template <int AL>
+    __device__ static void minima(const uint8_t* b, float* m) {
+        uint32_t h[4];
+        ld_words<4, AL>(b, h);
+        const float dm = h2f(h[0] >> 16);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            float sc, mn;
+            k4_scale_min(h + 1, j, sc, mn);
+            m[j] = dm * mn;
+        }
     }
 };
 

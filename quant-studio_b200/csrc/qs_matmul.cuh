@@ -139,7 +139,7 @@ cudaError_t launch_mm_few(int type, const MmArgs& a, const LaunchCtx& ctx);
 // (1 with minima, 2 with minima per 16 values, else 0)
 inline int64_t xs_bytes(int64_t chunks, int bn) { return (chunks * bn * 4 + 255) / 256 * 256; }
 inline int64_t mm_tc_workspace(int64_t units, int64_t chunks, int bn, bool lo, int sums) {
-    return xs_bytes(chunks, bn) + chunks * ((units + 1) / 2) * ((int64_t)bn * 128 * (lo ? 2 : 1) + 2 * sums * bn * 4);
+    return xs_bytes(chunks, bn) + chunks * ((units + 1) / 2 + (units * sums + 63) / 64) * (int64_t)bn * 128 * (lo ? 2 : 1);
 }
 // by the file that holds the type
 cudaError_t launch_mm_tc_legacy(int type, const MmArgs& a, int bn, bool lo, void* ws, const LaunchCtx& ctx);

@@ -10,22 +10,27 @@
 // below 2^15) it is float16 hi + lo, exact together down to 2^-39 of the row's largest. LO: the
 // products use both parts (Q6_K: hi hi, hi lo, lo hi), for float32 and float16 results. For
 // bfloat16 results hi alone is multiplied: its rounding, 2^-12 of a value, is 1/8 of the result's.
-// Minima are one more term, - ml[n, unit] * (scale * sum of levels)[t, unit], per 32 (16) values.
+// Minima: - ml[n, unit] * (scale * sum of levels)[t, unit] is a product of its own, with K / 32 (K / 16
+// for Q2_K) terms; it follows the levels as further stages of 64 terms, float16 like the activations
+// (LO: hi and lo of both), the weights' side times a power of two per row and 32 terms.
 //
 // A pass over K = 32 of a 128 x 256 tile is 271 cycles of the matrix unit (540 with LO). Scaling every 32
 // values by both operands' scales instead, with exact integers in D, was built first and took 1235 us
 // for 2048 slots of Q4_K 14336 x 4096: three float32 operations per value and unit are 768 cycles
 // (a packed f32x2 operation takes two), an SM has no more than 128 lanes.
 //
-// Roles in a CTA (one per SM, 16 warps):
-//   warps 0-7    own the tile's sums: lane = weight row, each warp half of the columns
-//   warps 8-11   unpack the weights: thread = row, two units per stage, block bytes loaded a stage ahead
-//   warp 12      issues the matrix products (and owns the tensor memory)
-//   warp 13      copies the activations' stage (one bulk copy: float16 rows as the matrix unit reads
-//                them, then the planes of scaled level sums), laid out beforehand by xpack_kernel
-// Stages are a ring in shared memory (full: unpacked + copied, empty: products done + planes
-// read); the accumulators are a ring in tensor memory. Every wait is bounded: one that runs out
-// records bit 0 of the fault word and its role leaves.
+// Roles in a CTA (one per SM, 12 warps, two of them idle):
+//   warps 0-7  unpack the weights (thread = row and unit of the stage, block bytes loaded PF stages
+//              ahead) and own the tile's sums (lane = weight row, each warp half of the columns),
+//              which they collect LAG stages behind
+//   warp 8     issues the matrix products (and owns the tensor memory)
+//   warp 9     copies the activations' stage (one bulk copy: float16 rows as the matrix unit reads
+//              them), laid out beforehand by xpack_kernel
+// Stages are a ring in shared memory (full: unpacked + copied, empty: products done); the
+// accumulators are a ring in tensor memory; the weights' scales are a longer ring of their own, which
+// no warp can lap: unpacking stage i waits for the products of stage i - NS, these for every warp's
+// stage i - NS, and that warp has then collected stage i - NS - 1 - LAG. Every wait is bounded: one that
+// runs out records bit 0 of the fault word and its role leaves.
 // The order of the 32 values within a unit does not matter to the sum; both operands use the one
 // that unpacks cheapest (word_halves).
 #pragma once
@@ -40,30 +45,35 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int TC_M = 128, TC_THREADS = 512;
+constexpr int TC_M = 128, TC_THREADS = 384;
 constexpr int TC_SMEM = 227 * 1024;
 
 template <int T, int BN, bool LO>
 struct TcCfg {
     using L = Lv<T>;
     static constexpr bool SPLIT = LO && T == QS_Q6_K;
-    static constexpr int SUMS = !L::HASMIN ? 0 : L::G16 ? 2 : 1;
+    static constexpr int SUMS = !L::HASMIN ? 0 : L::G16 ? 2 : 1;  // minima per unit
     static constexpr int GROUP = L::FOLD ? 4 : 0;  // stages that share an accumulator; 0: one per unit
-    static constexpr int A_BYTES = TC_M * 128, A_ALL = A_BYTES * (SPLIT ? 2 : 1), B_BYTES = BN * 128, B_ALL = B_BYTES * (LO ? 2 : 1);
-    static constexpr int P_BYTES = 2 * SUMS * BN * 4, X_BYTES = B_ALL + P_BYTES;  // one bulk copy
-    static constexpr int OFF_B = A_ALL, OFF_P = OFF_B + B_ALL, OFF_D = OFF_P + P_BYTES;
-    // weight scales [unit][128], then minima [unit][half][128]
-    static constexpr int STAGE = (OFF_D + 2 * (1 + SUMS) * TC_M * 4 + 1023) / 1024 * 1024;
-    static constexpr int FIT = (TC_SMEM - 4096) / STAGE, NS = FIT > 8 ? 8 : FIT;
+    static constexpr int A_BYTES = TC_M * 128, A_ALL = A_BYTES * (SPLIT ? 2 : 1), B_BYTES = BN * 128, X_BYTES = B_BYTES * (LO ? 2 : 1);
+    static constexpr int STAGE = A_ALL + X_BYTES;
+    static constexpr int LAG = GROUP ? 2 : 1;
+    // stages loaded ahead: as many as the registers next to the sums hold
+    static constexpr int PF = BN == 256 ? (L::WORDS <= 12 ? 2 : 1) : L::WORDS <= 6 ? 4 : L::WORDS <= 12 ? 3 : 2;
+    static constexpr int DR = 16;                      // ring of scales, [slot][unit][128]
+    static constexpr int D_BYTES = DR * 2 * TC_M * 4;
+    static constexpr int FIT = (TC_SMEM - 2048 - D_BYTES) / STAGE, NS = FIT > 8 ? 8 : FIT;
     static constexpr int NB = BN == 256 ? 2 : 4;       // accumulators in tensor memory
     static constexpr int COLS = NB * BN;
-    // 256 columns need 128 registers a thread for the sums alone: registers move from the other
-    // warpgroups to the two with the sums (192, 192, 88, 40 a thread of the 128 at launch)
+    // 256 columns are 128 registers a thread for the sums alone: the third warpgroup's registers move to
+    // the other two (232, 232, 40 a thread of the 168 at launch)
     static constexpr bool MOVE = BN == 256;
     static constexpr int OUT_PITCH = TC_M + 4;
-    static constexpr int BYTES = NS * STAGE + 1024;    // 1024 to align the ring
-    static_assert(NS >= 2, "two stages at least");
+    static constexpr int BYTES = NS * STAGE + D_BYTES + 1024;  // 1024 to align the ring
+    static_assert(NS >= LAG + 1 && DR >= NS + 1 + LAG, "ring lengths");
     static_assert(BN * OUT_PITCH * 4 <= NS * STAGE, "the tile leaves through the same memory");
+    // further stages with the minima of `units` units: 64 terms each, with LO once for the hi and
+    // once for the lo part of the weights' side
+    __host__ __device__ static int min_blocks(int units) { return (units * SUMS + 63) / 64; }
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -92,6 +102,11 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
         "{ .reg .b64 st; mbarrier.arrive.expect_tx.shared::cta.b64 st, [%3], %2; }\n"
         "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
         ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+template <class L>
+__device__ __forceinline__ float base_of(const uint32_t* r) {
+    if constexpr (L::FOLD) return L::base(r);
+    else return 0.0f;
 }
 // Shared-memory operand, K-major, rows of 128 bytes in the 128-byte swizzle: 8-row groups 1024
 // bytes apart
@@ -128,16 +143,17 @@ __device__ __forceinline__ void word_halves(uint32_t w, __half2 bias, __half2* h
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 
 // The slots' Q8_0 rows as the matrix unit reads them, [chunk][stage]: BN rows of 64 float16 values
-// (two units) in the 128-byte swizzle, with LO the rows' low parts behind them, then [unit][plane][slot]
-// floats (scale * sum of levels of the unit or of its halves); all times the row's power of two,
-// whose inverse goes to xs[chunk][slot]. Rows without a slot are zero. One warp per row: the largest
-// scale first, then lane l the units l, l + 32, ...
+// (two units) in the 128-byte swizzle, with LO the rows' low parts behind them; then as many stages as
+// hold 64 scaled level sums each (of a unit, or of its halves), times 2^-7. All times the row's power
+// of two, whose inverse goes to xs[chunk][slot]. Rows without a slot are zero. One warp per row: the
+// largest scale first, then lane l the units l, l + 32, ...
 template <int BN, int SUMS, bool LO>
 __global__ void __launch_bounds__(256) xpack_kernel(MmArgs a, uint8_t* out, float* xs) {
-    constexpr int B_BYTES = BN * 128, B_ALL = B_BYTES * (LO ? 2 : 1), X_BYTES = B_ALL + 2 * SUMS * BN * 4;
+    constexpr int B_BYTES = BN * 128, X_BYTES = B_BYTES * (LO ? 2 : 1);
     const Chunk ch = find_chunk<BN>(a, blockIdx.y);
     if (ch.group < 0 || (a.order && ch.group == a.n_exp)) return;
     const int lane = threadIdx.x & 31, t = blockIdx.x * 8 + (threadIdx.x >> 5), stages = (a.units + 1) / 2;
+    const int blocks = (a.units * SUMS + 63) / 64;
     const bool live = ch.lo + t < ch.hi;
     const int slot = live ? (a.order ? __ldg(a.order + ch.lo + t) : ch.lo + t) : 0;
     const uint8_t* row = a.x + (int64_t)(slot / a.x_div) * a.x_row;
@@ -145,44 +161,54 @@ __global__ void __launch_bounds__(256) xpack_kernel(MmArgs a, uint8_t* out, floa
     if (live)
         for (int u = lane; u < a.units; u += 32) top = max(top, ld_u16<1>(row + (int64_t)u * 34) & 0x7FFFu);
     top = __reduce_max_sync(0xffffffffu, top);
-    // 2^(7 - exponent): scales below 2^8, values below 2^15
+    // 2^(7 - exponent): scales below 2^8, values at most 2^15
     float up = 1.0f;
     if (top > 0 && top <= 0x7BFFu) up = __uint_as_float((uint32_t)(127 + 7 + 127 - (int)(__float_as_uint(h2f(top)) >> 23)) << 23);
     if (lane == 0) xs[(int64_t)blockIdx.y * BN + t] = 1.0f / up;
-    uint8_t* o = out + (int64_t)blockIdx.y * stages * X_BYTES;
-    for (int u = lane; u < 2 * stages; u += 32) {
+    uint8_t* o = out + (int64_t)blockIdx.y * (stages + blocks) * X_BYTES;
+    auto put_sum = [&](int p, float v) {  // term p of the level sums
+        const int c = (p & 63) >> 3;
+        uint8_t* at = o + (int64_t)(stages + (p >> 6)) * X_BYTES + t * 128 + ((c ^ (t & 7)) << 4) + (p & 7) * 2;
+        const __half h = __float2half_rn(v);
+        *reinterpret_cast<__half*>(at) = h;
+        if constexpr (LO) *reinterpret_cast<__half*>(at + B_BYTES) = __float2half_rn(v - __half2float(h));
+    };
+    const int last = max(2 * stages, SUMS ? blocks * 64 / SUMS : 0);
+    for (int u = lane; u < last; u += 32) {
         uint32_t q[8] = {0, 0, 0, 0, 0, 0, 0, 0};
         float d = 0.0f;
         if (live && u < a.units) {
             ld_words<8, 1>(row + (int64_t)u * 34 + 2, q);
             d = h2f(ld_u16<1>(row + (int64_t)u * 34)) * up;
         }
-        uint8_t* st = o + (int64_t)(u >> 1) * X_BYTES;
-        const int uu = u & 1;
+        if (u < 2 * stages) {
+            uint8_t* st = o + (int64_t)(u >> 1) * X_BYTES;
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-            uint32_t hi[4], lo[4];
+            for (int c = 0; c < 4; c++) {
+                uint32_t hi[4], lo[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                // halves of word 2 c + e / 2: bytes 0, 2 or 1, 3
-                const uint32_t w = q[2 * c + (e >> 1)] >> (8 * (e & 1));
-                const float v0 = d * (float)(int8_t)w, v1 = d * (float)(int8_t)(w >> 16);
-                const __half2 h = __floats2half2_rn(v0, v1);
-                const float2 f = __half22float2(h);
-                hi[e] = h2_bits(h);
-                if constexpr (LO) lo[e] = h2_bits(__floats2half2_rn(v0 - f.x, v1 - f.y));
+                for (int e = 0; e < 4; e++) {
+                    // halves of word 2 c + e / 2: bytes 0, 2 or 1, 3
+                    const uint32_t w = q[2 * c + (e >> 1)] >> (8 * (e & 1));
+                    const float v0 = d * (float)(int8_t)w, v1 = d * (float)(int8_t)(w >> 16);
+                    const __half2 h = __floats2half2_rn(v0, v1);
+                    const float2 f = __half22float2(h);
+                    hi[e] = h2_bits(h);
+                    if constexpr (LO) lo[e] = h2_bits(__floats2half2_rn(v0 - f.x, v1 - f.y));
+                }
+                uint8_t* p = st + t * 128 + (((4 * (u & 1) + c) ^ (t & 7)) << 4);
+                *reinterpret_cast<uint4*>(p) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                if constexpr (LO) *reinterpret_cast<uint4*>(p + B_BYTES) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
             }
-            uint8_t* p = st + t * 128 + (((4 * uu + c) ^ (t & 7)) << 4);
-            *reinterpret_cast<uint4*>(p) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            if constexpr (LO) *reinterpret_cast<uint4*>(p + B_BYTES) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
         if constexpr (SUMS > 0) {
-            float* p = reinterpret_cast<float*>(st + B_ALL) + uu * SUMS * BN + t;
             const int s0 = sum16(make_uint4(q[0], q[1], q[2], q[3])), s1 = sum16(make_uint4(q[4], q[5], q[6], q[7]));
-            if constexpr (SUMS == 1) p[0] = d * (float)(s0 + s1);
-            else {
-                p[0] = d * (float)s0;
-                p[BN] = d * (float)s1;
+            if (u < blocks * 64 / SUMS) {
+                if constexpr (SUMS == 1) put_sum(u, d * 0.0078125f * (float)(s0 + s1));
+                else {
+                    put_sum(2 * u, d * 0.0078125f * (float)s0);
+                    put_sum(2 * u + 1, d * 0.0078125f * (float)s1);
+                }
             }
         }
     }
@@ -192,7 +218,7 @@ template <int T, int BN, bool LO>
 __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8_t* xp, const float* xs) {
     using L = Lv<T>;
     using C = TcCfg<T, BN, LO>;
-    constexpr int UPB = L::QK / 32, SUMS = C::SUMS, NS = C::NS, NB = C::NB, GROUP = C::GROUP;
+    constexpr int UPB = L::QK / 32, SUMS = C::SUMS, NS = C::NS, NB = C::NB, GROUP = C::GROUP, LAG = C::LAG, PF = C::PF;
     constexpr int HALF = BN / 2;  // columns of a warp
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[3 * NS + 2 * NB];
@@ -202,12 +228,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
     if (ch.group < 0) return;  // the CTAs of a cluster share the chunk
     const uint32_t ring = (smem_u32(smem_raw) + 1023) & ~1023u;
     uint8_t* const ring_p = smem_raw + (ring - smem_u32(smem_raw));
+    float* const scales = reinterpret_cast<float*>(ring_p + NS * C::STAGE);
     const uint32_t full_w = smem_u32(bars), full_x = full_w + 8 * NS, empty = full_x + 8 * NS, acc_full = empty + 8 * NS, acc_empty = acc_full + 8 * NB;
     if (tid == 0) {
         for (int s = 0; s < NS; s++) {
-            mbar_init(full_w + 8 * s, 4);
+            mbar_init(full_w + 8 * s, 8);
             mbar_init(full_x + 8 * s, 1);
-            mbar_init(empty + 8 * s, 1 + 8);
+            mbar_init(empty + 8 * s, 1);
         }
         for (int b = 0; b < NB; b++) {
             mbar_init(acc_full + 8 * b, 1);
@@ -215,7 +242,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 12) {
+    if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "n"(C::COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
@@ -226,27 +253,33 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
 
     const int n0 = blockIdx.x * TC_M, cnt = ch.hi - ch.lo;
     const int stages = (a.units + 1) / 2, per = ((stages + a.splits - 1) / a.splits + 3) & ~3;  // whole superblocks
+    const int blocks = C::min_blocks(a.units);
     const bool real = !a.order || ch.group < a.n_exp;
-    const int k0 = blockIdx.z * per, k1 = real ? min(k0 + per, stages) : k0;
+    // this CTA's stages: k0 .. of the levels (`main` of them), then its share of the minima's blocks
+    const int k0 = min((int)blockIdx.z * per, stages), main = real ? min(per, stages - k0) : 0;
+    const int e0 = blocks * (int)blockIdx.z / a.splits, extra = real ? (blocks * ((int)blockIdx.z + 1) / a.splits - e0) * (LO ? 2 : 1) : 0;
+    const int total = main + extra;
+    // whether unit uu of stage i begins / ends an accumulator
+    auto begins = [&](int i, int uu) { return !GROUP || i >= main || (uu == 0 && i % (GROUP ? GROUP : 1) == 0); };
+    auto ends = [&](int i, int uu) { return !GROUP || i >= main || (uu == 1 && (i % (GROUP ? GROUP : 1) == GROUP - 1 || i + 1 == main)); };
 
-    if (warp >= 12) {
+    if (warp >= 8) {
         if constexpr (C::MOVE) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-        if (warp == 12) {
+        if (warp == 8) {
             if (lane == 0) {
                 // D float32, A and B float16 K-major, N = BN, M = 128
                 constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(TC_M >> 4) << 24);
-                int n_acc = 0;  // accumulators begun
+                int n_acc = 0;  // accumulators ended
                 bool ok = true;
-                for (int k = k0; k < k1 && ok; k++) {
-                    const int i = k - k0, s = i % NS, ph = (i / NS) & 1;
+                for (int i = 0; i < total && ok; i++) {
+                    const int s = i % NS, ph = (i / NS) & 1;
                     ok = mbar_wait(full_w + 8 * s, ph, a.fault) && mbar_wait(full_x + 8 * s, ph, a.fault);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint32_t st = ring + s * C::STAGE;
                     for (int uu = 0; uu < 2; uu++) {
-                        const bool first = GROUP ? uu == 0 && i % GROUP == 0 : true;
-                        const bool last = GROUP ? uu == 1 && (i % GROUP == GROUP - 1 || k + 1 == k1) : true;
                         const int b = n_acc % NB;
+                        const bool first = begins(i, uu);
                         if (first) {
                             if (!(ok = mbar_wait(acc_empty + 8 * b, ((n_acc / NB) & 1) ^ 1, a.fault))) break;
                             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -254,11 +287,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
 #pragma unroll
                         for (int kk = 0; kk < 2; kk++) {
                             const uint32_t at = uu * 64 + kk * 32;
-                            mma_f16(tmem + b * BN, operand_desc(st + at), operand_desc(st + C::OFF_B + at), idesc, !first || kk > 0);
-                            if constexpr (LO) mma_f16(tmem + b * BN, operand_desc(st + at), operand_desc(st + C::OFF_B + C::B_BYTES + at), idesc, true);
-                            if constexpr (C::SPLIT) mma_f16(tmem + b * BN, operand_desc(st + C::A_BYTES + at), operand_desc(st + C::OFF_B + at), idesc, true);
+                            mma_f16(tmem + b * BN, operand_desc(st + at), operand_desc(st + C::A_ALL + at), idesc, !first || kk > 0);
+                            if constexpr (LO) mma_f16(tmem + b * BN, operand_desc(st + at), operand_desc(st + C::A_ALL + C::B_BYTES + at), idesc, true);
+                            if constexpr (C::SPLIT) mma_f16(tmem + b * BN, operand_desc(st + C::A_BYTES + at), operand_desc(st + C::A_ALL + at), idesc, true);
                         }
-                        if (last) {
+                        if (ends(i, uu)) {
                             mma_commit(acc_full + 8 * b);
                             n_acc++;
                         }
@@ -270,112 +303,115 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
             asm volatile("bar.sync 1, 288;" ::: "memory");  // the sums' warps have read their last accumulator
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(C::COLS));
-        } else if (warp == 13 && lane == 0) {
-            const uint8_t* src = xp + (int64_t)blockIdx.y * stages * C::X_BYTES;
-            int k = k0;
-            for (; k < k1; k++) {
-                const int i = k - k0, s = i % NS;
+        } else if (warp == 9 && lane == 0) {
+            const uint8_t* src = xp + (int64_t)blockIdx.y * (stages + blocks) * C::X_BYTES;
+            int i = 0;
+            for (; i < total; i++) {
+                const int s = i % NS;
                 if (!mbar_wait(empty + 8 * s, ((i / NS) & 1) ^ 1, a.fault)) break;
-                bulk_load(ring + s * C::STAGE + C::OFF_B, src + (int64_t)k * C::X_BYTES, C::X_BYTES, full_x + 8 * s);
+                const int k = i < main ? k0 + i : stages + e0 + (i - main) / (LO ? 2 : 1);
+                bulk_load(ring + s * C::STAGE + C::A_ALL, src + (int64_t)k * C::X_BYTES, C::X_BYTES, full_x + 8 * s);
             }
             // no copy outlives the CTA
-            for (int j = max(k0, k - NS); j < k; j++) mbar_wait(full_x + 8 * ((j - k0) % NS), ((j - k0) / NS) & 1, a.fault);
-        }
-    } else if (warp >= 8) {
-        if constexpr (C::MOVE) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-        const int row = tid - 256;
-        const bool mine = n0 + row < a.n;
-        const uint8_t* w = a.w + (real ? ch.group * a.w_exp : 0) + (int64_t)(mine ? n0 + row : 0) * a.w_row;
-        uint32_t raw[2][L::WORDS];
-        auto load = [&](int k) {
-#pragma unroll
-            for (int uu = 0; uu < 2; uu++) {
-                const int u = 2 * k + uu;
-                if (mine && k < k1 && u < a.units) L::template load<L::MAXAL>(w + (int64_t)(u / UPB) * L::BB, u % UPB, raw[uu]);
-                else
-#pragma unroll
-                    for (int j = 0; j < L::WORDS; j++) raw[uu][j] = 0;  // zero scales
-            }
-        };
-        load(k0);
-        for (int k = k0; k < k1; k++) {
-            const int i = k - k0, s = i % NS;
-            uint8_t* st = ring_p + s * C::STAGE;
-            if (!mbar_wait(empty + 8 * s, ((i / NS) & 1) ^ 1, a.fault)) break;
-#pragma unroll
-            for (int uu = 0; uu < 2; uu++) {
-                const int j = (2 * k + uu) % UPB;
-                uint32_t q[8];
-                float dl[2], ml[2];
-                L::levels(raw[uu], j, a.kgrid, q, dl, ml);
-                const __half2 bias = __float2half2_rn(L::SIGNED ? 1152.0f : 1024.0f);
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    __half2 h[4];
-                    word_halves(L::SIGNED ? q[2 * c] ^ 0x80808080u : q[2 * c], bias, h);
-                    word_halves(L::SIGNED ? q[2 * c + 1] ^ 0x80808080u : q[2 * c + 1], bias, h + 2);
-                    uint8_t* o = st + row * 128 + (((4 * uu + c) ^ (row & 7)) << 4);
-                    if constexpr (L::FOLD) {
-                        const __half2 sc = __half2half2(__int2half_rn(L::sub(raw[uu], j, c >> 1)));
-                        __half2 p[4];
-#pragma unroll
-                        for (int e = 0; e < 4; e++) p[e] = __hmul2(h[e], sc);
-                        if constexpr (C::SPLIT) {  // the product's rounding error, exact in float16
-#pragma unroll
-                            for (int e = 0; e < 4; e++) h[e] = __hfma2(h[e], sc, __hneg2(p[e]));
-                            *reinterpret_cast<uint4*>(o + C::A_BYTES) = make_uint4(h2_bits(h[0]), h2_bits(h[1]), h2_bits(h[2]), h2_bits(h[3]));
-                        }
-#pragma unroll
-                        for (int e = 0; e < 4; e++) h[e] = p[e];
-                    }
-                    *reinterpret_cast<uint4*>(o) = make_uint4(h2_bits(h[0]), h2_bits(h[1]), h2_bits(h[2]), h2_bits(h[3]));
-                }
-                float* d = reinterpret_cast<float*>(st + C::OFF_D) + row;
-                if constexpr (L::FOLD) d[uu * TC_M] = L::base(raw[uu]);
-                else d[uu * TC_M] = dl[0];
-#pragma unroll
-                for (int p = 0; p < SUMS; p++) d[(2 + uu * SUMS + p) * TC_M] = -ml[p];
-            }
-            load(k + 1);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(full_w + 8 * s);
+            for (int j = max(0, i - NS); j < i; j++) mbar_wait(full_x + 8 * (j % NS), (j / NS) & 1, a.fault);
         }
     } else {
-        if constexpr (C::MOVE) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
-        const int row = (warp & 3) * 32 + lane, c0 = (warp >> 2) * HALF;
+        if constexpr (C::MOVE) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+        const int row = tid & 127, my = tid >> 7;  // weight row of the tile, unit of the stage
+        const bool mine = n0 + row < a.n;
+        const uint8_t* w = a.w + (real ? ch.group * a.w_exp : 0) + (int64_t)(mine ? n0 + row : 0) * a.w_row;
+        const int c0 = my * HALF;
         constexpr int NBT = HALF / 16;
         f32x2 acc[HALF / 2];
 #pragma unroll
         for (int i = 0; i < HALF / 2; i++) acc[i] = 0ull;
-        int n_acc = 0;  // accumulators read
-        bool ok = true;
-        for (int k = k0; k < k1 && ok; k++) {
-            const int i = k - k0, s = i % NS, ph = (i / NS) & 1;
-            ok = mbar_wait(full_w + 8 * s, ph, a.fault) && mbar_wait(full_x + 8 * s, ph, a.fault);
-            if (!ok) break;
-            const uint8_t* st = ring_p + s * C::STAGE;
-            const float* d = reinterpret_cast<const float*>(st + C::OFF_D) + row;
-            // minima: the planes' values of 4 columns to all lanes at once
+        uint32_t raw[PF][L::WORDS];
+        auto load = [&](int i, uint32_t* r) {
+            const int u = 2 * (k0 + i) + my;
+            if (mine && i < main && u < a.units) L::template load<L::MAXAL>(w + (int64_t)(u / UPB) * L::BB, u % UPB, r);
+            else
 #pragma unroll
-            for (int p = 0; p < 2 * SUMS; p++) {
-                const f32x2 ml = f2_splat(d[(2 + p) * TC_M]);
-                const float4* x = reinterpret_cast<const float4*>(st + C::OFF_P + (p * BN + c0) * 4);
+                for (int j = 0; j < L::WORDS; j++) r[j] = 0;  // zero scales
+        };
+        auto put = [&](uint8_t* st, int c, const __half2* h) {
+            *reinterpret_cast<uint4*>(st + row * 128 + (((4 * my + c) ^ (row & 7)) << 4)) = make_uint4(h2_bits(h[0]), h2_bits(h[1]), h2_bits(h[2]), h2_bits(h[3]));
+        };
+        auto unpack = [&](int i, const uint32_t* r) {
+            uint8_t* st = ring_p + i % NS * C::STAGE;
+            const int j = (2 * (k0 + i) + my) % UPB;
+            uint32_t q[8];
+            float dl[2], ml[2];
+            L::levels(r, j, a.kgrid, q, dl, ml);
+            const __half2 bias = __float2half2_rn(L::SIGNED ? 1152.0f : 1024.0f);
 #pragma unroll
-                for (int c = 0; c < HALF / 4; c++) {
-                    const float4 v = x[c];
-                    acc[2 * c] = f2_fma(ml, f2_pack(v.x, v.y), acc[2 * c]);
-                    acc[2 * c + 1] = f2_fma(ml, f2_pack(v.z, v.w), acc[2 * c + 1]);
+            for (int c = 0; c < 4; c++) {
+                __half2 h[4];
+                word_halves(L::SIGNED ? q[2 * c] ^ 0x80808080u : q[2 * c], bias, h);
+                word_halves(L::SIGNED ? q[2 * c + 1] ^ 0x80808080u : q[2 * c + 1], bias, h + 2);
+                if constexpr (L::FOLD) {
+                    const __half2 sc = __half2half2(__int2half_rn(L::sub(r, j, c >> 1)));
+                    __half2 p[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) p[e] = __hmul2(h[e], sc);
+                    if constexpr (C::SPLIT) {  // the product's rounding error, exact in float16
+#pragma unroll
+                        for (int e = 0; e < 4; e++) h[e] = __hfma2(h[e], sc, __hneg2(p[e]));
+                        put(st + C::A_BYTES, c, h);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; e++) h[e] = p[e];
                 }
+                put(st, c, h);
             }
+            scales[((i % C::DR) * 2 + my) * TC_M + row] = L::FOLD ? base_of<L>(r) : dl[0];
+        };
+        // 32 minima of the row (negated) times a power of two, its inverse (and the sums' 2^7) as the scale
+        auto unpack_minima = [&](int i) {
+            if constexpr (SUMS > 0) {
+                constexpr int PER = UPB * SUMS;  // minima of a block
+                uint8_t* st = ring_p + i % NS * C::STAGE;
+                const int e = (i - main) / (LO ? 2 : 1), part = LO ? (i - main) & 1 : 0, p0 = (e0 + e) * 64 + my * 32;
+                float m[32], top = 0.0f;
+#pragma unroll
+                for (int p = 0; p < 32; p += PER) {
+                    const bool in = mine && p0 + p < a.units * SUMS;
+#pragma unroll
+                    for (int j = 0; j < PER; j++) m[p + j] = 0.0f;
+                    if (in) L::template minima<L::MAXAL>(w + (int64_t)((p0 + p) / PER) * L::BB, m + p);
+                }
+#pragma unroll
+                for (int p = 0; p < 32; p++) top = fmaxf(top, fabsf(m[p]));
+                float up = 1.0f;  // the largest below 2^11
+                if (top > 0.0f && top < INFINITY) up = __uint_as_float((uint32_t)(127 + 10 + 127 - (int)(__float_as_uint(top) >> 23)) << 23);
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    __half2 h[4];
+#pragma unroll
+                    for (int x = 0; x < 4; x++) {
+                        const float v0 = -m[8 * c + 2 * x] * up, v1 = -m[8 * c + 2 * x + 1] * up;
+                        h[x] = __floats2half2_rn(v0, v1);
+                        if (LO && part) {
+                            const float2 f = __half22float2(h[x]);
+                            h[x] = __floats2half2_rn(v0 - f.x, v1 - f.y);
+                        }
+                    }
+                    put(st, c, h);
+                    if constexpr (C::SPLIT) put(st + C::A_BYTES, c, h);
+                }
+                scales[((i % C::DR) * 2 + my) * TC_M + row] = 128.0f / up;
+            }
+        };
+        int n_acc = 0;  // accumulators read
+        auto collect = [&](int i) {
 #pragma unroll
             for (int uu = 0; uu < 2; uu++) {
-                if (GROUP && (uu == 0 || (i % (GROUP ? GROUP : 1) != GROUP - 1 && k + 1 < k1))) continue;
+                if (!ends(i, uu)) continue;
                 const int b = n_acc % NB;
-                const f32x2 dl = f2_splat(d[uu * TC_M]);
-                if (!(ok = mbar_wait(acc_full + 8 * b, (n_acc / NB) & 1, a.fault))) break;
+                if (!mbar_wait(acc_full + 8 * b, (n_acc / NB) & 1, a.fault)) return false;
                 n_acc++;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                // a shared scale is this thread's own; else the stage was full before its product ended
+                const f32x2 dl = f2_splat(*(volatile float*)&scales[((i % C::DR) * 2 + (GROUP && i < main ? my : uu)) * TC_M + row]);
                 const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + b * BN + c0;
                 uint32_t v[2][16];
                 tmem_ld16(at, v[0]);
@@ -395,8 +431,28 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
                     }
                 }
             }
-            __syncwarp();
-            if (ok && lane == 0) mbar_arrive(empty + 8 * s);
+            return true;
+        };
+#pragma unroll
+        for (int p = 0; p < PF; p++) load(p, raw[p]);
+        bool ok = true;
+        for (int i0 = 0; i0 < total + LAG && ok; i0 += PF) {
+#pragma unroll
+            for (int p = 0; p < PF; p++) {
+                const int i = i0 + p;
+                if (i < total && ok) {
+                    ok = mbar_wait(empty + 8 * (i % NS), ((i / NS) & 1) ^ 1, a.fault);
+                    if (ok) {
+                        if (i < main) unpack(i, raw[p]);
+                        else unpack_minima(i);
+                        load(i + PF, raw[p]);
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(full_w + 8 * (i % NS));
+                    }
+                }
+                if (ok && i >= LAG && i - LAG < total) ok = collect(i - LAG);
+            }
         }
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         asm volatile("bar.sync 1, 288;" ::: "memory");
@@ -438,7 +494,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
     }
     __syncwarp();
     if (a.splits > 1) {
-        if (warp >= 8) cg::this_cluster().sync();
+        if (warp >= 8) cg::this_cluster().sync();  // the sums' warps have met the others' already
         cg::this_cluster().sync();  // the others may still read this tile
     }
 }
@@ -460,7 +516,7 @@ cudaError_t launch_tc_t(const MmArgs& a, void* ws, const LaunchCtx& ctx) {
             cudaFuncAttributes f;
             return cudaFuncGetAttributes(&f, tc_kernel<T, BN, LO>) == cudaSuccess ? f.numRegs : 0;
         }();
-        if (regs * TC_THREADS < 128 * (192 + 192 + 88 + 40)) return cudaErrorInvalidConfiguration;
+        if (regs * TC_THREADS < 128 * (232 + 232 + 40)) return cudaErrorInvalidConfiguration;
     }
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
