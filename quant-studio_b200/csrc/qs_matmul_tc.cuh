@@ -19,13 +19,14 @@
 // for 2048 slots of Q4_K 14336 x 4096: three float32 operations per value and unit are 768 cycles
 // (a packed f32x2 operation takes two), an SM has no more than 128 lanes.
 //
-// Roles in a CTA (one per SM, 12 warps, two of them idle):
-//   warps 0-7  unpack the weights (thread = row and unit of the stage, block bytes loaded PF stages
-//              ahead) and own the tile's sums (lane = weight row, each warp half of the columns),
-//              which they collect LAG stages behind
+// Roles in a CTA (one per SM, 12 warps):
+//   warps 0-7  unpack the weights (thread = row and unit of the stage) and own the tile's sums (lane =
+//              weight row, each warp half of the columns), which they collect LAG stages behind
 //   warp 8     issues the matrix products (and owns the tensor memory)
 //   warp 9     copies the activations' stage (one bulk copy: float16 rows as the matrix unit reads
 //              them), laid out beforehand by xpack_kernel
+//   warps 10, 11  copy the weights' bytes (cp.async) in steps of RS stages: the 16-byte pieces that
+//              cover a row's share wherever it starts, adjacent lanes adjacent pieces
 // Stages are a ring in shared memory (full: unpacked + copied, empty: products done); the
 // accumulators are a ring in tensor memory; the weights' scales are a longer ring of their own, which
 // no warp can lap: unpacking stage i waits for the products of stage i - NS, these for every warp's
@@ -56,19 +57,22 @@ struct TcCfg {
     static constexpr int GROUP = L::FOLD ? 4 : 0;  // stages that share an accumulator; 0: one per unit
     static constexpr int A_BYTES = TC_M * 128, A_ALL = A_BYTES * (SPLIT ? 2 : 1), B_BYTES = BN * 128, X_BYTES = B_BYTES * (LO ? 2 : 1);
     static constexpr int STAGE = A_ALL + X_BYTES;
-    static constexpr int LAG = GROUP ? 2 : 1;
-    // stages loaded ahead: as many as the registers next to the sums hold
-    static constexpr int PF = BN == 256 ? (L::WORDS <= 12 ? 2 : 1) : L::WORDS <= 6 ? 4 : L::WORDS <= 12 ? 3 : 2;
-    static constexpr int DR = 16;                      // ring of scales, [slot][unit][128]
+    // packed bytes: steps of RS stages (a superblock, or 4 blocks of 32), the bytes of a row's step and
+    // the pitch of the pieces that cover them, an odd number of pieces against bank conflicts
+    static constexpr int RS = L::QK == 256 ? 4 : 2, WB = RS * 64 / L::QK * L::BB;
+    static constexpr int COVER = L::MAXAL >= 16 ? WB : (WB + 16 - L::MAXAL + 15) / 16 * 16, WP = COVER / 16 % 2 ? COVER : COVER + 16;
+    static constexpr int RAW = TC_M * WP, RR = 2 * RAW <= 24 * 1024 ? 4 : 2;  // steps in the ring
+    static constexpr int DR = 8;                       // ring of scales, [slot][unit][128]
     static constexpr int D_BYTES = DR * 2 * TC_M * 4;
-    static constexpr int FIT = (TC_SMEM - 2048 - D_BYTES) / STAGE, NS = FIT > 8 ? 8 : FIT;
+    static constexpr int FIT = (TC_SMEM - 1024 - 512 - BN * 8 - D_BYTES - RR * RAW) / STAGE, NS = FIT > 4 ? 4 : FIT;
+    static constexpr int LAG = !GROUP ? 1 : NS > 3 ? 3 : NS - 1;
     static constexpr int NB = BN == 256 ? 2 : 4;       // accumulators in tensor memory
     static constexpr int COLS = NB * BN;
     // 256 columns are 128 registers a thread for the sums alone: the third warpgroup's registers move to
     // the other two (232, 232, 40 a thread of the 168 at launch)
     static constexpr bool MOVE = BN == 256;
     static constexpr int OUT_PITCH = TC_M + 4;
-    static constexpr int BYTES = NS * STAGE + D_BYTES + 1024;  // 1024 to align the ring
+    static constexpr int BYTES = NS * STAGE + D_BYTES + RR * RAW + 1024;  // 1024 to align the ring
     static_assert(NS >= LAG + 1 && DR >= NS + 1 + LAG, "ring lengths");
     static_assert(BN * OUT_PITCH * 4 <= NS * STAGE, "the tile leaves through the same memory");
     // further stages with the minima of `units` units: 64 terms each, with LO once for the hi and
@@ -102,6 +106,9 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
         "{ .reg .b64 st; mbarrier.arrive.expect_tx.shared::cta.b64 st, [%3], %2; }\n"
         "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
         ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 template <class L>
 __device__ __forceinline__ float base_of(const uint32_t* r) {
@@ -218,18 +225,22 @@ template <int T, int BN, bool LO>
 __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8_t* xp, const float* xs) {
     using L = Lv<T>;
     using C = TcCfg<T, BN, LO>;
-    constexpr int UPB = L::QK / 32, SUMS = C::SUMS, NS = C::NS, NB = C::NB, GROUP = C::GROUP, LAG = C::LAG, PF = C::PF;
+    constexpr int UPB = L::QK / 32, SUMS = C::SUMS, NS = C::NS, NB = C::NB, GROUP = C::GROUP, LAG = C::LAG, RS = C::RS, RR = C::RR;
     constexpr int HALF = BN / 2;  // columns of a warp
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bars[3 * NS + 2 * NB];
+    __shared__ __align__(8) uint64_t bars[3 * NS + 2 * NB + 2 * RR];
     __shared__ uint32_t s_tmem;
+    __shared__ int s_slot[BN];   // the tile's slots and their rows' powers of two
+    __shared__ float s_up[BN];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const Chunk ch = find_chunk<BN>(a, blockIdx.y);
     if (ch.group < 0) return;  // the CTAs of a cluster share the chunk
     const uint32_t ring = (smem_u32(smem_raw) + 1023) & ~1023u;
     uint8_t* const ring_p = smem_raw + (ring - smem_u32(smem_raw));
     float* const scales = reinterpret_cast<float*>(ring_p + NS * C::STAGE);
-    const uint32_t full_w = smem_u32(bars), full_x = full_w + 8 * NS, empty = full_x + 8 * NS, acc_full = empty + 8 * NS, acc_empty = acc_full + 8 * NB;
+    const uint8_t* const bytes_p = ring_p + NS * C::STAGE + C::D_BYTES;
+    const uint32_t full_w = smem_u32(bars), full_x = full_w + 8 * NS, empty = full_x + 8 * NS, acc_full = empty + 8 * NS, acc_empty = acc_full + 8 * NB,
+                   raw_full = acc_empty + 8 * NB, raw_empty = raw_full + 8 * RR;
     if (tid == 0) {
         for (int s = 0; s < NS; s++) {
             mbar_init(full_w + 8 * s, 8);
@@ -240,7 +251,18 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
             mbar_init(acc_full + 8 * b, 1);
             mbar_init(acc_empty + 8 * b, 8);
         }
+        for (int r = 0; r < RR; r++) {
+            mbar_init(raw_full + 8 * r, 64);
+            mbar_init(raw_empty + 8 * r, 8);
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    {
+        const bool some = !a.order || ch.group < a.n_exp;
+        for (int t = tid; t < BN; t += TC_THREADS) {
+            s_slot[t] = ch.lo + t < ch.hi ? (a.order ? __ldg(a.order + ch.lo + t) : ch.lo + t) : 0;
+            s_up[t] = some ? __ldg(xs + (int64_t)blockIdx.y * BN + t) : 1.0f;
+        }
     }
     if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "n"(C::COLS) : "memory");
@@ -271,8 +293,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
                 constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(TC_M >> 4) << 24);
                 int n_acc = 0;  // accumulators ended
                 bool ok = true;
+                int s = 0, ph = 0;
                 for (int i = 0; i < total && ok; i++) {
-                    const int s = i % NS, ph = (i / NS) & 1;
                     ok = mbar_wait(full_w + 8 * s, ph, a.fault) && mbar_wait(full_x + 8 * s, ph, a.fault);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -297,12 +319,37 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
                         }
                     }
                     if (ok) mma_commit(empty + 8 * s);
+                    if (++s == NS) {
+                        s = 0;
+                        ph ^= 1;
+                    }
                 }
             }
             __syncwarp();
             asm volatile("bar.sync 1, 288;" ::: "memory");  // the sums' warps have read their last accumulator
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(C::COLS));
+        } else if (warp >= 10) {
+            // one warp half of the rows each; adjacent lanes take adjacent pieces of a row
+            constexpr int P = C::COVER / 16, HALF_ROWS = TC_M / 2;
+            const int first = (warp - 10) * HALF_ROWS, rows = min(HALF_ROWS, a.n - n0 - first), steps = (main + RS - 1) / RS;
+            const uint8_t* w = a.w + (real ? ch.group * a.w_exp : 0) + (int64_t)(n0 + first) * a.w_row;
+            const int64_t len = (int64_t)a.units / UPB * L::BB;
+            for (int k = 0; k < steps; k++) {
+                const int r = k % RR;
+                if (!mbar_wait(raw_empty + 8 * r, ((k / RR) & 1) ^ 1, a.fault)) break;
+                const int64_t lo = (int64_t)(k0 / RS + k) * C::WB, hi = min(lo + C::WB, len);
+                const uint32_t dst = smem_u32(bytes_p) + r * C::RAW + first * C::WP;
+#pragma unroll 4
+                for (int i = lane; i < HALF_ROWS * P; i += 32) {
+                    const int t = i / P, piece = i - t * P;
+                    const uint8_t* row = w + t * a.w_row;
+                    const uint8_t* q = (const uint8_t*)((uintptr_t)(row + lo) & ~(uintptr_t)15) + piece * 16;
+                    if (t < rows && q < row + hi) cp16(dst + t * C::WP + piece * 16, q);
+                }
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(raw_full + 8 * r) : "memory");
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
         } else if (warp == 9 && lane == 0) {
             const uint8_t* src = xp + (int64_t)blockIdx.y * (stages + blocks) * C::X_BYTES;
             int i = 0;
@@ -325,20 +372,20 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
         f32x2 acc[HALF / 2];
 #pragma unroll
         for (int i = 0; i < HALF / 2; i++) acc[i] = 0ull;
-        uint32_t raw[PF][L::WORDS];
-        auto load = [&](int i, uint32_t* r) {
-            const int u = 2 * (k0 + i) + my;
-            if (mine && i < main && u < a.units) L::template load<L::MAXAL>(w + (int64_t)(u / UPB) * L::BB, u % UPB, r);
-            else
-#pragma unroll
-                for (int j = 0; j < L::WORDS; j++) r[j] = 0;  // zero scales
-        };
         auto put = [&](uint8_t* st, int c, const __half2* h) {
             *reinterpret_cast<uint4*>(st + row * 128 + (((4 * my + c) ^ (row & 7)) << 4)) = make_uint4(h2_bits(h[0]), h2_bits(h[1]), h2_bits(h[2]), h2_bits(h[3]));
         };
-        auto unpack = [&](int i, const uint32_t* r) {
-            uint8_t* st = ring_p + i % NS * C::STAGE;
-            const int j = (2 * (k0 + i) + my) % UPB;
+        // k0 is a whole number of steps, so stage i is stage i % RS of step i / RS
+        auto unpack = [&](int i, uint8_t* st) {
+            const int u = 2 * (k0 + i) + my, in = 2 * (i % RS) + my, j = in % UPB;
+            uint32_t r[L::WORDS];
+            if (mine && u < a.units) {
+                const uint32_t off = L::MAXAL >= 16 ? 0 : (uint32_t)(uintptr_t)(w + (int64_t)(k0 / RS + i / RS) * C::WB) & 15;
+                L::template load<L::MAXAL, true>(bytes_p + (i / RS) % RR * C::RAW + row * C::WP + off + in / UPB * L::BB, j, r);
+            } else {
+#pragma unroll
+                for (int e = 0; e < L::WORDS; e++) r[e] = 0;  // zero scales
+            }
             uint32_t q[8];
             float dl[2], ml[2];
             L::levels(r, j, a.kgrid, q, dl, ml);
@@ -366,10 +413,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
             scales[((i % C::DR) * 2 + my) * TC_M + row] = L::FOLD ? base_of<L>(r) : dl[0];
         };
         // 32 minima of the row (negated) times a power of two, its inverse (and the sums' 2^7) as the scale
-        auto unpack_minima = [&](int i) {
+        auto unpack_minima = [&](int i, uint8_t* st) {
             if constexpr (SUMS > 0) {
                 constexpr int PER = UPB * SUMS;  // minima of a block
-                uint8_t* st = ring_p + i % NS * C::STAGE;
                 const int e = (i - main) / (LO ? 2 : 1), part = LO ? (i - main) & 1 : 0, p0 = (e0 + e) * 64 + my * 32;
                 float m[32], top = 0.0f;
 #pragma unroll
@@ -433,26 +479,33 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
             }
             return true;
         };
-#pragma unroll
-        for (int p = 0; p < PF; p++) load(p, raw[p]);
         bool ok = true;
-        for (int i0 = 0; i0 < total + LAG && ok; i0 += PF) {
-#pragma unroll
-            for (int p = 0; p < PF; p++) {
-                const int i = i0 + p;
-                if (i < total && ok) {
-                    ok = mbar_wait(empty + 8 * (i % NS), ((i / NS) & 1) ^ 1, a.fault);
-                    if (ok) {
-                        if (i < main) unpack(i, raw[p]);
-                        else unpack_minima(i);
-                        load(i + PF, raw[p]);
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        int s = 0, ph = 1;  // stage of the ring and the parity that its last use ended with
+        for (int i = 0; i < total + LAG && ok; i++) {
+            if (i < total) {
+                ok = mbar_wait(empty + 8 * s, ph, a.fault);
+                if (!ok) break;
+                uint8_t* st = ring_p + s * C::STAGE;
+                if (i < main) {
+                    const int r = i / RS;
+                    if (i % RS == 0 && !(ok = mbar_wait(raw_full + 8 * (r % RR), (r / RR) & 1, a.fault))) break;
+                    unpack(i, st);
+                    if (i % RS == RS - 1 || i + 1 == main) {
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(full_w + 8 * (i % NS));
+                        if (lane == 0) mbar_arrive(raw_empty + 8 * (r % RR));
                     }
+                } else {
+                    unpack_minima(i, st);
                 }
-                if (ok && i >= LAG && i - LAG < total) ok = collect(i - LAG);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full_w + 8 * s);
+                if (++s == NS) {
+                    s = 0;
+                    ph ^= 1;
+                }
             }
+            if (i >= LAG) ok = collect(i - LAG);
         }
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         asm volatile("bar.sync 1, 288;" ::: "memory");
@@ -474,22 +527,24 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
         const int type = a.part ? (int)SRC_F32 : a.out_type;
         const int64_t stride = a.part ? a.n : a.out_stride;
         const bool vec = n0 + TC_M <= a.n && stride % 4 == 0 && ((uintptr_t)out & 15) == 0;
-        for (int t = warp * ranks + rank; t < cnt; t += 8 * ranks) {
-            const int64_t slot = a.order ? __ldg(a.order + ch.lo + t) : ch.lo + t;
-            const int64_t at = slot * stride + n0;
-            float4 v;
-            if (ranks > 1) {
-                v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (ranks == 1) {
+#pragma unroll 4
+            for (int t = warp; t < cnt; t += 8) {
+                const float4 v = *reinterpret_cast<const float4*>(o + t * C::OUT_PITCH + 4 * lane);
+                const float u = s_up[t];
+                store_row4(out, (int64_t)s_slot[t] * stride + n0, type, make_float4(v.x * u, v.y * u, v.z * u, v.w * u), lane, n0, a.n, vec);
+            }
+        } else {
+            for (int t = warp * ranks + rank; t < cnt; t += 8 * ranks) {
+                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
                 for (int r = 0; r < ranks; r++) {
                     const float4 f = *reinterpret_cast<const float4*>(cg::this_cluster().map_shared_rank(o, r) + t * C::OUT_PITCH + 4 * lane);
                     v.x += f.x; v.y += f.y; v.z += f.z; v.w += f.w;
                 }
-            } else {
-                v = *reinterpret_cast<const float4*>(o + t * C::OUT_PITCH + 4 * lane);
+                const float u = s_up[t];
+                store_row4(out, (int64_t)s_slot[t] * stride + n0, type, make_float4(v.x * u, v.y * u, v.z * u, v.w * u), lane, n0, a.n, vec);
             }
-            const float sx = real ? __ldg(xs + (int64_t)blockIdx.y * BN + t) : 1.0f;
-            v = make_float4(v.x * sx, v.y * sx, v.z * sx, v.w * sx);
-            store_row4(out, at, type, v, lane, n0, a.n, vec);
         }
     }
     __syncwarp();
