@@ -115,14 +115,19 @@ __device__ __forceinline__ float base_of(const uint32_t* r) {
     if constexpr (L::FOLD) return L::base(r);
     else return 0.0f;
 }
-// Shared-memory operand, K-major, rows of 128 bytes in the 128-byte swizzle: 8-row groups 1024
-// bytes apart
-__device__ __forceinline__ uint64_t operand_desc(uint32_t addr) {
-    return (uint64_t)((addr & 0x3FFFF) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+// Shared-memory operands K-major, rows of 128 bytes in the 128-byte swizzle: 8-row groups 1024
+// bytes apart. a, b: addresses in 16-byte units
+__device__ __forceinline__ void mma_f16(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
+    constexpr uint32_t HI = (1024 >> 4) | (1u << 14) | (2u << 29);
+    asm volatile(
+        "{ .reg .pred p; .reg .b64 x, y; mov.b64 x, {%1, %5}; mov.b64 y, {%2, %5}; setp.ne.u32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p; }"
+        ::"r"(d), "r"(a | 0x10000u), "r"(b | 0x10000u), "r"(idesc), "r"((uint32_t)add), "r"(HI) : "memory");
 }
-__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{ .reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(p));
+    return p != 0;
 }
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
@@ -228,7 +233,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
     constexpr int UPB = L::QK / 32, SUMS = C::SUMS, NS = C::NS, NB = C::NB, GROUP = C::GROUP, LAG = C::LAG, RS = C::RS, RR = C::RR;
     constexpr int HALF = BN / 2;  // columns of a warp
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bars[3 * NS + 2 * NB + 2 * RR];
+    __shared__ __align__(8) uint64_t bars[2 * NS + 2 * NB + 2 * RR];
     __shared__ uint32_t s_tmem;
     __shared__ int s_slot[BN];   // the tile's slots and their rows' powers of two
     __shared__ float s_up[BN];
@@ -239,12 +244,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
     uint8_t* const ring_p = smem_raw + (ring - smem_u32(smem_raw));
     float* const scales = reinterpret_cast<float*>(ring_p + NS * C::STAGE);
     const uint8_t* const bytes_p = ring_p + NS * C::STAGE + C::D_BYTES;
-    const uint32_t full_w = smem_u32(bars), full_x = full_w + 8 * NS, empty = full_x + 8 * NS, acc_full = empty + 8 * NS, acc_empty = acc_full + 8 * NB,
+    const uint32_t full = smem_u32(bars), empty = full + 8 * NS, acc_full = empty + 8 * NS, acc_empty = acc_full + 8 * NB,
                    raw_full = acc_empty + 8 * NB, raw_empty = raw_full + 8 * RR;
     if (tid == 0) {
         for (int s = 0; s < NS; s++) {
-            mbar_init(full_w + 8 * s, 8);
-            mbar_init(full_x + 8 * s, 1);
+            mbar_init(full + 8 * s, 8 + 1);
             mbar_init(empty + 8 * s, 1);
         }
         for (int b = 0; b < NB; b++) {
@@ -288,41 +292,44 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
     if (warp >= 8) {
         if constexpr (C::MOVE) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (warp == 8) {
-            if (lane == 0) {
-                // D float32, A and B float16 K-major, N = BN, M = 128
-                constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(TC_M >> 4) << 24);
-                int n_acc = 0;  // accumulators ended
+            // the whole warp runs the loop, so that addresses stay in uniform registers; one lane issues
+            const bool leader = elect_one();
+            // D float32, A and B float16 K-major, N = BN, M = 128
+            constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(TC_M >> 4) << 24);
+            int b = 0, b_ph = 1;  // accumulator, parity of its last release
+            int s = 0, ph = 0;
+            for (int i = 0; i < total; i++) {
+                if (!mbar_wait(full + 8 * s, ph, a.fault)) break;
+                const uint32_t st = (ring + s * C::STAGE) >> 4;
                 bool ok = true;
-                int s = 0, ph = 0;
-                for (int i = 0; i < total && ok; i++) {
-                    ok = mbar_wait(full_w + 8 * s, ph, a.fault) && mbar_wait(full_x + 8 * s, ph, a.fault);
-                    if (!ok) break;
+#pragma unroll
+                for (int uu = 0; uu < 2; uu++) {
+                    const bool first = begins(i, uu);
+                    if (first && !(ok = mbar_wait(acc_empty + 8 * b, b_ph, a.fault))) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t st = ring + s * C::STAGE;
-                    for (int uu = 0; uu < 2; uu++) {
-                        const int b = n_acc % NB;
-                        const bool first = begins(i, uu);
-                        if (first) {
-                            if (!(ok = mbar_wait(acc_empty + 8 * b, ((n_acc / NB) & 1) ^ 1, a.fault))) break;
-                            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        }
+                    if (leader) {
 #pragma unroll
                         for (int kk = 0; kk < 2; kk++) {
-                            const uint32_t at = uu * 64 + kk * 32;
-                            mma_f16(tmem + b * BN, operand_desc(st + at), operand_desc(st + C::A_ALL + at), idesc, !first || kk > 0);
-                            if constexpr (LO) mma_f16(tmem + b * BN, operand_desc(st + at), operand_desc(st + C::A_ALL + C::B_BYTES + at), idesc, true);
-                            if constexpr (C::SPLIT) mma_f16(tmem + b * BN, operand_desc(st + C::A_BYTES + at), operand_desc(st + C::A_ALL + at), idesc, true);
-                        }
-                        if (ends(i, uu)) {
-                            mma_commit(acc_full + 8 * b);
-                            n_acc++;
+                            constexpr uint32_t X = C::A_ALL >> 4;
+                            const uint32_t at = st + uu * 4 + kk * 2;
+                            mma_f16(tmem + b * BN, at, at + X, idesc, !first || kk > 0);
+                            if constexpr (LO) mma_f16(tmem + b * BN, at, at + X + (C::B_BYTES >> 4), idesc, true);
+                            if constexpr (C::SPLIT) mma_f16(tmem + b * BN, at + (C::A_BYTES >> 4), at + X, idesc, true);
                         }
                     }
-                    if (ok) mma_commit(empty + 8 * s);
-                    if (++s == NS) {
-                        s = 0;
-                        ph ^= 1;
+                    if (ends(i, uu)) {
+                        if (leader) mma_commit(acc_full + 8 * b);
+                        if (++b == NB) {
+                            b = 0;
+                            b_ph ^= 1;
+                        }
                     }
+                }
+                if (!ok) break;
+                if (leader) mma_commit(empty + 8 * s);
+                if (++s == NS) {
+                    s = 0;
+                    ph ^= 1;
                 }
             }
             __syncwarp();
@@ -357,10 +364,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
                 const int s = i % NS;
                 if (!mbar_wait(empty + 8 * s, ((i / NS) & 1) ^ 1, a.fault)) break;
                 const int k = i < main ? k0 + i : stages + e0 + (i - main) / (LO ? 2 : 1);
-                bulk_load(ring + s * C::STAGE + C::A_ALL, src + (int64_t)k * C::X_BYTES, C::X_BYTES, full_x + 8 * s);
+                bulk_load(ring + s * C::STAGE + C::A_ALL, src + (int64_t)k * C::X_BYTES, C::X_BYTES, full + 8 * s);
             }
             // no copy outlives the CTA
-            for (int j = max(0, i - NS); j < i; j++) mbar_wait(full_x + 8 * (j % NS), (j / NS) & 1, a.fault);
+            for (int j = max(0, i - NS); j < i; j++) mbar_wait(full + 8 * (j % NS), (j / NS) & 1, a.fault);
         }
     } else {
         if constexpr (C::MOVE) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
@@ -447,14 +454,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
                 scales[((i % C::DR) * 2 + my) * TC_M + row] = 128.0f / up;
             }
         };
-        int n_acc = 0;  // accumulators read
+        int b = 0, b_ph = 0;  // accumulator to read, its parity
         auto collect = [&](int i) {
 #pragma unroll
             for (int uu = 0; uu < 2; uu++) {
                 if (!ends(i, uu)) continue;
-                const int b = n_acc % NB;
-                if (!mbar_wait(acc_full + 8 * b, (n_acc / NB) & 1, a.fault)) return false;
-                n_acc++;
+                if (!mbar_wait(acc_full + 8 * b, b_ph, a.fault)) return false;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 // a shared scale is this thread's own; else the stage was full before its product ended
                 const f32x2 dl = f2_splat(*(volatile float*)&scales[((i % C::DR) * 2 + (GROUP && i < main ? my : uu)) * TC_M + row]);
@@ -475,6 +480,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
                         __syncwarp();
                         if (lane == 0) mbar_arrive(acc_empty + 8 * b);
                     }
+                }
+                if (++b == NB) {
+                    b = 0;
+                    b_ph ^= 1;
                 }
             }
             return true;
@@ -499,7 +508,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(full_w + 8 * s);
+                if (lane == 0) mbar_arrive(full + 8 * s);
                 if (++s == NS) {
                     s = 0;
                     ph ^= 1;
