@@ -253,8 +253,8 @@ int qs_matmul_experts(int ggml_type, const void* w, int64_t w_row_bytes, int64_t
                       const int32_t* order, const int32_t* offsets, int64_t n_tokens, int top_k, const float* weights,
                       void* out, int out_type, int64_t out_row_stride, void* workspace, int64_t workspace_bytes,
                       void* stream);
-int qs_matmul_experts_workspace(int ggml_type, int n_experts, int64_t n, int64_t k, int64_t n_tokens, int top_k, int sum,
-                                int out_type, int64_t* bytes);
+int qs_matmul_experts_workspace(int ggml_type, int n_experts, int64_t n, int64_t k, int64_t n_tokens, int top_k,
+                                int x_per_slot, int sum, int out_type, int64_t* bytes);
 
 /*
  * Fault word of `device`: bit 0 is set when a quantize kernel gave up waiting for one of its

@@ -447,39 +447,40 @@ bool has_min(int type) {
 
 // How a product runs: which kernel, its tile, over how many CTAs a tile's rows are split.
 struct MmPlan {
-    bool few, lo;
+    enum { FEW, MID, TC } kind;
+    bool lo;
     int bn, splits;
     int64_t part_off, bytes;  // workspace: laid-out activations, then the slots' results before a sum
 };
 
-// slots: output rows before a weighted sum; groups: weight matrices that share them. The tile
-// kernel keeps one CTA on each of a B200's 148 SMs.
-MmPlan mm_plan(int type, int64_t n, int64_t k, int64_t slots, int64_t groups, bool experts, bool sum, bool lo) {
+// slots: output rows before a weighted sum; groups: weight matrices that share them; x_rows:
+// activation rows. The number of CTAs is set against a B200's 148 SMs.
+MmPlan mm_plan(int type, int64_t n, int64_t k, int64_t slots, int64_t groups, int64_t x_rows, bool experts, bool sum, bool lo) {
     MmPlan p;
     const int64_t avg = (slots + groups - 1) / groups, units = k / 32, stages = (units + 1) / 2;
-    // rows that the small kernel can not hold go to the tiles whatever their number
-    p.few = (groups == 1 ? slots <= qs::FEW_SLOTS : avg <= 4) && units * qs::FEW_SLOTS * qs::FEW_UNIT_MAX <= qs::FEW_SMEM_MAX;
+    // rows that the kernel for few slots can not hold go to the next one
+    const bool holds = units * qs::FEW_SLOTS * qs::FEW_UNIT_MAX <= qs::FEW_SMEM_MAX;
+    p.kind = (experts ? avg <= 1 : slots <= 4) && holds ? MmPlan::FEW : avg <= 64 ? MmPlan::MID : MmPlan::TC;
     p.lo = lo;
-    p.bn = avg <= 32 ? 32 : avg <= 64 ? 64 : avg <= 128 || lo ? 128 : 256;
+    p.bn = avg <= 8 ? 8 : avg <= 16 ? 16 : avg <= 32 ? 32 : avg <= 64 ? 64 : avg <= 128 || lo ? 128 : 256;
     p.splits = 1;
     const int64_t chunks = groups == 1 ? (slots + p.bn - 1) / p.bn : slots / p.bn + (groups < slots ? groups : slots) / 2 + 1;
-    const int64_t tiles = (n + 127) / 128 * chunks;
-    if (tiles > 0 && tiles < 148) {
-        int64_t s = 148 / tiles;
+    const int64_t tiles = (n + 127) / 128 * chunks, ctas = p.kind == MmPlan::MID ? 2 * 148 : 148;
+    if (tiles > 0 && tiles < ctas) {
+        int64_t s = ctas / tiles;
         if (s > 8) s = 8;                    // a cluster
-        if (s > stages / 8) s = stages / 8;  // 8 stages each at least
+        if (s > stages / 8) s = stages / 8;  // 512 values each at least
         if (s > 1) {
-            const int64_t per = ((stages + s - 1) / s + 3) / 4 * 4;
+            const int64_t per = ((stages + s - 1) / s + 3) / 4 * 4;  // whole superblocks
             p.splits = (int)((stages + per - 1) / per);
         }
     }
+    const int sums = !has_min(type) ? 0 : type == qs::QS_Q2_K ? 2 : 1;
     int64_t xp = 0;
-    if (!p.few) {
-        const int sums = !has_min(type) ? 0 : type == qs::QS_Q2_K ? 2 : 1;
-        xp = (qs::mm_tc_workspace(units, qs::max_chunks(experts, slots, groups, p.bn), p.bn, lo, sums) + 255) / 256 * 256;
-    }
-    p.part_off = xp;
-    p.bytes = xp + (sum ? slots * n * 4 : 0);
+    if (p.kind == MmPlan::MID) xp = qs::mm_mid_workspace(units, x_rows, sums);
+    if (p.kind == MmPlan::TC) xp = qs::mm_tc_workspace(units, qs::max_chunks(experts, slots, groups, p.bn), p.bn, lo, sums);
+    p.part_off = (xp + 255) / 256 * 256;
+    p.bytes = p.part_off + (sum ? slots * n * 4 : 0);
     return p;
 }
 
@@ -512,12 +513,14 @@ int check_mm_operands(const TypeInfo* ti, const void* w, int64_t w_row_bytes, in
     return QS_OK;
 }
 
-int run_mm(int ggml_type, const MmPlan& p, qs::MmArgs& a, int64_t k, int top_k, const float* weights, const int* ids, void* workspace,
-           const qs::LaunchCtx& ctx) {
+int run_mm(int ggml_type, const MmPlan& p, qs::MmArgs& a, int64_t k, int64_t x_rows, int top_k, const float* weights, const int* ids,
+           void* workspace, const qs::LaunchCtx& ctx) {
     a.units = (int)(k / 32);
     a.splits = p.splits;
     a.part = weights ? reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + p.part_off) : nullptr;
-    cudaError_t e = p.few ? qs::launch_mm_few(ggml_type, a, ctx) : qs::launch_mm_tc(ggml_type, a, p.bn, p.lo, workspace, ctx);
+    cudaError_t e = p.kind == MmPlan::FEW   ? qs::launch_mm_few(ggml_type, a, ctx)
+                    : p.kind == MmPlan::MID ? qs::launch_mm_mid(ggml_type, a, p.bn, (int)x_rows, workspace, ctx)
+                                            : qs::launch_mm_tc(ggml_type, a, p.bn, p.lo, workspace, ctx);
     if (e == cudaSuccess && weights) e = qs::launch_mm_sum(a, top_k, weights, ids, ctx);
     return e == cudaSuccess ? QS_OK : cuda_fail(e, "matmul launch");
 }
@@ -636,7 +639,7 @@ QS_API int qs_matmul_workspace(int ggml_type, int64_t n, int64_t k, int64_t n_ro
     const TypeInfo* ti;
     if (!is_src(out_type)) return fail(QS_EINVAL, "output type %d is not F32/F16/BF16", out_type);
     if (int rc = check_mm(ggml_type, n, k, n_rows, 1, &ti)) return rc;
-    if (bytes) *bytes = mm_plan(ggml_type, n, k, n_rows, 1, false, false, out_type != QS_SRC_BF16).bytes;
+    if (bytes) *bytes = mm_plan(ggml_type, n, k, n_rows, 1, n_rows, false, false, out_type != QS_SRC_BF16).bytes;
     return QS_OK;
 }
 
@@ -647,7 +650,7 @@ QS_API int qs_matmul(int ggml_type, const void* w, int64_t w_row_bytes, int64_t 
     if (rc) return rc;
     if (n_rows == 0) return QS_OK;
     if ((rc = check_mm_operands(ti, w, w_row_bytes, k, x, x_row_bytes, out, out_type, out_row_stride, n))) return rc;
-    const MmPlan p = mm_plan(ggml_type, n, k, n_rows, 1, false, false, out_type != QS_SRC_BF16);
+    const MmPlan p = mm_plan(ggml_type, n, k, n_rows, 1, n_rows, false, false, out_type != QS_SRC_BF16);
     if ((rc = check_workspace(workspace, workspace_bytes, p.bytes))) return rc;
     CurrentContextGuard keep;
     int device;
@@ -670,17 +673,18 @@ QS_API int qs_matmul(int ggml_type, const void* w, int64_t w_row_bytes, int64_t 
     a.out_type = out_type;
     a.kgrid = qs::iq_kgrid(d->iq, ggml_type);
     a.fault = d->fault;
-    return run_mm(ggml_type, p, a, k, 1, nullptr, nullptr, workspace, qs::LaunchCtx{static_cast<cudaStream_t>(stream), device, d->num_sms});
+    return run_mm(ggml_type, p, a, k, n_rows, 1, nullptr, nullptr, workspace, qs::LaunchCtx{static_cast<cudaStream_t>(stream), device, d->num_sms});
 }
 
-QS_API int qs_matmul_experts_workspace(int ggml_type, int n_experts, int64_t n, int64_t k, int64_t n_tokens, int top_k, int sum, int out_type,
-                                       int64_t* bytes) {
+QS_API int qs_matmul_experts_workspace(int ggml_type, int n_experts, int64_t n, int64_t k, int64_t n_tokens, int top_k, int x_per_slot, int sum,
+                                       int out_type, int64_t* bytes) {
     const TypeInfo* ti;
     if (!is_src(out_type)) return fail(QS_EINVAL, "output type %d is not F32/F16/BF16", out_type);
     if (n_experts < 1 || n_experts > QS_MAX_EXPERTS) return fail(QS_EINVAL, "%d experts are not in 1 .. %d", n_experts, QS_MAX_EXPERTS);
     if (top_k < 1 || top_k > QS_MAX_EXPERTS) return fail(QS_EINVAL, "%d experts per token are not in 1 .. %d", top_k, QS_MAX_EXPERTS);
     if (int rc = check_mm(ggml_type, n, k, n_tokens, top_k, &ti)) return rc;
-    if (bytes) *bytes = mm_plan(ggml_type, n, k, n_tokens * top_k, n_experts, true, sum != 0, out_type != QS_SRC_BF16).bytes;
+    if (bytes) *bytes = mm_plan(ggml_type, n, k, n_tokens * top_k, n_experts, x_per_slot ? n_tokens * top_k : n_tokens, true, sum != 0,
+                                out_type != QS_SRC_BF16).bytes;
     return QS_OK;
 }
 
@@ -700,8 +704,8 @@ QS_API int qs_matmul_experts(int ggml_type, const void* w, int64_t w_row_bytes, 
     if (!ids || !order || !offsets) return fail(QS_EINVAL, "null ids, order or offsets");
     if (!aligned(ids, 4) || !aligned(order, 4) || !aligned(offsets, 4) || (weights && !aligned(weights, 4)))
         return fail(QS_EINVAL, "a pointer is not aligned to its elements");
-    const int64_t slots = n_tokens * top_k;
-    const MmPlan p = mm_plan(ggml_type, n, k, slots, n_experts, true, weights != nullptr, out_type != QS_SRC_BF16);
+    const int64_t slots = n_tokens * top_k, x_rows = x_per_slot ? slots : n_tokens;
+    const MmPlan p = mm_plan(ggml_type, n, k, slots, n_experts, x_rows, true, weights != nullptr, out_type != QS_SRC_BF16);
     if ((rc = check_workspace(workspace, workspace_bytes, p.bytes))) return rc;
     CurrentContextGuard keep;
     int device;
@@ -729,7 +733,7 @@ QS_API int qs_matmul_experts(int ggml_type, const void* w, int64_t w_row_bytes, 
     a.out_type = out_type;
     a.kgrid = qs::iq_kgrid(d->iq, ggml_type);
     a.fault = d->fault;
-    return run_mm(ggml_type, p, a, k, top_k, weights, ids, workspace,
+    return run_mm(ggml_type, p, a, k, x_rows, top_k, weights, ids, workspace,
                   qs::LaunchCtx{static_cast<cudaStream_t>(stream), device, d->num_sms});
 }
 

@@ -131,9 +131,13 @@ __device__ __forceinline__ int sum16(const uint4& v) {
 }
 
 // shared memory that the kernel for few slots may use: (32 levels, a scale, up to 2 sums) per unit
-// and slot, for up to 8 slots
-constexpr int FEW_SMEM_MAX = 200 * 1024, FEW_SLOTS = 8, FEW_UNIT_MAX = 44;
+// and slot, for up to 4 slots
+constexpr int FEW_SMEM_MAX = 200 * 1024, FEW_SLOTS = 4, FEW_UNIT_MAX = 44;
 cudaError_t launch_mm_few(int type, const MmArgs& a, const LaunchCtx& ctx);
+// up to 64 slots a matrix (qs_matmul_mid.cu): tiles of bn = 8, 16, 32 or 64 slots; ws: mm_mid_workspace
+// bytes; rows: activation rows
+inline int64_t mm_mid_workspace(int64_t units, int64_t rows, int sums) { return rows * ((units + 3) / 4 * 4) * (32 + 4 * (1 + sums)); }
+cudaError_t launch_mm_mid(int type, const MmArgs& a, int bn, int rows, void* ws, const LaunchCtx& ctx);
 // tcgen05 tiles (qs_matmul_tc.cuh): tiles of bn slots; lo: both float16 parts of the activations. ws:
 // mm_tc_workspace bytes for `chunks` chunks (the rows' powers of two lead); sums: level sums per unit
 // (1 with minima, 2 with minima per 16 values, else 0)

@@ -201,9 +201,7 @@ cudaError_t launch_few_t(const MmArgs& a, const LaunchCtx& ctx) {
 template <int T>
 cudaError_t launch_few(const MmArgs& a, const LaunchCtx& ctx) {
     // one slot per expert is the rule when a few tokens share many experts
-    if (a.slots == 1 || (a.order && a.slots <= a.n_exp)) return launch_few_t<T, 1>(a, ctx);
-    if (!a.order && a.slots <= 4) return launch_few_t<T, 4>(a, ctx);
-    return launch_few_t<T, 8>(a, ctx);
+    return a.slots == 1 || a.order ? launch_few_t<T, 1>(a, ctx) : launch_few_t<T, 4>(a, ctx);
 }
 
 }  // namespace

@@ -600,10 +600,8 @@ cudaError_t launch_tc_t(const MmArgs& a, void* ws, const LaunchCtx& ctx) {
 
 template <int T>
 cudaError_t launch_tc(const MmArgs& a, int bn, bool lo, void* ws, const LaunchCtx& ctx) {
-    if (lo) return bn == 32 ? launch_tc_t<T, 32, true>(a, ws, ctx) : bn == 64 ? launch_tc_t<T, 64, true>(a, ws, ctx) : launch_tc_t<T, 128, true>(a, ws, ctx);
-    return bn == 32   ? launch_tc_t<T, 32, false>(a, ws, ctx)
-           : bn == 64 ? launch_tc_t<T, 64, false>(a, ws, ctx)
-           : bn == 128 ? launch_tc_t<T, 128, false>(a, ws, ctx) : launch_tc_t<T, 256, false>(a, ws, ctx);
+    if (lo) return launch_tc_t<T, 128, true>(a, ws, ctx);
+    return bn == 128 ? launch_tc_t<T, 128, false>(a, ws, ctx) : launch_tc_t<T, 256, false>(a, ws, ctx);
 }
 
 }  // namespace

@@ -72,7 +72,7 @@ def lib() -> ctypes.CDLL:
             L.qs_matmul_workspace.argtypes = [c_i, c_i64, c_i64, c_i64, c_i, p_i64]
             L.qs_matmul_experts.argtypes = [c_i, c_vp, c_i64, c_i64, c_i, c_i64, c_i64, c_vp, c_i64, c_i, c_vp, c_vp, c_vp, c_i64, c_i,
                                             c_vp, c_vp, c_i, c_i64, c_vp, c_i64, c_vp]
-            L.qs_matmul_experts_workspace.argtypes = [c_i, c_i, c_i64, c_i64, c_i64, c_i, c_i, c_i, p_i64]
+            L.qs_matmul_experts_workspace.argtypes = [c_i, c_i, c_i64, c_i64, c_i64, c_i, c_i, c_i, c_i, p_i64]
             L.qs_last_error.restype = ctypes.c_char_p
             _lib = L
     return _lib

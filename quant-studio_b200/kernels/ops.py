@@ -242,7 +242,7 @@ def matmul_experts(blocks: torch.Tensor, ggml_type: int, x_q8: torch.Tensor, pla
     row = blocks.stride(1) if n > 1 else -(-blocks.shape[2] // 16) * 16  # a stride that nothing steps over fits any alignment
     expert = blocks.stride(0) if experts > 1 else n * row
     per_slot, summed = int(rows != tokens), int(weights is not None)
-    size = _experts_workspace(int(ggml_type), experts, n, k, tokens, top_k, summed, SRC_IDS[out_dtype])
+    size = _experts_workspace(int(ggml_type), experts, n, k, tokens, top_k, per_slot, summed, SRC_IDS[out_dtype])
     out = torch.empty(shape, dtype=out_dtype, device=blocks.device)
     ws = torch.empty(size, dtype=torch.uint8, device=blocks.device) if size else None
     order = plan.table.data_ptr()

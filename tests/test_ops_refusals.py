@@ -71,8 +71,8 @@ def test_matmul_type():
     assert lib().qs_matmul_workspace(12, 8, 256, 1, 0, ctypes.byref(n)) == OK and n.value == 0
     assert lib().qs_matmul_workspace(12, 8, 256, 1, 2, ctypes.byref(n)) == E
     assert lib().qs_matmul_workspace(12, 8, 256, 0, 0, ctypes.byref(n)) == OK and n.value == 0
-    assert lib().qs_matmul_experts_workspace(12, 4, 8, 256, 2, 2, 0, 0, ctypes.byref(n)) == OK and n.value == 0
-    assert lib().qs_matmul_experts_workspace(12, 4, 8, 256, 2, 2, 1, 0, ctypes.byref(n)) == OK and n.value == 2 * 2 * 8 * 4
+    assert lib().qs_matmul_experts_workspace(12, 4, 8, 256, 2, 2, 0, 0, 0, ctypes.byref(n)) == OK and n.value == 0
+    assert lib().qs_matmul_experts_workspace(12, 4, 8, 256, 2, 2, 0, 1, 0, ctypes.byref(n)) == OK and n.value == 2 * 2 * 8 * 4
 
 
 @pytest.mark.parametrize("t,al", [(12, 16), (13, 16), (7, 8), (23, 8), (3, 4), (10, 4), (2, 2), (14, 2), (18, 2)])
