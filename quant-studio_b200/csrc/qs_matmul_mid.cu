@@ -68,6 +68,9 @@ struct MidCfg {
     static constexpr int UNIT_X = BN * 32 + (1 + SUMS) * BN * 4;
     static constexpr int FIT = (MID_SMEM - MID_WARPS * OWN - BN * 16) / UNIT_X / 8 * 8, SL = FIT > 128 ? 128 : FIT;
     static constexpr int PITCH = SL * 32 + 16, OFF_XD = BN * PITCH, OFF_OWN = OFF_XD + (1 + SUMS) * SL * BN * 4;
+    // the two units of 4 that half warp x unpacks: neighbours share their bytes in most formats, Q6_K's
+    // low nibbles belong to units j and j + 2
+    __device__ static int item(int x, int h) { return T == QS_Q6_K ? x + 2 * h : 2 * x + h; }
     static constexpr int OUT_PITCH = MID_ROWS + 4;
     static constexpr int BYTES = OFF_OWN + MID_WARPS * OWN;
     static_assert(SL >= 8, "a superblock of activations");
@@ -125,7 +128,7 @@ __global__ void __launch_bounds__(MID_THREADS, 2) mid_kernel(MmArgs a, const int
 #pragma unroll
     for (int j = 0; j < NT; j++) acc[j][0] = acc[j][1] = 0ull;
     const f32x2 nmagic = f2_splat(-12582912.0f);
-    const int ir = lane & 15;  // the row that this lane unpacks, of units lane / 16 and lane / 16 + 2
+    const int ir = lane & 15;  // the row that this lane unpacks
 
     int k = 0;
     for (int us = u0; us < u1; us += SL) {
@@ -148,25 +151,29 @@ __global__ void __launch_bounds__(MID_THREADS, 2) mid_kernel(MmArgs a, const int
             __syncwarp();
             const uint8_t* raw = own + k % RR * C::RAW;
             const int live = min(RU, nu - su);
+            const uint32_t off = L::MAXAL >= 16 ? 0 : (uint32_t)(uintptr_t)(w + ir * a.w_row + (int64_t)(u0 / RU + k) * C::WB) & 15;
 #pragma unroll
             for (int q4 = 0; q4 < RU; q4 += 4) {
                 if (RU > 4 && q4 >= live) break;
+                // both units' bytes first: units that share bytes load them once
+                uint32_t r[2][L::WORDS];
 #pragma unroll
                 for (int h2 = 0; h2 < 2; h2++) {
-                    const int u = (lane >> 4) + 2 * h2, in = q4 + u;
-                    uint32_t q[8];
-                    float dl[2], ml[2];
+                    const int in = q4 + C::item(lane >> 4, h2);
                     if (ir < wrows && in < live) {
-                        const uint32_t off = L::MAXAL >= 16 ? 0 : (uint32_t)(uintptr_t)(w + ir * a.w_row + (int64_t)(u0 / RU + k) * C::WB) & 15;
-                        uint32_t r[L::WORDS];
-                        L::template load<L::MAXAL, true>(raw + ir * C::WP + off + in / UPB * L::BB, in % UPB, r);
-                        L::levels(r, in % UPB, a.kgrid, q, dl, ml);
+                        L::template load<L::MAXAL, true>(raw + ir * C::WP + off + in / UPB * L::BB, in % UPB, r[h2]);
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 8; e++) q[e] = 0;
-                        dl[0] = dl[1] = ml[0] = ml[1] = 0.0f;
+                        for (int e = 0; e < L::WORDS; e++) r[h2][e] = 0;  // zero scales
                     }
-                    if (h2 == 0) __syncwarp();  // the last 4 units are used up
+                }
+                __syncwarp();  // the last 4 units are used up
+#pragma unroll
+                for (int h2 = 0; h2 < 2; h2++) {
+                    const int u = C::item(lane >> 4, h2);
+                    uint32_t q[8];
+                    float dl[2], ml[2];
+                    L::levels(r[h2], (q4 + u) % UPB, a.kgrid, q, dl, ml);
 #pragma unroll
                     for (int h = 0; h < 2; h++)
                         *reinterpret_cast<uint4*>(lev + ir * 128 + (((2 * u + h) ^ (ir & 7)) << 4)) = make_uint4(q[4 * h], q[4 * h + 1], q[4 * h + 2], q[4 * h + 3]);
