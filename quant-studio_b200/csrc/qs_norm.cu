@@ -4,12 +4,11 @@
 //   r = 1 / sqrt(mean(t^2) + eps),  p = t * weight
 //   per 32 values: m = max |p|, levels sign(p) floor(127 |p| / m + 1/2), scale f16(m r / 127)
 //
-// The levels do not depend on r, and |p| / m is compared with the borders between two levels
-// as in 64 bits: in float32 first (error below 3e-5 of a level), and in double where a value lies
-// within 4e-5 of a border. m is kept as a float pair (product and its FMA remainder: exact) and
-// the sum of squares as a float pair per thread (TwoSum) and in double across threads, so the
-// float16 scale is the rounded float32 of the 64-bit value too. A row holding inf or NaN
-// gets NaN scales and zero levels.
+// The levels do not depend on r, and |p| / m is compared with the borders between two levels as in 64
+// bits: in float32 first, where a level's error is below 3e-5 of a step and a scale's below 3e-7; blocks
+// with a value within 4e-5 of a border, or a scale within 4e-7 of a float16 border, are done again in
+// double by their warp (about one warp pass of 8 blocks in 25). The sum of squares is in double
+// throughout. A row holding inf or NaN gets NaN scales and zero levels.
 #include "qs_kernels.h"
 
 namespace qs {
@@ -27,12 +26,6 @@ struct NormArgs {
     int k;
     double eps;
 };
-
-__device__ __forceinline__ void two_sum(float& hi, float& lo, float v) {
-    const float s = __fadd_rn(hi, v), b = __fsub_rn(s, hi);
-    lo = __fadd_rn(lo, __fadd_rn(__fsub_rn(hi, __fsub_rn(s, b)), __fsub_rn(v, b)));
-    hi = s;
-}
 
 __device__ __forceinline__ double block_sum(double v, double* red) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
@@ -122,14 +115,13 @@ __global__ void __launch_bounds__(CH == 0 ? 1024 : CH == 4 ? 512 : 1024) norm_ke
     const int64_t row = blockIdx.x;
     constexpr int NC = CH == 0 ? 1 : CH;
     float v[NC][8];
-    float hi = 0.0f, lo = 0.0f;
+    double s0 = 0.0, s1 = 0.0;
     auto add_squares = [&](const float* t) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float p = __fmul_rn(t[i], t[i]);
-            two_sum(hi, lo, p);
-            // products of 16-bit values are exact in float32
-            if constexpr (SRC == SRC_F32) lo = __fadd_rn(lo, __fmaf_rn(t[i], t[i], -p));
+        for (int i = 0; i < 8; i += 2) {
+            const double x = (double)t[i], y = (double)t[i + 1];
+            s0 = fma(x, x, s0);
+            s1 = fma(y, y, s1);
         }
     };
     if constexpr (CH == 0) {
@@ -147,25 +139,10 @@ __global__ void __launch_bounds__(CH == 0 ? 1024 : CH == 4 ? 512 : 1024) norm_ke
         for (int j = 0; j < NC; j++)
             if (tid + j * (int)blockDim.x < nchunk) add_squares(v[j]);
     }
-    double sum = block_sum((double)hi + (double)lo, red);
-    // squares beyond float32's range, or so small that they were lost: once more in double
-    if (!(sum < 1e37) || sum < 1e-27 * (double)a.k) {
-        double s = 0.0;
-        if constexpr (CH == 0) {
-            for (int c = tid; c < nchunk; c += blockDim.x) {
-                reload_chunk<SRC, RES>(a, row, c, v[0]);
-                for (int i = 0; i < 8; i++) s += (double)v[0][i] * (double)v[0][i];
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < NC; j++)
-                if (tid + j * (int)blockDim.x < nchunk)
-                    for (int i = 0; i < 8; i++) s += (double)v[j][i] * (double)v[j][i];
-        }
-        sum = block_sum(s, red);
-    }
+    const double sum = block_sum(s0 + s1, red);
     const bool bad = !(sum <= 1.7e308);
     const double r127 = 1.0 / sqrt(sum / (double)a.k + a.eps) / 127.0;
+    const float r127f = (float)r127;
     uint8_t* out = a.dst + row * a.dst_stride;
     const int rounds = (nchunk + blockDim.x - 1) / blockDim.x;
 #pragma unroll
@@ -183,51 +160,54 @@ __global__ void __launch_bounds__(CH == 0 ? 1024 : CH == 4 ? 512 : 1024) norm_ke
         float mh = 0.0f, p[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            p[i] = live ? __fmul_rn(fabsf(t[i]), fabsf(w[i])) : 0.0f;
-            mh = fmaxf(mh, p[i]);
+            p[i] = live ? __fmul_rn(t[i], w[i]) : 0.0f;
+            mh = fmaxf(mh, fabsf(p[i]));
         }
         mh = fmaxf(mh, __shfl_xor_sync(0xffffffffu, mh, 1));
         mh = fmaxf(mh, __shfl_xor_sync(0xffffffffu, mh, 2));
-        const bool plain = mh > 1e-25f && mh < 1e37f;  // products and remainders are normal numbers
-        double m;
-        {
-            float me = -INFINITY;  // the largest remainder among the largest products
+        // 127 p / m plus 1.5 * 2^23: the level is the low byte
+        const float inv = __fdiv_rn(127.0f, mh);
+        float off = 0.0f;
+        uint32_t z[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (live && p[i] == mh) me = fmaxf(me, __fmaf_rn(fabsf(t[i]), fabsf(w[i]), -p[i]));
-            me = fmaxf(me, __shfl_xor_sync(0xffffffffu, me, 1));
-            me = fmaxf(me, __shfl_xor_sync(0xffffffffu, me, 2));
-            m = (double)mh + (double)me;
+        for (int i = 0; i < 8; i++) {
+            const float y = __fmaf_rn(p[i], inv, 12582912.0f);
+            off = fmaxf(off, fabsf(__fmaf_rn(p[i], inv, -__fadd_rn(y, -12582912.0f))));
+            z[i] = __float_as_uint(y);
         }
-        if (!plain) {
-            m = 0.0;
+        uint32_t q[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+            q[i] = __byte_perm(__byte_perm(z[4 * i], z[4 * i + 1], 0x0040u), __byte_perm(z[4 * i + 2], z[4 * i + 3], 0x0040u), 0x5410u);
+        const float ds = __fmul_rn(mh, r127f);
+        uint16_t d = f16_bits(ds);
+        const bool sure = mh > 1e-25f && mh < 1e37f && off < 0.49996f &&  // products are normal numbers
+                          f16_bits(__fmul_rn(ds, 1.0f - 4e-7f)) == f16_bits(__fmul_rn(ds, 1.0f + 4e-7f));
+        if (!__all_sync(0xffffffffu, sure || !live || bad)) {
+            double m = 0.0;
+#pragma unroll
             for (int i = 0; i < 8; i++)
                 if (live) m = fmax(m, fabs((double)t[i] * (double)w[i]));
-        }
-        // the 4 lanes of a block agree on `plain`; the exchange is for all lanes
-        {
-            const double o1 = __shfl_xor_sync(0xffffffffu, m, 1);
-            if (!plain) m = fmax(m, o1);
-            const double o2 = __shfl_xor_sync(0xffffffffu, m, 2);
-            if (!plain) m = fmax(m, o2);
-        }
-        const float inv = __fdiv_rn(127.0f, mh);
-        uint32_t q[2] = {0, 0};
-        if (live && !bad && m > 0.0) {
+            m = fmax(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            m = fmax(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            q[0] = q[1] = 0;
+            if (live && m > 0.0 && m <= 1.7e308) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float u = __fadd_rn(__fmul_rn(p[i], inv), 0.5f);
-                float f = floorf(u);
-                if (!plain || u - f < 4e-5f || u - f > 1.0f - 4e-5f)
-                    f = (float)floor(__dadd_rn(__dmul_rn(127.0, fabs((double)t[i] * (double)w[i]) / m), 0.5));
-                int l = (int)f;
-                if ((__float_as_uint(t[i]) ^ __float_as_uint(w[i])) >> 31) l = -l;
-                q[i >> 2] |= (uint32_t)(l & 0xFF) << (8 * (i & 3));
+                for (int i = 0; i < 8; i++) {
+                    const double x = (double)t[i] * (double)w[i];
+                    const int l = (int)floor(__dadd_rn(__dmul_rn(127.0, fabs(x) / m), 0.5));
+                    const uint32_t byte = (uint32_t)(x < 0.0 ? -l : l) & 0xFFu;
+                    if (i < 4) q[0] |= byte << (8 * i);
+                    else q[1] |= byte << (8 * (i - 4));
+                }
             }
+            d = m <= 1.7e308 ? f16_bits((float)(m * r127)) : (uint16_t)0x7E00;
+        }
+        if (bad) {
+            q[0] = q[1] = 0;
+            d = 0x7E00;
         }
         // 34-byte blocks: staged per warp, then whole 16-byte pieces where they line up
-        const float df = (float)(m * r127);
-        const uint16_t d = bad || !(m <= 1.7e308) ? (uint16_t)0x7E00 : f16_bits(df);
         uint8_t* sb = stage[warp] + (lane >> 2) * 34;
         const int o = 2 + 8 * (lane & 3);
         __syncwarp();

@@ -24,32 +24,160 @@ __device__ __forceinline__ float logit_at(const RouteArgs& a, int64_t i) {
     return a.src == SRC_BF16 ? __uint_as_float((uint32_t)b << 16) : f16_val(b);
 }
 
-// Order of the selection values as unsigned words: larger value, larger word; 0 for what can
-// not be chosen (-inf and NaN). -0 counts as +0.
-__device__ __forceinline__ unsigned long long order_key(double v) {
-    if (!(v > -INFINITY)) return 0ull;
-    const unsigned long long b = (unsigned long long)__double_as_longlong(v + 0.0);
-    return (b >> 63) ? ~b : b | 0x8000000000000000ull;
-}
-__device__ __forceinline__ double key_value(unsigned long long k) {
-    if (k == 0ull) return -INFINITY;
-    return __longlong_as_double((long long)((k >> 63) ? k & 0x7FFFFFFFFFFFFFFFull : ~k));
-}
-
-__device__ __forceinline__ unsigned long long warp_max(unsigned long long v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const unsigned long long u = __shfl_xor_sync(0xffffffffu, v, o);
-        v = u > v ? u : v;
+// Selection values as unsigned words of the same order: larger value, larger word; 0 for what can not
+// be chosen (-inf and NaN). -0 counts as +0.
+struct Key32 {
+    typedef uint32_t K;
+    __device__ static K of(float v) {
+        if (!(v > -INFINITY)) return 0u;
+        const uint32_t b = __float_as_uint(v + 0.0f);
+        return (b >> 31) ? ~b : b | 0x80000000u;
     }
-    return v;
-}
+    __device__ static float value(K k) { return k == 0u ? -INFINITY : __uint_as_float((k >> 31) ? k & 0x7FFFFFFFu : ~k); }
+    __device__ static K warp_max(K v) { return __reduce_max_sync(0xffffffffu, v); }
+};
+struct Key64 {
+    typedef unsigned long long K;
+    __device__ static K of(double v) {
+        if (!(v > -INFINITY)) return 0ull;
+        const K b = (K)__double_as_longlong(v + 0.0);
+        return (b >> 63) ? ~b : b | 0x8000000000000000ull;
+    }
+    __device__ static double value(K k) { return k == 0ull ? -INFINITY : __longlong_as_double((long long)((k >> 63) ? k & 0x7FFFFFFFFFFFFFFFull : ~k)); }
+    __device__ static K warp_max(K v) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const K u = __shfl_xor_sync(0xffffffffu, v, o);
+            v = u > v ? u : v;
+        }
+        return v;
+    }
+};
 
 constexpr int ROUTE_WARPS = 4;
 
-// One warp per token; lane l holds experts l, l + 32, ... (EPL of them). The selection values
-// are doubles, so that near ties fall as in exact arithmetic; without a bias (and without sums
-// over groups) scores are monotone in the logits, and the logits themselves are compared.
+// The top_k experts by key, lane r keeps the r-th (-1: none is left); lane l holds the keys of experts
+// l, l + 32, ... gap: the smallest difference between two values whose order decided something
+// (sums of two count half).
+template <class W, int EPL>
+__device__ __forceinline__ int choose(const RouteArgs& a, typename W::K* key, int lane, float& gap) {
+    typedef typename W::K K;
+    gap = INFINITY;
+    if (a.n_groups > 1) {
+        // group scores; lane g (and g + 32) keeps those of its group
+        const int gs = a.n_exp / a.n_groups;
+        K gk[2] = {0, 0};
+        auto score = [&](K best, K second, int g) {
+            const K m1 = W::warp_max(best);
+            K v = m1;
+            if (a.top2) {  // one holder of the largest gives its second
+                const unsigned who = __ballot_sync(0xffffffffu, best == m1);
+                const K m2 = W::warp_max(lane == __ffs(who) - 1 ? second : best);
+                v = W::of(W::value(m1) + W::value(m2));
+            }
+            if ((g & 31) == lane) gk[g >> 5] = v;
+        };
+        if (gs % 32 == 0) {  // whole registers belong to one group: a single pass
+            K best = 0, second = 0;
+            int g = 0, left = gs;
+#pragma unroll
+            for (int i = 0; i < EPL; i++) {
+                const K k = key[i];
+                second = k > best ? best : (k > second ? k : second);
+                best = k > best ? k : best;
+                left -= 32;
+                if (left == 0) {
+                    if (g < a.n_groups) score(best, second, g);
+                    g++;
+                    left = gs;
+                    best = second = 0;
+                }
+            }
+        } else {
+            for (int g = 0; g < a.n_groups; g++) {
+                K best = 0, second = 0;
+                const int lo = g * gs - lane, hi = lo + gs;  // of 32 i
+#pragma unroll
+                for (int i = 0; i < EPL; i++)
+                    if (32 * i >= lo && 32 * i < hi) {
+                        const K k = key[i];
+                        second = k > best ? best : (k > second ? k : second);
+                        best = k > best ? k : best;
+                    }
+                score(best, second, g);
+            }
+        }
+        // keep the best groups, ties to the lowest; a group without a usable score comes last
+        unsigned long long keep = 0ull;  // bit g
+        float before = INFINITY;
+        for (int r = 0; r <= a.kept && r < a.n_groups; r++) {
+            K b = 0;
+            int bg = 0x7FFFFFFF;
+#pragma unroll
+            for (int h = 1; h >= 0; h--) {
+                const int g = lane + 32 * h;
+                if (g < a.n_groups && !((keep >> g) & 1ull) && gk[h] >= b) { b = gk[h]; bg = g; }
+            }
+            const K m = W::warp_max(b);
+            if (r == a.kept) {  // the best of the rest
+                if (m) gap = (before - (float)W::value(m)) * (a.top2 ? 0.5f : 1.0f);
+                break;
+            }
+            if (b != m) bg = 0x7FFFFFFF;
+            keep |= 1ull << __reduce_min_sync(0xffffffffu, bg);
+            before = (float)W::value(m);
+        }
+        if (gs % 32 == 0) {
+            int g = 0, left = gs;
+#pragma unroll
+            for (int i = 0; i < EPL; i++) {
+                if (g >= a.n_groups || !((keep >> g) & 1ull)) key[i] = 0;
+                left -= 32;
+                if (left == 0) {
+                    g++;
+                    left = gs;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < EPL; i++) {
+                const int e = lane + 32 * i;
+                if (e < a.n_exp && !((keep >> (e / gs)) & 1ull)) key[i] = 0;
+            }
+        }
+    }
+    // the k largest, one after the other, ties to the lowest expert
+    int my_id = -1;
+    float before = INFINITY;
+    for (int r = 0; r <= a.top_k; r++) {
+        K b = key[0];
+#pragma unroll
+        for (int i = 1; i < EPL; i++) b = key[i] > b ? key[i] : b;
+        const K m = W::warp_max(b);
+        if (m == 0) break;  // nothing usable is left
+        const float v = (float)W::value(m);
+        gap = fminf(gap, before - v);
+        before = v;
+        if (r == a.top_k) break;
+        int be = EPL;  // this lane's first holder
+#pragma unroll
+        for (int i = EPL - 1; i >= 0; i--)
+            if (key[i] == m) be = i;
+        const int mine = be < EPL ? lane + 32 * be : 0x7FFFFFFF, e = __reduce_min_sync(0xffffffffu, mine);
+        if (lane == r) my_id = e;
+#pragma unroll
+        for (int i = 0; i < EPL; i++)
+            if (mine == e && be == i) key[i] = 0;
+    }
+    return my_id;
+}
+
+// One warp per token. Without a bias (and without sums over groups) scores are monotone in the
+// logits, whose float32 values are compared as they are. Otherwise the selection values are
+// computed in float32, each within `err` of its exact value; where two of them that decide come
+// within 2 err of one another the row is done again in double, so that near ties fall as in
+// exact arithmetic (about one row in 1000 for 256 experts; doubles throughout took 43 us instead of
+// the time below for 8192 rows).
 template <int EPL>
 __global__ void __launch_bounds__(32 * ROUTE_WARPS) route_kernel(RouteArgs a) {
     const int lane = threadIdx.x & 31;
@@ -68,105 +196,66 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS) route_kernel(RouteArgs a) {
     // exp(z - zmax); the largest (+inf too) gives 1
     auto soft = [&](float v) { return v == zmax ? 1.0 : exp((double)v - (double)zmax); };
     auto sigm = [&](float v) { return 1.0 / (1.0 + exp(-(double)v)); };
-    double sum = 1.0;
-    unsigned long long key[EPL];
-    if (direct) {
+    auto bias = [&](int i) { return a.bias && lane + 32 * i < a.n_exp ? __ldg(a.bias + lane + 32 * i) : 0.0f; };
+    double sum = 1.0;  // of all softmax scores, where it is needed
+    int my_id;
+    float gap;
+    {
+        uint32_t key[EPL];
+        if (direct) {
 #pragma unroll
-        for (int i = 0; i < EPL; i++) key[i] = order_key((double)z[i]);
-        if (!a.sigmoid && !a.renorm) {
-            sum = 0.0;
-#pragma unroll
-            for (int i = 0; i < EPL; i++)
-                if (key[i]) sum += soft(z[i]);
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        }
-    } else {
-        double s[EPL];
-        sum = 0.0;
-#pragma unroll
-        for (int i = 0; i < EPL; i++) {
-            s[i] = !(z[i] > -INFINITY) ? 0.0 : a.sigmoid ? sigm(z[i]) : soft(z[i]);
-            sum += s[i];
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (a.sigmoid) sum = 1.0;
-#pragma unroll
-        for (int i = 0; i < EPL; i++) {
-            const int e = lane + 32 * i;
-            const bool can = z[i] > -INFINITY;
-            key[i] = can ? order_key((a.sigmoid ? s[i] : s[i] / sum) + (a.bias ? (double)__ldg(a.bias + e) : 0.0)) : 0ull;
-        }
-    }
-    if (a.n_groups > 1) {
-        // group scores; lane g (and g + 32) keeps those of its group
-        const int gs = a.n_exp / a.n_groups;
-        unsigned long long gk[2] = {0ull, 0ull};
-        for (int g = 0; g < a.n_groups; g++) {
-            unsigned long long best = 0ull;
+            for (int i = 0; i < EPL; i++) key[i] = Key32::of(z[i]);
+            my_id = choose<Key32, EPL>(a, key, lane, gap);
+        } else {
+            float s[EPL], total = 0.0f, top = 0.0f;
 #pragma unroll
             for (int i = 0; i < EPL; i++) {
-                const int e = lane + 32 * i;
-                if (e / gs == g && key[i] > best) best = key[i];
+                const bool can = z[i] > -INFINITY;
+                s[i] = !can ? 0.0f : a.sigmoid ? __fdividef(1.0f, 1.0f + expf(-z[i])) : z[i] == zmax ? 1.0f : expf(z[i] - zmax);
+                total += s[i];
             }
-            const unsigned long long m1 = warp_max(best);
-            unsigned long long score = m1;
-            if (a.top2) {
-                // the second largest: the first one's lowest-numbered holder steps aside
-                int mine = 0x7FFFFFFF;
+            float inv = 1.0f;
+            if (!a.sigmoid) {
 #pragma unroll
-                for (int i = EPL - 1; i >= 0; i--) {
-                    const int e = lane + 32 * i;
-                    if (e / gs == g && key[i] == m1) mine = e;
-                }
-                const int first = __reduce_min_sync(0xffffffffu, mine);
-                best = 0ull;
+                for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+                inv = total > 0.0f ? __frcp_rn(total) : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < EPL; i++) {
+                const float b = bias(i);
+                if (fabsf(b) < INFINITY) top = fmaxf(top, fabsf(b));
+                key[i] = z[i] > -INFINITY ? Key32::of(s[i] * inv + b) : 0u;
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            my_id = choose<Key32, EPL>(a, key, lane, gap);
+            // scores are at most 1 and good to 24 + EPL float32 steps of it (the exponential, its rounded
+            // argument, the sum and the reciprocal), the sum with the bias to one of 1 + |bias|
+            const float err = (1.0f + top) * (24.0f + EPL) * 5.9604645e-8f;
+            if (!(gap > 2.0f * err)) {
+                unsigned long long wide[EPL];
+                double d[EPL];
+                double all = 0.0;
 #pragma unroll
                 for (int i = 0; i < EPL; i++) {
-                    const int e = lane + 32 * i;
-                    if (e / gs == g && e != first && key[i] > best) best = key[i];
+                    d[i] = !(z[i] > -INFINITY) ? 0.0 : a.sigmoid ? sigm(z[i]) : soft(z[i]);
+                    all += d[i];
                 }
-                score = order_key(key_value(m1) + key_value(warp_max(best)));
-            }
-            if ((g & 31) == lane) gk[g >> 5] = score;
-        }
-        // keep the best groups, ties to the lowest; a group without a usable score comes last
-        unsigned long long keep = 0ull;  // bit g
-        for (int r = 0; r < a.kept; r++) {
-            unsigned long long b = 0ull;
-            int bg = 0x7FFFFFFF;
 #pragma unroll
-            for (int h = 1; h >= 0; h--) {
-                const int g = lane + 32 * h;
-                if (g < a.n_groups && !((keep >> g) & 1ull) && gk[h] >= b) { b = gk[h]; bg = g; }
-            }
-            const unsigned long long m = warp_max(b);
-            if (b != m) bg = 0x7FFFFFFF;
-            keep |= 1ull << __reduce_min_sync(0xffffffffu, bg);
-        }
+                for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
 #pragma unroll
-        for (int i = 0; i < EPL; i++) {
-            const int e = lane + 32 * i;
-            if (e < a.n_exp && !((keep >> (e / gs)) & 1ull)) key[i] = 0ull;
+                for (int i = 0; i < EPL; i++) wide[i] = z[i] > -INFINITY ? Key64::of((a.sigmoid ? d[i] : d[i] / all) + (double)bias(i)) : 0ull;
+                my_id = choose<Key64, EPL>(a, wide, lane, gap);
+            }
         }
     }
-    // the k largest, one after the other, ties to the lowest expert; lane r keeps the r-th
-    int my_id = -1;
-    for (int r = 0; r < a.top_k; r++) {
-        unsigned long long b = 0ull;
-        int be = 0x7FFFFFFF;
-#pragma unroll
-        for (int i = EPL - 1; i >= 0; i--)
-            if (key[i] >= b && key[i]) { b = key[i]; be = lane + 32 * i; }
-        const unsigned long long m = warp_max(b);
-        if (m == 0ull) break;  // nothing usable is left
-        if (b != m) be = 0x7FFFFFFF;
-        const int e = __reduce_min_sync(0xffffffffu, be);
-        if (lane == r) my_id = e;
+    if (!a.sigmoid && !a.renorm) {
+        sum = 0.0;
 #pragma unroll
         for (int i = 0; i < EPL; i++)
-            if (lane + 32 * i == e) key[i] = 0ull;
+            if (z[i] > -INFINITY) sum += soft(z[i]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     }
     const float v = my_id >= 0 ? logit_at(a, row * a.stride + my_id) : -INFINITY;
     if (a.renorm && !a.sigmoid) {  // any common factor cancels: the largest chosen one is 1
