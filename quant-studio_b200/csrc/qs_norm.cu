@@ -24,8 +24,17 @@ struct NormArgs {
     int64_t x_stride, res_stride, total_stride;  // elements
     int64_t dst_stride;                          // bytes
     int k;
-    double eps;
+    double eps, inv_k;
 };
+
+// 1 / sqrt(x) to about one step: two Newton steps from the float32 approximation (2^-22, squared twice)
+__device__ __forceinline__ double rsqrt64(double x) {
+    if (!(x > 1e-30 && x < 1e30)) return 1.0 / sqrt(x);
+    double y = (double)rsqrtf((float)x);
+#pragma unroll
+    for (int i = 0; i < 2; i++) y = fma(y * 0.5, fma(-x * y, y, 1.0), y);
+    return y;
+}
 
 __device__ __forceinline__ double block_sum(double v, double* red) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
@@ -108,7 +117,7 @@ __device__ __forceinline__ void reload_chunk(const NormArgs& a, int64_t row, int
 // thread keeps in registers between the two passes over the row; CH = 0: rows longer than the
 // registers hold, read twice (the second time from L2).
 template <int SRC, bool RES, int CH>
-__global__ void __launch_bounds__(CH == 0 ? 1024 : CH == 4 ? 512 : 1024) norm_kernel(NormArgs a) {
+__global__ void __launch_bounds__(1024) norm_kernel(NormArgs a) {
     __shared__ double red[32];
     __shared__ __align__(16) uint8_t stage[32][272];  // 8 blocks per warp
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nchunk = a.k >> 3;
@@ -139,9 +148,12 @@ __global__ void __launch_bounds__(CH == 0 ? 1024 : CH == 4 ? 512 : 1024) norm_ke
         for (int j = 0; j < NC; j++)
             if (tid + j * (int)blockDim.x < nchunk) add_squares(v[j]);
     }
+    // the first weights are on their way during the sum
+    float w[8];
+    if (tid < nchunk) load_f32<8>(a.w + 8 * (int64_t)tid, w);
     const double sum = block_sum(s0 + s1, red);
     const bool bad = !(sum <= 1.7e308);
-    const double r127 = 1.0 / sqrt(sum / (double)a.k + a.eps) / 127.0;
+    const double r127 = rsqrt64(fma(sum, a.inv_k, a.eps)) * (1.0 / 127.0);
     const float r127f = (float)r127;
     uint8_t* out = a.dst + row * a.dst_stride;
     const int rounds = (nchunk + blockDim.x - 1) / blockDim.x;
@@ -152,10 +164,9 @@ __global__ void __launch_bounds__(CH == 0 ? 1024 : CH == 4 ? 512 : 1024) norm_ke
         if (c0 >= nchunk) break;  // whole warps leave together
         float* t = v[CH == 0 ? 0 : j];
         const bool live = c < nchunk;  // nchunk is a multiple of 4: the 4 lanes of a block agree
-        float w[8];
         if (live) {
             if constexpr (CH == 0) reload_chunk<SRC, RES>(a, row, c, t);
-            load_f32<8>(a.w + 8 * (int64_t)c, w);
+            if (j > 0) load_f32<8>(a.w + 8 * (int64_t)c, w);
         }
         float mh = 0.0f, p[8];
 #pragma unroll
@@ -166,7 +177,7 @@ __global__ void __launch_bounds__(CH == 0 ? 1024 : CH == 4 ? 512 : 1024) norm_ke
         mh = fmaxf(mh, __shfl_xor_sync(0xffffffffu, mh, 1));
         mh = fmaxf(mh, __shfl_xor_sync(0xffffffffu, mh, 2));
         // 127 p / m plus 1.5 * 2^23: the level is the low byte
-        const float inv = __fdiv_rn(127.0f, mh);
+        const float inv = __fdividef(127.0f, mh);
         float off = 0.0f;
         uint32_t z[8];
 #pragma unroll
@@ -181,27 +192,51 @@ __global__ void __launch_bounds__(CH == 0 ? 1024 : CH == 4 ? 512 : 1024) norm_ke
             q[i] = __byte_perm(__byte_perm(z[4 * i], z[4 * i + 1], 0x0040u), __byte_perm(z[4 * i + 2], z[4 * i + 3], 0x0040u), 0x5410u);
         const float ds = __fmul_rn(mh, r127f);
         uint16_t d = f16_bits(ds);
-        const bool sure = mh > 1e-25f && mh < 1e37f && off < 0.49996f &&  // products are normal numbers
-                          f16_bits(__fmul_rn(ds, 1.0f - 4e-7f)) == f16_bits(__fmul_rn(ds, 1.0f + 4e-7f));
-        if (!__all_sync(0xffffffffu, sure || !live || bad)) {
-            double m = 0.0;
+        const bool normal = mh > 1e-25f && mh < 1e37f;  // products and their remainders are normal numbers
+        const bool sure = off < 0.49996f && f16_bits(__fmul_rn(ds, 1.0f - 4e-7f)) == f16_bits(__fmul_rn(ds, 1.0f + 4e-7f));
+        if (!__all_sync(0xffffffffu, (normal && sure) || !live || bad)) {
+            if (__all_sync(0xffffffffu, normal || !live || bad)) {
+                // the block's exact largest product: the largest remainder among the largest products
+                float me = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (live) m = fmax(m, fabs((double)t[i] * (double)w[i]));
-            m = fmax(m, __shfl_xor_sync(0xffffffffu, m, 1));
-            m = fmax(m, __shfl_xor_sync(0xffffffffu, m, 2));
-            q[0] = q[1] = 0;
-            if (live && m > 0.0 && m <= 1.7e308) {
+                for (int i = 0; i < 8; i++)
+                    if (live && fabsf(p[i]) == mh) me = fmaxf(me, __fmaf_rn(fabsf(t[i]), fabsf(w[i]), -fabsf(p[i])));
+                me = fmaxf(me, __shfl_xor_sync(0xffffffffu, me, 1));
+                me = fmaxf(me, __shfl_xor_sync(0xffffffffu, me, 2));
+                const double m = (double)mh + (double)me;
+                d = f16_bits((float)(m * r127));
+                // a value next to a border: on which side 127 x lies of m times the border (a half; on it,
+                // away from zero)
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const double x = (double)t[i] * (double)w[i];
-                    const int l = (int)floor(__dadd_rn(__dmul_rn(127.0, fabs(x) / m), 0.5));
-                    const uint32_t byte = (uint32_t)(x < 0.0 ? -l : l) & 0xFFu;
-                    if (i < 4) q[0] |= byte << (8 * i);
-                    else q[1] |= byte << (8 * (i - 4));
+                    const float n = __fadd_rn(__uint_as_float(z[i]), -12582912.0f), f = __fmaf_rn(p[i], inv, -n);
+                    if (live && fabsf(f) >= 0.49996f) {
+                        const double h = (double)n + (f > 0.0f ? 0.5 : -0.5), x = (double)t[i] * (double)w[i];
+                        // the distance from the border: next to it both differences are exact
+                        const double y = 127.0 * x, over = fma(-h, m, y) + fma(127.0, x, -y);
+                        const int level = (int)(over > 0.0 || (over == 0.0 && h > 0.0) ? h + 0.5 : h - 0.5);
+                        const int sh = 8 * (i & 3);
+                        q[i >> 2] = (q[i >> 2] & ~(0xFFu << sh)) | (((uint32_t)level & 0xFFu) << sh);
+                    }
                 }
+            } else {
+                double m = 0.0;
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (live) m = fmax(m, fabs((double)t[i] * (double)w[i]));
+                m = fmax(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                m = fmax(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                q[0] = q[1] = 0;
+                if (live && m > 0.0 && m <= 1.7e308) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const double x = (double)t[i] * (double)w[i];
+                        const int l = (int)floor(__dadd_rn(__dmul_rn(127.0, fabs(x) / m), 0.5));
+                        q[i >> 2] |= ((uint32_t)(x < 0.0 ? -l : l) & 0xFFu) << (8 * (i & 3));
+                    }
+                }
+                d = m <= 1.7e308 ? f16_bits((float)(m * r127)) : (uint16_t)0x7E00;
             }
-            d = m <= 1.7e308 ? f16_bits((float)(m * r127)) : (uint16_t)0x7E00;
         }
         if (bad) {
             q[0] = q[1] = 0;
@@ -234,10 +269,10 @@ template <int SRC, bool RES>
 cudaError_t launch_t(const NormArgs& a, int64_t rows, const LaunchCtx& ctx) {
     const int nchunk = a.k / 8;
     const int whole = (nchunk + 31) / 32 * 32;
-    // Few rows: as many threads per row as it has chunks (latency). Many: 4 chunks a thread.
+    // Few rows: as many threads per row as it has chunks (latency). Many: 2 chunks a thread.
     const bool few = rows < 4 * (int64_t)ctx.num_sms;
     if (few && whole <= 1024) norm_kernel<SRC, RES, 1><<<(unsigned)rows, whole, 0, ctx.stream>>>(a);
-    else if (nchunk <= 4 * 512) norm_kernel<SRC, RES, 4><<<(unsigned)rows, ((nchunk + 3) / 4 + 31) / 32 * 32, 0, ctx.stream>>>(a);
+    else if (nchunk <= 2 * 1024) norm_kernel<SRC, RES, 2><<<(unsigned)rows, ((nchunk + 1) / 2 + 31) / 32 * 32, 0, ctx.stream>>>(a);
     else norm_kernel<SRC, RES, 0><<<(unsigned)rows, 1024, 0, ctx.stream>>>(a);
     return cudaGetLastError();
 }
@@ -262,6 +297,7 @@ cudaError_t launch_rms_norm_q8(const NormCall& c, const LaunchCtx& ctx) {
     a.dst_stride = c.dst_row_bytes;
     a.k = (int)c.k;
     a.eps = c.eps;
+    a.inv_k = 1.0 / (double)c.k;
     switch (c.x_type) {
     case SRC_F32: return launch_s<SRC_F32>(a, c.n_rows, ctx);
     case SRC_F16: return launch_s<SRC_F16>(a, c.n_rows, ctx);
