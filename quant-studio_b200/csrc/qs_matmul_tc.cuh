@@ -19,19 +19,20 @@
 // for 2048 slots of Q4_K 14336 x 4096: three float32 operations per value and unit are 768 cycles
 // (a packed f32x2 operation takes two), an SM has no more than 128 lanes.
 //
-// Roles in a CTA (one per SM, 12 warps):
-//   warps 0-7  unpack the weights (thread = row and unit of the stage) and own the tile's sums (lane =
-//              weight row, each warp half of the columns), which they collect LAG stages behind
-//   warp 8     issues the matrix products (and owns the tensor memory)
-//   warp 9     copies the activations' stage (one bulk copy: float16 rows as the matrix unit reads
-//              them), laid out beforehand by xpack_kernel
-//   warps 10, 11  copy the weights' bytes (cp.async) in steps of RS stages: the 16-byte pieces that
-//              cover a row's share wherever it starts, adjacent lanes adjacent pieces
+// Roles in a CTA (one per SM, 20 warps):
+//   warps 0-7    own the tile's sums: lane = weight row, each warp half of the columns
+//   warps 8-15   unpack the weights, warps 8-11 the even stages, 12-15 the odd ones (thread = row, both
+//                units of the stage: a stage's unpacking is mostly latency, so two are under way)
+//   warp 16      issues the matrix products (and owns the tensor memory)
+//   warp 17      copies the activations' stage (one bulk copy: float16 rows as the matrix unit reads
+//                them), laid out beforehand by xpack_kernel
+//   warps 18, 19 copy the weights' bytes (cp.async) in steps of RS stages: the 16-byte pieces that
+//                cover a row's share wherever it starts, adjacent lanes adjacent pieces
 // Stages are a ring in shared memory (full: unpacked + copied, empty: products done); the
 // accumulators are a ring in tensor memory; the weights' scales are a longer ring of their own, which
-// no warp can lap: unpacking stage i waits for the products of stage i - NS, these for every warp's
-// stage i - NS, and that warp has then collected stage i - NS - 1 - LAG. Every wait is bounded: one that
-// runs out records bit 0 of the fault word and its role leaves.
+// the unpacking can not lap: stage i waits for the products of stage i - NS, these for the release of
+// their accumulator, so the sums are at most NS + 7 stages behind. Every wait is bounded: one that runs
+// out records bit 0 of the fault word and its role leaves.
 // The order of the 32 values within a unit does not matter to the sum; both operands use the one
 // that unpacks cheapest (word_halves).
 #pragma once
@@ -46,7 +47,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int TC_M = 128, TC_THREADS = 384;
+constexpr int TC_M = 128, TC_THREADS = 640;
 constexpr int TC_SMEM = 227 * 1024;
 
 template <int T, int BN, bool LO>
@@ -62,18 +63,18 @@ struct TcCfg {
     static constexpr int RS = L::QK == 256 ? 4 : 2, WB = RS * 64 / L::QK * L::BB;
     static constexpr int COVER = L::MAXAL >= 16 ? WB : (WB + 16 - L::MAXAL + 15) / 16 * 16, WP = COVER / 16 % 2 ? COVER : COVER + 16;
     static constexpr int RAW = TC_M * WP, RR = 2 * RAW <= 24 * 1024 ? 4 : 2;  // steps in the ring
-    static constexpr int DR = 8;                       // ring of scales, [slot][unit][128]
+    static constexpr int DR = 16;                      // ring of scales, [slot][unit][128]
     static constexpr int D_BYTES = DR * 2 * TC_M * 4;
     static constexpr int FIT = (TC_SMEM - 1024 - 512 - BN * 8 - D_BYTES - RR * RAW) / STAGE, NS = FIT > 4 ? 4 : FIT;
-    static constexpr int LAG = !GROUP ? 1 : NS > 3 ? 3 : NS - 1;
     static constexpr int NB = BN == 256 ? 2 : 4;       // accumulators in tensor memory
     static constexpr int COLS = NB * BN;
-    // 256 columns are 128 registers a thread for the sums alone: the third warpgroup's registers move to
-    // the other two (232, 232, 40 a thread of the 168 at launch)
-    static constexpr bool MOVE = BN == 256;
+    // the sums of 256 columns are 128 registers a thread: registers move to their two warpgroups
+    // (160, 160, 64, 64, 32 a thread of the 96 at launch)
+    static constexpr int R_SUM = 160, R_UNPACK = 64, R_REST = 32, R_LAUNCH = 96;
+    static_assert(2 * R_SUM + 2 * R_UNPACK + R_REST <= 5 * R_LAUNCH, "the shares are what the launch has");
     static constexpr int OUT_PITCH = TC_M + 4;
     static constexpr int BYTES = NS * STAGE + D_BYTES + RR * RAW + 1024;  // 1024 to align the ring
-    static_assert(NS >= LAG + 1 && DR >= NS + 1 + LAG, "ring lengths");
+    static_assert(NS >= 2 && DR >= NS + 8, "ring lengths");
     static_assert(BN * OUT_PITCH * 4 <= NS * STAGE, "the tile leaves through the same memory");
     // further stages with the minima of `units` units: 64 terms each, with LO once for the hi and
     // once for the lo part of the weights' side
@@ -151,6 +152,12 @@ __device__ __forceinline__ void word_halves(uint32_t w, __half2 bias, __half2* h
     const uint32_t a = (w & 0x00FF00FFu) | 0x64006400u, b = ((w >> 8) & 0x00FF00FFu) | 0x64006400u;
     h[0] = __hsub2(*reinterpret_cast<const __half2*>(&a), bias);
     h[1] = __hsub2(*reinterpret_cast<const __half2*>(&b), bias);
+}
+// the same, times sc plus less
+__device__ __forceinline__ void word_fma(uint32_t w, __half2 sc, __half2 less, __half2* h) {
+    const uint32_t a = (w & 0x00FF00FFu) | 0x64006400u, b = ((w >> 8) & 0x00FF00FFu) | 0x64006400u;
+    h[0] = __hfma2(*reinterpret_cast<const __half2*>(&a), sc, less);
+    h[1] = __hfma2(*reinterpret_cast<const __half2*>(&b), sc, less);
 }
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 
@@ -230,7 +237,7 @@ template <int T, int BN, bool LO>
 __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8_t* xp, const float* xs) {
     using L = Lv<T>;
     using C = TcCfg<T, BN, LO>;
-    constexpr int UPB = L::QK / 32, SUMS = C::SUMS, NS = C::NS, NB = C::NB, GROUP = C::GROUP, LAG = C::LAG, RS = C::RS, RR = C::RR;
+    constexpr int UPB = L::QK / 32, SUMS = C::SUMS, NS = C::NS, NB = C::NB, GROUP = C::GROUP, RS = C::RS, RR = C::RR;
     constexpr int HALF = BN / 2;  // columns of a warp
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[2 * NS + 2 * NB + 2 * RR];
@@ -248,11 +255,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
                    raw_full = acc_empty + 8 * NB, raw_empty = raw_full + 8 * RR;
     if (tid == 0) {
         for (int s = 0; s < NS; s++) {
-            mbar_init(full + 8 * s, 8 + 1);
+            mbar_init(full + 8 * s, 4 + 1);
             mbar_init(empty + 8 * s, 1);
         }
         for (int b = 0; b < NB; b++) {
-            mbar_init(acc_full + 8 * b, 1);
+            mbar_init(acc_full + 8 * b, 2);
             mbar_init(acc_empty + 8 * b, 8);
         }
         for (int r = 0; r < RR; r++) {
@@ -268,7 +275,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
             s_up[t] = some ? __ldg(xs + (int64_t)blockIdx.y * BN + t) : 1.0f;
         }
     }
-    if (warp == 8) {
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "n"(C::COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
@@ -289,9 +296,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
     auto begins = [&](int i, int uu) { return !GROUP || i >= main || (uu == 0 && i % (GROUP ? GROUP : 1) == 0); };
     auto ends = [&](int i, int uu) { return !GROUP || i >= main || (uu == 1 && (i % (GROUP ? GROUP : 1) == GROUP - 1 || i + 1 == main)); };
 
-    if (warp >= 8) {
-        if constexpr (C::MOVE) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-        if (warp == 8) {
+    if (warp >= 16) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::R_REST));
+        if (warp == 16) {
             // the whole warp runs the loop, so that addresses stay in uniform registers; one lane issues
             const bool leader = elect_one();
             // D float32, A and B float16 K-major, N = BN, M = 128
@@ -318,7 +325,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
                         }
                     }
                     if (ends(i, uu)) {
-                        if (leader) mma_commit(acc_full + 8 * b);
+                        // the products' end, and a release of its own for the scales that came with `full`
+                        if (leader) {
+                            mma_commit(acc_full + 8 * b);
+                            mbar_arrive(acc_full + 8 * b);
+                        }
                         if (++b == NB) {
                             b = 0;
                             b_ph ^= 1;
@@ -336,10 +347,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
             asm volatile("bar.sync 1, 288;" ::: "memory");  // the sums' warps have read their last accumulator
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(C::COLS));
-        } else if (warp >= 10) {
+        } else if (warp >= 18) {
             // one warp half of the rows each; adjacent lanes take adjacent pieces of a row
             constexpr int P = C::COVER / 16, HALF_ROWS = TC_M / 2;
-            const int first = (warp - 10) * HALF_ROWS, rows = min(HALF_ROWS, a.n - n0 - first), steps = (main + RS - 1) / RS;
+            const int first = (warp - 18) * HALF_ROWS, rows = min(HALF_ROWS, a.n - n0 - first), steps = (main + RS - 1) / RS;
             const uint8_t* w = a.w + (real ? ch.group * a.w_exp : 0) + (int64_t)(n0 + first) * a.w_row;
             const int64_t len = (int64_t)a.units / UPB * L::BB;
             for (int k = 0; k < steps; k++) {
@@ -357,7 +368,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
                 asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(raw_full + 8 * r) : "memory");
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
-        } else if (warp == 9 && lane == 0) {
+        } else if (warp == 17 && lane == 0) {
             const uint8_t* src = xp + (int64_t)blockIdx.y * (stages + blocks) * C::X_BYTES;
             int i = 0;
             for (; i < total; i++) {
@@ -369,152 +380,167 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
             // no copy outlives the CTA
             for (int j = max(0, i - NS); j < i; j++) mbar_wait(full + 8 * (j % NS), (j / NS) & 1, a.fault);
         }
-    } else {
-        if constexpr (C::MOVE) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
-        const int row = tid & 127, my = tid >> 7;  // weight row of the tile, unit of the stage
+    } else if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::R_UNPACK));
+        const int row = tid & 127, odd = (warp - 8) >> 2;  // weight row of the tile, stages 2 j + odd
         const bool mine = n0 + row < a.n;
         const uint8_t* w = a.w + (real ? ch.group * a.w_exp : 0) + (int64_t)(mine ? n0 + row : 0) * a.w_row;
-        const int c0 = my * HALF;
+        auto put = [&](uint8_t* st, int c, const __half2* h) {  // piece c of the row
+            *reinterpret_cast<uint4*>(st + row * 128 + ((c ^ (row & 7)) << 4)) = make_uint4(h2_bits(h[0]), h2_bits(h[1]), h2_bits(h[2]), h2_bits(h[3]));
+        };
+        // k0 is a whole number of steps, so stage i is stage i % RS of step i / RS
+        auto unpack = [&](int i, uint8_t* st, const uint8_t* bytes) {
+            const uint32_t off = L::MAXAL >= 16 ? 0 : (uint32_t)(uintptr_t)(w + (int64_t)(k0 / RS + i / RS) * C::WB) & 15;
+            uint32_t r[2][L::WORDS];
+#pragma unroll
+            for (int uu = 0; uu < 2; uu++) {
+                const int in = 2 * (i % RS) + uu;
+                if (mine && 2 * (k0 + i) + uu < a.units) {
+                    L::template load<L::MAXAL, true>(bytes + row * C::WP + off + in / UPB * L::BB, in % UPB, r[uu]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < L::WORDS; e++) r[uu][e] = 0;  // zero scales
+                }
+            }
+#pragma unroll
+            for (int uu = 0; uu < 2; uu++) {
+                const int j = (2 * (i % RS) + uu) % UPB;
+                uint32_t q[8];
+                float dl[2], ml[2];
+                L::levels(r[uu], j, a.kgrid, q, dl, ml);
+                // the bytes' float16 is 1024 + byte; less the bias, times the sub-scale: one exact operation
+                // where bias * sub-scale is a float16 (not for Q6_K's factors of up to 128)
+                constexpr float BIAS = L::SIGNED ? 1152.0f : 1024.0f;
+                constexpr uint32_t FLIP = L::SIGNED ? 0x80808080u : 0u;
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    __half2 h[4];
+                    if constexpr (L::FOLD && T != QS_Q6_K) {
+                        const float sub = (float)L::sub(r[uu], j, c >> 1);
+                        const __half2 sc = __float2half2_rn(sub), less = __float2half2_rn(-BIAS * sub);
+                        word_fma(q[2 * c] ^ FLIP, sc, less, h);
+                        word_fma(q[2 * c + 1] ^ FLIP, sc, less, h + 2);
+                    } else {
+                        const __half2 bias = __float2half2_rn(BIAS);
+                        word_halves(q[2 * c] ^ FLIP, bias, h);
+                        word_halves(q[2 * c + 1] ^ FLIP, bias, h + 2);
+                        if constexpr (L::FOLD) {
+                            const __half2 sc = __float2half2_rn((float)L::sub(r[uu], j, c >> 1));
+                            __half2 p[4];
+#pragma unroll
+                            for (int e = 0; e < 4; e++) p[e] = __hmul2(h[e], sc);
+                            if constexpr (C::SPLIT) {  // the product's rounding error, exact in float16
+#pragma unroll
+                                for (int e = 0; e < 4; e++) h[e] = __hfma2(h[e], sc, __hneg2(p[e]));
+                                put(st + C::A_BYTES, 4 * uu + c, h);
+                            }
+#pragma unroll
+                            for (int e = 0; e < 4; e++) h[e] = p[e];
+                        }
+                    }
+                    put(st, 4 * uu + c, h);
+                }
+                scales[((i % C::DR) * 2 + uu) * TC_M + row] = L::FOLD ? base_of<L>(r[uu]) : dl[0];
+            }
+        };
+        // 2 x 32 minima of the row (negated), each half times a power of two, its inverse (and the sums' 2^7)
+        // as the scale
+        auto unpack_minima = [&](int i, uint8_t* st) {
+            if constexpr (SUMS > 0) {
+                constexpr int PER = UPB * SUMS;  // minima of a block
+                const int e = (i - main) / (LO ? 2 : 1), part = LO ? (i - main) & 1 : 0;
+#pragma unroll 1
+                for (int uu = 0; uu < 2; uu++) {
+                    const int p0 = (e0 + e) * 64 + uu * 32;
+                    float m[32], top = 0.0f;
+#pragma unroll
+                    for (int p = 0; p < 32; p += PER) {
+                        const bool in = mine && p0 + p < a.units * SUMS;
+#pragma unroll
+                        for (int j = 0; j < PER; j++) m[p + j] = 0.0f;
+                        if (in) L::template minima<L::MAXAL>(w + (int64_t)((p0 + p) / PER) * L::BB, m + p);
+                    }
+#pragma unroll
+                    for (int p = 0; p < 32; p++) top = fmaxf(top, fabsf(m[p]));
+                    float up = 1.0f;  // the largest below 2^11
+                    if (top > 0.0f && top < INFINITY) up = __uint_as_float((uint32_t)(127 + 10 + 127 - (int)(__float_as_uint(top) >> 23)) << 23);
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        __half2 h[4];
+#pragma unroll
+                        for (int x = 0; x < 4; x++) {
+                            const float v0 = -m[8 * c + 2 * x] * up, v1 = -m[8 * c + 2 * x + 1] * up;
+                            h[x] = __floats2half2_rn(v0, v1);
+                            if (LO && part) {
+                                const float2 f = __half22float2(h[x]);
+                                h[x] = __floats2half2_rn(v0 - f.x, v1 - f.y);
+                            }
+                        }
+                        put(st, 4 * uu + c, h);
+                    }
+                    scales[((i % C::DR) * 2 + uu) * TC_M + row] = 128.0f / up;
+                }
+            }
+        };
+        int s = odd % NS, ph = odd / NS & 1 ? 0 : 1;  // stage of the ring, the parity that its last use ended with
+        for (int i = odd; i < total; i += 2) {
+            if (!mbar_wait(empty + 8 * s, ph, a.fault)) break;
+            uint8_t* st = ring_p + s * C::STAGE;
+            if (i < main) {
+                const int k = i / RS, r = k % RR;
+                if (i % RS == odd && !mbar_wait(raw_full + 8 * r, (k / RR) & 1, a.fault)) break;
+                unpack(i, st, bytes_p + r * C::RAW);
+                if (i % RS == RS - 2 + odd) {  // this half's last stage of the step
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(raw_empty + 8 * r);
+                }
+            } else {
+                unpack_minima(i, st);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full + 8 * s);
+            s += 2;
+            if (s >= NS) {
+                s -= NS;
+                ph ^= 1;
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::R_SUM));
+        const int row = (warp & 3) * 32 + lane, c0 = (warp >> 2) * HALF;
         constexpr int NBT = HALF / 16;
         f32x2 acc[HALF / 2];
 #pragma unroll
         for (int i = 0; i < HALF / 2; i++) acc[i] = 0ull;
-        auto put = [&](uint8_t* st, int c, const __half2* h) {
-            *reinterpret_cast<uint4*>(st + row * 128 + (((4 * my + c) ^ (row & 7)) << 4)) = make_uint4(h2_bits(h[0]), h2_bits(h[1]), h2_bits(h[2]), h2_bits(h[3]));
-        };
-        // k0 is a whole number of steps, so stage i is stage i % RS of step i / RS
-        auto unpack = [&](int i, uint8_t* st) {
-            const int u = 2 * (k0 + i) + my, in = 2 * (i % RS) + my, j = in % UPB;
-            uint32_t r[L::WORDS];
-            if (mine && u < a.units) {
-                const uint32_t off = L::MAXAL >= 16 ? 0 : (uint32_t)(uintptr_t)(w + (int64_t)(k0 / RS + i / RS) * C::WB) & 15;
-                L::template load<L::MAXAL, true>(bytes_p + (i / RS) % RR * C::RAW + row * C::WP + off + in / UPB * L::BB, j, r);
-            } else {
-#pragma unroll
-                for (int e = 0; e < L::WORDS; e++) r[e] = 0;  // zero scales
-            }
-            uint32_t q[8];
-            float dl[2], ml[2];
-            L::levels(r, j, a.kgrid, q, dl, ml);
-            const __half2 bias = __float2half2_rn(L::SIGNED ? 1152.0f : 1024.0f);
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                __half2 h[4];
-                word_halves(L::SIGNED ? q[2 * c] ^ 0x80808080u : q[2 * c], bias, h);
-                word_halves(L::SIGNED ? q[2 * c + 1] ^ 0x80808080u : q[2 * c + 1], bias, h + 2);
-                if constexpr (L::FOLD) {
-                    const __half2 sc = __half2half2(__int2half_rn(L::sub(r, j, c >> 1)));
-                    __half2 p[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) p[e] = __hmul2(h[e], sc);
-                    if constexpr (C::SPLIT) {  // the product's rounding error, exact in float16
-#pragma unroll
-                        for (int e = 0; e < 4; e++) h[e] = __hfma2(h[e], sc, __hneg2(p[e]));
-                        put(st + C::A_BYTES, c, h);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; e++) h[e] = p[e];
-                }
-                put(st, c, h);
-            }
-            scales[((i % C::DR) * 2 + my) * TC_M + row] = L::FOLD ? base_of<L>(r) : dl[0];
-        };
-        // 32 minima of the row (negated) times a power of two, its inverse (and the sums' 2^7) as the scale
-        auto unpack_minima = [&](int i, uint8_t* st) {
-            if constexpr (SUMS > 0) {
-                constexpr int PER = UPB * SUMS;  // minima of a block
-                const int e = (i - main) / (LO ? 2 : 1), part = LO ? (i - main) & 1 : 0, p0 = (e0 + e) * 64 + my * 32;
-                float m[32], top = 0.0f;
-#pragma unroll
-                for (int p = 0; p < 32; p += PER) {
-                    const bool in = mine && p0 + p < a.units * SUMS;
-#pragma unroll
-                    for (int j = 0; j < PER; j++) m[p + j] = 0.0f;
-                    if (in) L::template minima<L::MAXAL>(w + (int64_t)((p0 + p) / PER) * L::BB, m + p);
-                }
-#pragma unroll
-                for (int p = 0; p < 32; p++) top = fmaxf(top, fabsf(m[p]));
-                float up = 1.0f;  // the largest below 2^11
-                if (top > 0.0f && top < INFINITY) up = __uint_as_float((uint32_t)(127 + 10 + 127 - (int)(__float_as_uint(top) >> 23)) << 23);
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    __half2 h[4];
-#pragma unroll
-                    for (int x = 0; x < 4; x++) {
-                        const float v0 = -m[8 * c + 2 * x] * up, v1 = -m[8 * c + 2 * x + 1] * up;
-                        h[x] = __floats2half2_rn(v0, v1);
-                        if (LO && part) {
-                            const float2 f = __half22float2(h[x]);
-                            h[x] = __floats2half2_rn(v0 - f.x, v1 - f.y);
-                        }
-                    }
-                    put(st, c, h);
-                    if constexpr (C::SPLIT) put(st + C::A_BYTES, c, h);
-                }
-                scales[((i % C::DR) * 2 + my) * TC_M + row] = 128.0f / up;
-            }
-        };
         int b = 0, b_ph = 0;  // accumulator to read, its parity
-        auto collect = [&](int i) {
-#pragma unroll
+        bool ok = true;
+        for (int i = 0; i < total && ok; i++) {
             for (int uu = 0; uu < 2; uu++) {
                 if (!ends(i, uu)) continue;
-                if (!mbar_wait(acc_full + 8 * b, b_ph, a.fault)) return false;
+                if (!(ok = mbar_wait(acc_full + 8 * b, b_ph, a.fault))) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                // a shared scale is this thread's own; else the stage was full before its product ended
-                const f32x2 dl = f2_splat(*(volatile float*)&scales[((i % C::DR) * 2 + (GROUP && i < main ? my : uu)) * TC_M + row]);
+                const f32x2 dl = f2_splat(*(volatile float*)&scales[((i % C::DR) * 2 + uu) * TC_M + row]);
                 const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + b * BN + c0;
-                uint32_t v[2][16];
-                tmem_ld16(at, v[0]);
-                tmem_wait_ld(v[0]);
 #pragma unroll
                 for (int bt = 0; bt < NBT; bt++) {
-                    if (bt + 1 < NBT) tmem_ld16(at + 16 * (bt + 1), v[(bt + 1) & 1]);
-                    const uint32_t* r = v[bt & 1];
-#pragma unroll
-                    for (int c = 0; c < 8; c++)
-                        acc[bt * 8 + c] = f2_fma(dl, f2_pack(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1])), acc[bt * 8 + c]);
-                    if (bt + 1 < NBT) tmem_wait_ld(v[(bt + 1) & 1]);
-                    if (bt + 2 == NBT || NBT == 1) {  // the last loads are in registers
+                    uint32_t r[16];
+                    tmem_ld16(at + 16 * bt, r);
+                    tmem_wait_ld(r);
+                    if (bt == NBT - 1) {  // the last loads are in registers
                         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                         __syncwarp();
                         if (lane == 0) mbar_arrive(acc_empty + 8 * b);
                     }
+#pragma unroll
+                    for (int c = 0; c < 8; c++)
+                        acc[bt * 8 + c] = f2_fma(dl, f2_pack(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1])), acc[bt * 8 + c]);
                 }
                 if (++b == NB) {
                     b = 0;
                     b_ph ^= 1;
                 }
             }
-            return true;
-        };
-        bool ok = true;
-        int s = 0, ph = 1;  // stage of the ring and the parity that its last use ended with
-        for (int i = 0; i < total + LAG && ok; i++) {
-            if (i < total) {
-                ok = mbar_wait(empty + 8 * s, ph, a.fault);
-                if (!ok) break;
-                uint8_t* st = ring_p + s * C::STAGE;
-                if (i < main) {
-                    const int r = i / RS;
-                    if (i % RS == 0 && !(ok = mbar_wait(raw_full + 8 * (r % RR), (r / RR) & 1, a.fault))) break;
-                    unpack(i, st);
-                    if (i % RS == RS - 1 || i + 1 == main) {
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(raw_empty + 8 * (r % RR));
-                    }
-                } else {
-                    unpack_minima(i, st);
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(full + 8 * s);
-                if (++s == NS) {
-                    s = 0;
-                    ph ^= 1;
-                }
-            }
-            if (i >= LAG) ok = collect(i - LAG);
         }
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         asm volatile("bar.sync 1, 288;" ::: "memory");
@@ -575,13 +601,12 @@ cudaError_t launch_tc_t(const MmArgs& a, void* ws, const LaunchCtx& ctx) {
     if (e != cudaSuccess) return e;
     auto kernel = tc_kernel<T, BN, LO>;
     if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::BYTES)) != cudaSuccess) return e;
-    if constexpr (C::MOVE) {  // the warpgroups' shares must be there at launch
-        static const int regs = [] {
-            cudaFuncAttributes f;
-            return cudaFuncGetAttributes(&f, tc_kernel<T, BN, LO>) == cudaSuccess ? f.numRegs : 0;
-        }();
-        if (regs * TC_THREADS < 128 * (232 + 232 + 40)) return cudaErrorInvalidConfiguration;
-    }
+    // the warpgroups' shares must be there at launch
+    static const int regs = [] {
+        cudaFuncAttributes f;
+        return cudaFuncGetAttributes(&f, tc_kernel<T, BN, LO>) == cudaSuccess ? f.numRegs : 0;
+    }();
+    if (regs < C::R_LAUNCH) return cudaErrorInvalidConfiguration;
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3((unsigned)((a.n + TC_M - 1) / TC_M), (unsigned)chunks, (unsigned)a.splits);
