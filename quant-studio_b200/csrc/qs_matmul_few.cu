@@ -1,10 +1,11 @@
 // Packed products for few slots per weight matrix (one decoded token, a small batch).
 //
-// The weights' bytes are the work: each is read once, a warp takes whole weight rows, lane l the
-// units l, l + 32, ... of a row, and the levels meet those of up to NT slots in 4-way integer
-// dot products (dp4a). The slots' Q8_0 rows are staged in shared memory once per CTA. A
-// warp's (row, unit) steps form one sequence over its rows, loaded PF steps ahead, so that
-// loads are in flight across row ends too.
+// The weights' bytes are the work: each is read once, and the levels meet those of up to NT slots in
+// 4-way integer dot products (dp4a). A lane takes two units at a time, a pair that shares its bytes
+// where the format has such pairs (both nibbles of the same 32 bytes). LPR lanes share a weight row (all
+// 32, fewer for short rows); lane l takes the pairs l, l + LPR, ... The slots' Q8_0 rows are staged in
+// shared memory once per CTA. A warp's (rows, pair) steps form one sequence, loaded PF steps ahead, so
+// that loads are in flight across row ends too. The rows are dealt out so that the CTAs run in one wave.
 #include <algorithm>
 
 #include "qs_matmul.cuh"
@@ -17,26 +18,29 @@ template <int T, int NT>
 struct FewCfg {
     using L = Lv<T>;
     static constexpr int SUMS = !L::HASMIN ? 0 : L::G16 ? 2 : 1;
-    static constexpr int PF = L::WORDS <= 6 ? 4 : 2;  // steps loaded ahead
+    static constexpr int PF = L::WORDS <= 6 ? 3 : 2;  // steps loaded ahead
+    static constexpr int PPB = L::QK == 256 ? 4 : 1;  // pairs of a superblock
+    // unit h of pair p: neighbours, but Q6_K's low nibbles belong to units j and j + 2
+    __host__ __device__ static int unit(int p, int h) { return T == QS_Q6_K ? 4 * (p >> 1) + (p & 1) + 2 * h : 2 * p + h; }
     // bytes per unit of a slot: levels as two planes of 16 bytes, scale, scale * sums of levels
     static constexpr int UNIT = 32 + 4 + 4 * SUMS;
-    static int bytes(int units) { return NT * units * UNIT; }
+    static int bytes(int units) { return NT * (units + 1) / 2 * 2 * UNIT; }
 };
 
 template <int T, int NT>
-__global__ void __launch_bounds__(512) few_kernel(MmArgs a, int rows_per_warp) {
+__global__ void __launch_bounds__(512) few_kernel(MmArgs a, int rows_per_warp, int lpr) {
     using L = Lv<T>;
     using C = FewCfg<T, NT>;
-    constexpr int UPB = L::QK / 32, SUMS = C::SUMS, PF = C::PF;
+    constexpr int UPB = L::QK / 32, SUMS = C::SUMS, PF = C::PF, PPB = C::PPB;
     extern __shared__ __align__(16) uint8_t smem[];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, units = a.units;
-    uint4* const xq = reinterpret_cast<uint4*>(smem);                         // [slot][half][unit]
-    float* const xd = reinterpret_cast<float*>(smem + NT * units * 32);       // [slot][unit]
-    float* const xs = xd + NT * units;                                        // [half][slot][unit]
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, units = a.units, pairs = (units + 1) >> 1;
+    uint4* const xq = reinterpret_cast<uint4*>(smem);                                // [slot][unit of pair][half][pair]
+    float* const xd = reinterpret_cast<float*>(smem + NT * pairs * 64);              // [slot][unit of pair][pair]
+    float* const xs = xd + NT * pairs * 2;                                           // [half][slot][unit of pair][pair]
     const Chunk ch = find_chunk<NT>(a, blockIdx.y);
     if (ch.group < 0) return;
     const int n0 = (blockIdx.x * (blockDim.x >> 5) + warp) * rows_per_warp, cnt = ch.hi - ch.lo;
-    const int rows = min(rows_per_warp, a.n - n0), iters = (units + 31) >> 5;  // rows may be <= 0
+    const int rows = min(rows_per_warp, a.n - n0);  // may be <= 0
     auto put = [&](int r, int t, float v) {
         const int64_t slot = a.order ? __ldg(a.order + ch.lo + t) : ch.lo + t;
         if (a.part) a.part[slot * a.n + n0 + r] = v;
@@ -46,93 +50,111 @@ __global__ void __launch_bounds__(512) few_kernel(MmArgs a, int rows_per_warp) {
         for (int i = lane; i < rows * cnt; i += 32) put(i / cnt, i % cnt, 0.0f);
         return;
     }
-    // unit lane + 32 i of a row is unit j of its block for every i: UPB divides 32
-    const int j = lane % UPB, full = units >> 5;
-    constexpr int HOP = 32 / UPB * L::BB;  // bytes between a lane's blocks
-    const bool tail = lane < (units & 31);
-    const uint8_t* row_at = a.w + ch.group * a.w_exp + (int64_t)n0 * a.w_row + (lane / UPB) * L::BB;
+    // lpr is a multiple of PPB, so lane l's pairs l + lpr i lie at the same place of their blocks
+    const int l = lane & (lpr - 1), sub = lane / lpr, at_once = 32 / lpr;  // lane of the row, row of the pass
+    const int iters = (pairs + lpr - 1) / lpr, hop = lpr / PPB * (UPB == 1 ? 2 : 1) * L::BB;
+    const int place = l % PPB;
+    const uint8_t* row_at = a.w + ch.group * a.w_exp + (int64_t)(n0 + sub) * a.w_row + (UPB == 1 ? 2 * l : l / PPB) * L::BB;
     const uint8_t* at = row_at;
-    uint32_t raw[PF][L::WORDS];
-    int lr = 0, li = 0;  // row and step of the next load
-    auto load = [&](uint32_t* r) {
-        if (lr < rows && (li < full || tail)) L::template load<L::MAXAL>(at, j, r);
-        at += HOP;
-        if (++li == iters) {
-            li = 0;
-            lr++;
-            at = row_at += a.w_row;
+    uint32_t raw[PF][2][L::WORDS];
+    int lr = sub, lp = l;  // row and pair of the next load
+    auto load = [&](uint32_t (*r)[L::WORDS]) {
+        if (lr < rows && lp < pairs) {
+            if constexpr (UPB == 1) {
+                L::template load<L::MAXAL>(at, 0, r[0]);
+                if (2 * lp + 1 < units) {
+                    L::template load<L::MAXAL>(at + L::BB, 0, r[1]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < L::WORDS; e++) r[1][e] = 0;  // zero scale
+                }
+            } else {
+                L::template load<L::MAXAL>(at, C::unit(place, 0), r[0]);
+                L::template load<L::MAXAL>(at, C::unit(place, 1), r[1]);
+            }
+        }
+        at += hop;
+        lp += lpr;
+        if (lp - l >= iters * lpr) {
+            lp = l;
+            lr += at_once;
+            at = row_at += a.w_row * at_once;
         }
     };
 #pragma unroll
     for (int p = 0; p < PF; p++) load(raw[p]);
 
-    for (int i = tid; i < NT * 2 * units; i += blockDim.x) {
-        const int h = i & 1, k = i >> 1, t = k / units, u = k - t * units;
+    for (int i = tid; i < NT * 2 * pairs * 2; i += blockDim.x) {
+        const int h = i & 1, k = i >> 1, t = k / (2 * pairs), u = k - t * 2 * pairs;
+        const int p = T == QS_Q6_K ? 2 * (u >> 2) + (u & 1) : u >> 1, e = T == QS_Q6_K ? (u >> 1) & 1 : u & 1;
         uint4 q = make_uint4(0, 0, 0, 0);
         float d = 0.0f;
-        if (t < cnt) {
+        int s = 0, other = 0;
+        if (t < cnt && u < units) {
             const int slot = a.order ? __ldg(a.order + ch.lo + t) : ch.lo + t;
             const uint8_t* b = a.x + (slot / a.x_div) * a.x_row + (int64_t)u * 34;
             q = ld_16b(b + 2 + 16 * h);
             d = h2f(ld_u16<1>(b));
-        }
-        xq[(t * 2 + h) * units + u] = q;
-        if (h == 0) xd[t * units + u] = d;
-        if constexpr (SUMS == 2) xs[(h * NT + t) * units + u] = d * (float)sum16(q);
-        if constexpr (SUMS == 1) {
+            if constexpr (SUMS > 0) s = sum16(q);
             // the other half's sum, computed again rather than exchanged: lanes may have left the loop
-            const int o = t < cnt ? sum16(ld_16b(a.x + ((a.order ? __ldg(a.order + ch.lo + t) : ch.lo + t) / a.x_div) * a.x_row + (int64_t)u * 34 + 2 + 16 * (h ^ 1))) : 0;
-            if (h == 0) xs[t * units + u] = d * (float)(sum16(q) + o);
+            if constexpr (SUMS == 1) other = sum16(ld_16b(b + 2 + 16 * (h ^ 1)));
         }
+        xq[((t * 2 + e) * 2 + h) * pairs + p] = q;
+        if (h == 0) xd[(t * 2 + e) * pairs + p] = d;
+        if constexpr (SUMS == 2) xs[((h * NT + t) * 2 + e) * pairs + p] = d * (float)s;
+        if constexpr (SUMS == 1)
+            if (h == 0) xs[(t * 2 + e) * pairs + p] = d * (float)(s + other);
     }
     __syncthreads();
 
     float acc[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) acc[t] = 0.0f;
-    int cr = 0, ci = 0;  // row and step at hand
-    const int steps = rows > 0 ? rows * iters : 0;
+    int cr = 0, cp = l;  // first row of the pass, pair at hand
+    const int passes = rows > 0 ? (rows + at_once - 1) / at_once : 0, steps = passes * iters;
     for (int s = 0; s < steps; s += PF) {
 #pragma unroll
         for (int p = 0; p < PF; p++) {
             if (s + p >= steps) break;
-            uint32_t q[8];
-            float dl[2], ml[2];
-            const bool live = ci < full || tail;
-            const int cu = ci * 32 + lane;
-            if (live) L::levels(raw[p], j, a.kgrid, q, dl, ml);
-            load(raw[p]);
+            const bool live = cp < pairs && cr + sub < rows;
             if (live) {
 #pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    const uint4 xa = xq[(2 * t) * units + cu], xb = xq[(2 * t + 1) * units + cu];
-                    const float d = xd[t * units + cu];
-                    int s0 = __dp4a((int)q[0], (int)xa.x, 0), s1 = 0;
-                    s0 = __dp4a((int)q[1], (int)xa.y, s0);
-                    s0 = __dp4a((int)q[2], (int)xa.z, s0);
-                    s0 = __dp4a((int)q[3], (int)xa.w, s0);
-                    if (!L::G16) s1 = s0;
-                    s1 = __dp4a((int)q[4], (int)xb.x, s1);
-                    s1 = __dp4a((int)q[5], (int)xb.y, s1);
-                    s1 = __dp4a((int)q[6], (int)xb.z, s1);
-                    s1 = __dp4a((int)q[7], (int)xb.w, s1);
-                    if (L::G16) acc[t] = __fmaf_rn(dl[0] * d, (float)s0, acc[t]);
-                    acc[t] = __fmaf_rn(dl[1] * d, (float)s1, acc[t]);
-                    if constexpr (SUMS >= 1) acc[t] = __fmaf_rn(-ml[0], xs[t * units + cu], acc[t]);
-                    if constexpr (SUMS == 2) acc[t] = __fmaf_rn(-ml[1], xs[(NT + t) * units + cu], acc[t]);
+                for (int e = 0; e < 2; e++) {
+                    uint32_t q[8];
+                    float dl[2], ml[2];
+                    L::levels(raw[p][e], UPB == 1 ? 0 : C::unit(place, e), a.kgrid, q, dl, ml);
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        const uint4 xa = xq[((t * 2 + e) * 2) * pairs + cp], xb = xq[((t * 2 + e) * 2 + 1) * pairs + cp];
+                        const float d = xd[(t * 2 + e) * pairs + cp];
+                        int s0 = __dp4a((int)q[0], (int)xa.x, 0), s1 = 0;
+                        s0 = __dp4a((int)q[1], (int)xa.y, s0);
+                        s0 = __dp4a((int)q[2], (int)xa.z, s0);
+                        s0 = __dp4a((int)q[3], (int)xa.w, s0);
+                        if (!L::G16) s1 = s0;
+                        s1 = __dp4a((int)q[4], (int)xb.x, s1);
+                        s1 = __dp4a((int)q[5], (int)xb.y, s1);
+                        s1 = __dp4a((int)q[6], (int)xb.z, s1);
+                        s1 = __dp4a((int)q[7], (int)xb.w, s1);
+                        if (L::G16) acc[t] = __fmaf_rn(dl[0] * d, (float)s0, acc[t]);
+                        acc[t] = __fmaf_rn(dl[1] * d, (float)s1, acc[t]);
+                        if constexpr (SUMS >= 1) acc[t] = __fmaf_rn(-ml[0], xs[(t * 2 + e) * pairs + cp], acc[t]);
+                        if constexpr (SUMS == 2) acc[t] = __fmaf_rn(-ml[1], xs[((NT + t) * 2 + e) * pairs + cp], acc[t]);
+                    }
                 }
             }
-            if (++ci == iters) {  // the row's end
+            load(raw[p]);
+            cp += lpr;
+            if (cp - l >= iters * lpr) {  // the rows' end
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
                     float v = acc[t];
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-                    if (lane == 0 && t < cnt) put(cr, t, v);
+                    for (int o = lpr >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+                    if (l == 0 && t < cnt && cr + sub < rows) put(cr + sub, t, v);
                     acc[t] = 0.0f;
                 }
-                ci = 0;
-                cr++;
+                cp = l;
+                cr += at_once;
             }
         }
     }
@@ -181,8 +203,13 @@ cudaError_t launch_few_t(const MmArgs& a, const LaunchCtx& ctx) {
     const int64_t chunks = max_chunks(a, NT);
     const int bytes = FewCfg<T, NT>::bytes(a.units);
     if (chunks > 65535 || bytes > FEW_SMEM_MAX) return cudaErrorInvalidConfiguration;
-    cudaError_t e = cudaFuncSetAttribute(few_kernel<T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_SMEM_MAX);
-    if (e != cudaSuccess) return e;
+    if (bytes > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(few_kernel<T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_SMEM_MAX);
+        if (e != cudaSuccess) return e;
+    }
+    const int pairs = (a.units + 1) / 2;
+    int lpr = 32;  // lanes of a row: no more than it has pairs (at least a superblock's 4)
+    while (lpr > 4 && lpr / 2 >= pairs) lpr /= 2;
     // Activations beyond a quarter of an SM's shared memory: fewer CTAs fit, with 16 warps each.
     const int warps = bytes <= 48 * 1024 ? 8 : 16;
     // Rows per warp such that the CTAs of all chunks fit the SMs at once: one wave of equal shares.
@@ -192,9 +219,11 @@ cudaError_t launch_few_t(const MmArgs& a, const LaunchCtx& ctx) {
     }();
     const int per_sm = std::max(1, std::min({65536 / (regs * 32 * warps), 64 / warps, 227 * 1024 / (bytes + 1024)}));
     const int64_t ctas = std::max<int64_t>(1, (int64_t)per_sm * ctx.num_sms / chunks);
-    const int64_t rpw = std::min<int64_t>(16, (a.n + ctas * warps - 1) / (ctas * warps));
+    const int at_once = 32 / lpr;
+    int64_t rpw = std::min<int64_t>(16, (a.n + ctas * warps - 1) / (ctas * warps));
+    rpw = (rpw + at_once - 1) / at_once * at_once;
     const dim3 grid((unsigned)((a.n + warps * rpw - 1) / (warps * rpw)), (unsigned)chunks);
-    few_kernel<T, NT><<<grid, 32 * warps, bytes, ctx.stream>>>(a, (int)rpw);
+    few_kernel<T, NT><<<grid, 32 * warps, bytes, ctx.stream>>>(a, (int)rpw, lpr);
     return cudaGetLastError();
 }
 
