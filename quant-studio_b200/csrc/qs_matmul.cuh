@@ -13,6 +13,8 @@
 // each warp finds its own from the offsets.
 #pragma once
 
+#include <atomic>
+
 #include "qs_levels.cuh"
 
 namespace qs {
@@ -117,6 +119,15 @@ __device__ __forceinline__ void store_row4(void* out, int64_t at, int type, floa
         for (int c = 0; c < 4; c++)
             if (n0 + 4 * lane + c < n) store_val(out, at + 4 * lane + c, type, e[c]);
     }
+}
+
+// Dynamic shared memory beyond 48 KB for a kernel, asked for once per device (`asked`: bits of the
+// devices, one word per kernel).
+inline cudaError_t allow_smem(const void* kernel, int bytes, int device, std::atomic<unsigned long long>& asked) {
+    if (device >= 0 && device < 64 && (asked.load(std::memory_order_relaxed) >> device) & 1ull) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && device >= 0 && device < 64) asked.fetch_or(1ull << device, std::memory_order_relaxed);
+    return e;
 }
 
 // 16 bytes at any address

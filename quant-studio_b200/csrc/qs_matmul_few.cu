@@ -203,8 +203,9 @@ cudaError_t launch_few_t(const MmArgs& a, const LaunchCtx& ctx) {
     const int64_t chunks = max_chunks(a, NT);
     const int bytes = FewCfg<T, NT>::bytes(a.units);
     if (chunks > 65535 || bytes > FEW_SMEM_MAX) return cudaErrorInvalidConfiguration;
+    static std::atomic<unsigned long long> asked{0};
     if (bytes > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(few_kernel<T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_SMEM_MAX);
+        const cudaError_t e = allow_smem((const void*)few_kernel<T, NT>, FEW_SMEM_MAX, ctx.device, asked);
         if (e != cudaSuccess) return e;
     }
     const int pairs = (a.units + 1) / 2;

@@ -300,7 +300,8 @@ cudaError_t launch_mid_t(const MmArgs& a, const int8_t* xq, const float* xd, int
     using C = MidCfg<T, NT>;
     const int64_t chunks = max_chunks(a, C::BN);
     if (chunks > 65535) return cudaErrorInvalidConfiguration;
-    cudaError_t e = cudaFuncSetAttribute(mid_kernel<T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::BYTES);
+    static std::atomic<unsigned long long> asked{0};
+    const cudaError_t e = allow_smem((const void*)mid_kernel<T, NT>, C::BYTES, ctx.device, asked);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));

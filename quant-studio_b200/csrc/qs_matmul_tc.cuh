@@ -600,7 +600,8 @@ cudaError_t launch_tc_t(const MmArgs& a, void* ws, const LaunchCtx& ctx) {
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     auto kernel = tc_kernel<T, BN, LO>;
-    if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::BYTES)) != cudaSuccess) return e;
+    static std::atomic<unsigned long long> asked{0};
+    if ((e = allow_smem((const void*)kernel, C::BYTES, ctx.device, asked)) != cudaSuccess) return e;
     // the warpgroups' shares must be there at launch
     static const int regs = [] {
         cudaFuncAttributes f;
