@@ -2,7 +2,7 @@
 // float32 sums in tensor memory).
 //
 // Weights: integer levels are exact in float16, and so is level * sub-scale of the formats with one
-// scale per superblock (at most 2048): for those D sums W' x over a superblock of 256 values, and
+// scale per superblock (at most 2048): for those D sums W' x over a superblock of 256 values (LO: half of it), and
 //   acc[n, t] += d[n, superblock] * D[n, t]
 // in float32 registers. Formats with a scale per 32 values are scaled and added every 32. Q6_K's
 // level * sub-scale (up to 4096) is float16 hi + lo, exact together.
@@ -55,7 +55,9 @@ struct TcCfg {
     using L = Lv<T>;
     static constexpr bool SPLIT = LO && T == QS_Q6_K;
     static constexpr int SUMS = !L::HASMIN ? 0 : L::G16 ? 2 : 1;  // minima per unit
-    static constexpr int GROUP = L::FOLD ? 4 : 0;  // stages that share an accumulator; 0: one per unit
+    // stages that share an accumulator (0: one per unit). The matrix unit adds with truncation: over 256
+    // values that cost 4.6e-7 of a result, half of it over 128
+    static constexpr int GROUP = !L::FOLD ? 0 : LO ? 2 : 4;
     static constexpr int A_BYTES = TC_M * 128, A_ALL = A_BYTES * (SPLIT ? 2 : 1), B_BYTES = BN * 128, X_BYTES = B_BYTES * (LO ? 2 : 1);
     static constexpr int STAGE = A_ALL + X_BYTES;
     // packed bytes: steps of RS stages (a superblock, or 4 blocks of 32), the bytes of a row's step and
