@@ -4,7 +4,8 @@ packed weights with Q8_0 activations.
 The next step after quantizing: a layer whose weights stay packed. `rms_norm_q8` makes the
 8-bit activations, `route` and `expert_plan` choose and group the experts, `matmul` and
 `matmul_experts` multiply. Everything runs on the current stream of the operands' device;
-outputs and workspaces are new tensors, so calls may be captured into a CUDA graph.
+outputs and workspaces are new tensors, so calls may be captured into a CUDA graph (after a
+first call on the device outside of a capture, which prepares it).
 """
 
 from __future__ import annotations
@@ -199,8 +200,9 @@ def _experts_workspace(*sizes: int) -> int:
 
 def matmul(blocks: torch.Tensor, ggml_type: int, x_q8: torch.Tensor, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """(rows, n) products of packed weights (n, row bytes) with Q8_0 activations (rows, k / 32 * 34):
-    the decoded activations times the decoded weights transposed. Level products are exact
-    integers, scales and sums float32, rounded once to out_dtype. Row strides may exceed the rows;
+    the decoded activations times the decoded weights transposed. Levels are multiplied exactly, scales
+    and sums are float32, rounded once to out_dtype (bfloat16 results of more than 64 rows: from
+    activations rounded to 11 bits, 1/8 of the result's own rounding). Row strides may exceed the rows;
     weight rows must start on multiples of 16 bytes for Q4_K / Q5_K, 8 for Q5_1 / IQ4_XS, 4 for
     Q4_1 / Q2_K, 2 for the others.
     """
