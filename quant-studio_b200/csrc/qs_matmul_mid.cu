@@ -30,6 +30,12 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)_
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
+__device__ __forceinline__ void cp16_or_zero(uint32_t dst, const void* src, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp4_or_zero(uint32_t dst, const void* src, bool live) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0) : "memory");
+}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -134,17 +140,19 @@ __global__ void __launch_bounds__(MID_THREADS, 2) mid_kernel(MmArgs a, const int
     for (int us = u0; us < u1; us += SL) {
         const int nu = min(SL, u1 - us);
         __syncthreads();  // the last slice is used up
+        // all copies under way at once; rows without a slot are filled with zeros
+#pragma unroll 4
         for (int i = tid; i < BN * nu * 2; i += MID_THREADS) {
             const int t = i / (nu * 2), c = i - t * nu * 2, row = s_row[t];
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (row >= 0) v = __ldg(reinterpret_cast<const uint4*>(xq + (int64_t)row * units_pad * 32 + (int64_t)us * 32) + c);
-            *reinterpret_cast<uint4*>(smem + t * C::PITCH + c * 16) = v;
+            cp16_or_zero(x_a + t * C::PITCH + c * 16, xq + ((int64_t)max(row, 0) * units_pad + us) * 32 + c * 16, row >= 0);
         }
+#pragma unroll 4
         for (int i = tid; i < (1 + SUMS) * BN * nu; i += MID_THREADS) {
             const int u = i % nu, pt = i / nu, t = pt % BN, row = s_row[t];
-            reinterpret_cast<float*>(smem + C::OFF_XD)[(pt / BN * SL + u) * BN + t] =
-                row >= 0 ? __ldg(xd + pt / BN * x_plane + (int64_t)row * units_pad + us + u) : 0.0f;
+            cp4_or_zero(x_a + C::OFF_XD + ((pt / BN * SL + u) * BN + t) * 4, xd + pt / BN * x_plane + (int64_t)max(row, 0) * units_pad + us + u, row >= 0);
         }
+        cp_commit();
+        cp_wait<0>();
         __syncthreads();
         for (int su = 0; su < nu; su += RU, k++) {
             cp_wait<RR - 1>();

@@ -179,8 +179,13 @@ __global__ void __launch_bounds__(256) xpack_kernel(MmArgs a, uint8_t* out, floa
     const int slot = live ? (a.order ? __ldg(a.order + ch.lo + t) : ch.lo + t) : 0;
     const uint8_t* row = a.x + (int64_t)(slot / a.x_div) * a.x_row;
     uint32_t top = 0;  // largest |scale| as float16 bits; above 0x7BFF: inf or NaN
-    if (live)
-        for (int u = lane; u < a.units; u += 32) top = max(top, ld_u16<1>(row + (int64_t)u * 34) & 0x7FFFu);
+    for (int u0 = lane; u0 < a.units; u0 += 32 * 8) {  // 8 loads under way
+        uint32_t d[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) d[j] = live && u0 + 32 * j < a.units ? ld_u16<1>(row + (int64_t)(u0 + 32 * j) * 34) & 0x7FFFu : 0u;
+#pragma unroll
+        for (int j = 0; j < 8; j++) top = max(top, d[j]);
+    }
     top = __reduce_max_sync(0xffffffffu, top);
     // 2^(7 - exponent): scales below 2^8, values at most 2^15
     float up = 1.0f;
@@ -195,13 +200,22 @@ __global__ void __launch_bounds__(256) xpack_kernel(MmArgs a, uint8_t* out, floa
         if constexpr (LO) *reinterpret_cast<__half*>(at + B_BYTES) = __float2half_rn(v - __half2float(h));
     };
     const int last = max(2 * stages, SUMS ? blocks * 64 / SUMS : 0);
-    for (int u = lane; u < last; u += 32) {
-        uint32_t q[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        float d = 0.0f;
+    uint32_t next[9];  // the next unit's levels and scale
+    auto load = [&](int u) {
+#pragma unroll
+        for (int e = 0; e < 9; e++) next[e] = 0;
         if (live && u < a.units) {
-            ld_words<8, 1>(row + (int64_t)u * 34 + 2, q);
-            d = h2f(ld_u16<1>(row + (int64_t)u * 34)) * up;
+            ld_words<8, 1>(row + (int64_t)u * 34 + 2, next);
+            next[8] = ld_u16<1>(row + (int64_t)u * 34);
         }
+    };
+    load(lane);
+    for (int u = lane; u < last; u += 32) {
+        uint32_t q[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) q[e] = next[e];
+        const float d = h2f(next[8]) * up;
+        load(u + 32);
         if (u < 2 * stages) {
             uint8_t* st = o + (int64_t)(u >> 1) * X_BYTES;
 #pragma unroll
