@@ -6,6 +6,11 @@
 // 32, fewer for short rows); lane l takes the pairs l, l + LPR, ... The slots' Q8_0 rows are staged in
 // shared memory once per CTA. A warp's (rows, pair) steps form one sequence, loaded PF steps ahead, so
 // that loads are in flight across row ends too. The rows are dealt out so that the CTAs run in one wave.
+//
+// Measured for one slot: Q4_K 14336 x 4096 (33 MB) 14.5 us, 2.3 TB/s; Q4_K / Q4_0 / Q8_0 4096 x 4096 6.2 / 6.5 /
+// 6.8 us, of which about 3 us are launch, staging and first loads. Bound: 280 instructions per pair step of a
+// warp at 58 % of the issue slots. With more than a few slots the dot products (half rate on this GPU) take
+// over: 4 slots 12 us, and from 5 on the tensor cores' kernel is faster.
 #include <algorithm>
 
 #include "qs_matmul.cuh"

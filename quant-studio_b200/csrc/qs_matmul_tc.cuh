@@ -33,6 +33,12 @@
 // the unpacking can not lap: stage i waits for the products of stage i - NS, these for the release of
 // their accumulator, so the sums are at most NS + 7 stages behind. Every wait is bounded: one that runs
 // out records bit 0 of the fault word and its role leaves.
+// Measured: 2048 slots of Q4_K 14336 x 4096 to bfloat16 338 us with xpack_kernel (11 us), 711 TFLOP/s, 43 % of the
+// measured bf16 rate; 4096 slots of 4096 x 4096 205 us; 1024 to float32 (LO) 108 us. Without any unpacking or
+// copying the same loop takes 247 us: a stage moves 105 KB through shared memory (operands read by
+// the matrix unit, unpacked and copied data), 820 cycles at 128 bytes each, against 512 of products. Tiles of
+// 256 columns halve what a column costs in unpacking; two CTAs that share the columns' operand would be the
+// next step.
 // The order of the 32 values within a unit does not matter to the sum; both operands use the one
 // that unpacks cheapest (word_halves).
 #pragma once
