@@ -56,31 +56,36 @@ __device__ __forceinline__ Chunk find_chunk(const MmArgs& a, int c) {
     }
     const int lane = threadIdx.x & 31;
     int run = 0;
-    for (int base = 0; base <= a.n_exp; base += 32) {
-        const int e = base + lane;
-        int lo = 0, hi = 0;
-        if (e <= a.n_exp) {
-            lo = __ldg(a.offsets + e);
-            hi = e < a.n_exp ? __ldg(a.offsets + e + 1) : a.slots;
-        }
-        const int cnt = (hi - lo + C - 1) / C;
-        int inc = cnt;
+    constexpr int W = 4;  // windows of 32 groups whose offsets are on their way together
+    for (int base = 0; base <= a.n_exp; base += 32 * W) {
+        int lo[W], hi[W];
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += u;
+        for (int j = 0; j < W; j++) {
+            const int e = base + 32 * j + lane;
+            lo[j] = e <= a.n_exp ? __ldg(a.offsets + e) : 0;
+            hi[j] = e < a.n_exp ? __ldg(a.offsets + e + 1) : e == a.n_exp ? a.slots : 0;
         }
-        const int first = run + inc - cnt;
-        const unsigned hit = __ballot_sync(0xffffffffu, c >= first && c < first + cnt);
-        if (hit) {
-            const int l = __ffs(hit) - 1;
-            const int g_first = __shfl_sync(0xffffffffu, first, l);
-            r.group = base + l;
-            r.lo = __shfl_sync(0xffffffffu, lo, l) + (c - g_first) * C;
-            r.hi = min(r.lo + C, __shfl_sync(0xffffffffu, hi, l));
-            return r;
+#pragma unroll
+        for (int j = 0; j < W; j++) {
+            const int cnt = (hi[j] - lo[j] + C - 1) / C;
+            int inc = cnt;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += u;
+            }
+            const int first = run + inc - cnt;
+            const unsigned hit = __ballot_sync(0xffffffffu, c >= first && c < first + cnt);
+            if (hit) {
+                const int l = __ffs(hit) - 1;
+                const int g_first = __shfl_sync(0xffffffffu, first, l);
+                r.group = base + 32 * j + l;
+                r.lo = __shfl_sync(0xffffffffu, lo[j], l) + (c - g_first) * C;
+                r.hi = min(r.lo + C, __shfl_sync(0xffffffffu, hi[j], l));
+                return r;
+            }
+            run += __shfl_sync(0xffffffffu, inc, 31);
         }
-        run += __shfl_sync(0xffffffffu, inc, 31);
     }
     return r;
 }

@@ -251,12 +251,10 @@ def experts_want(x, w, qtype, ids, weights, per_slot, out="float32"):
     t, k = ids.shape
     n = w.shape[1]
     y, b = np.zeros((t, k, n)), np.zeros((t, k, n))
-    for i in range(t):
-        for j in range(k):
-            if 0 <= ids[i, j] < w.shape[0]:
-                r = i * k + j if per_slot else i
-                yy, bb = ref.product(x[r:r + 1], w[ids[i, j]], qtype, out)
-                y[i, j], b[i, j] = yy[0], bb[0]
+    for e in range(w.shape[0]):
+        i, j = np.nonzero(ids == e)
+        if len(i):
+            y[i, j], b[i, j] = ref.product(x[i * k + j if per_slot else i], w[e], qtype, out)
     if weights is None:
         return y, b
     wt = weights[..., None].astype(np.float64)
@@ -281,6 +279,41 @@ def test_experts(qtype, tokens, top, e, per_slot, weighted):
     p = ops.expert_plan(cuda(ids), e)
     got = ops.matmul_experts(cuda(w), int(ref.GTYPE[qtype]), cuda(x), p, weights=None if wt is None else cuda(wt))
     check_product(got, *experts_want(x, w, qtype, ids, wt, per_slot or top == 1))
+
+
+@pytest.mark.parametrize("tokens,top,e", [(3000, 4, 300), (800, 4, 20), (700, 2, 9), (2100, 1, 1000)])
+@pytest.mark.parametrize("dtype,weighted", [("float32", False), ("bfloat16", True)])
+def test_experts_many(tokens, top, e, dtype, weighted):
+    """Many experts of very different popularity, ids that name none, several tiles per expert."""
+    rng = np.random.default_rng(e)
+    n, k = 70, 512
+    w = ref.random_blocks("q5_k", (e, n), k, rng)
+    x = ref.random_blocks("q8_0", (tokens,), k, rng)
+    ids = np.minimum((e * rng.random((tokens, top)) ** 2).astype(np.int32), e - 1)
+    ids[rng.random((tokens, top)) < 0.05] = -1
+    wt = rng.random((tokens, top)).astype(np.float32) if weighted else None
+    got = ops.matmul_experts(cuda(w), 13, cuda(x), ops.expert_plan(cuda(ids), e), weights=None if wt is None else cuda(wt), out_dtype=DT[dtype])
+    check_product(got, *experts_want(x, w, "q5_k", ids, wt, False, dtype))
+
+
+def test_products_on_two_streams():
+    """Products of every kernel under way at the same time give the bits that they give alone."""
+    rng = np.random.default_rng(31)
+    w = cuda(ref.random_blocks("q4_k", (1024,), 2048, rng))
+    xs = [cuda(ref.random_blocks("q8_0", (r,), 2048, rng)) for r in (1, 4, 7, 60, 100, 600)]
+    want = [ops.matmul(w, 12, x, out_dtype=d) for x in xs for d in (torch.float32, torch.bfloat16)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for _ in range(4):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                order = xs[i:] + xs[:i]
+                got.append([ops.matmul(w, 12, x, out_dtype=d) for x in order for d in (torch.float32, torch.bfloat16)])
+    torch.cuda.synchronize()
+    for n, g in enumerate(got):
+        i = 2 * (n % 3)
+        assert all(torch.equal(p, q) for p, q in zip(g, want[i:] + want[:i]))
 
 
 def test_experts_all_empty_and_one_crowded():
