@@ -37,8 +37,9 @@
 // measured bf16 rate; 4096 slots of 4096 x 4096 205 us; 1024 to float32 (LO) 108 us. Without any unpacking or
 // copying the same loop takes 247 us: a stage moves 105 KB through shared memory (operands read by
 // the matrix unit, unpacked and copied data), 820 cycles at 128 bytes each, against 512 of products. Tiles of
-// 256 columns halve what a column costs in unpacking; two CTAs that share the columns' operand would be the
-// next step.
+// 256 columns halve what a column costs in unpacking. Pairs of CTAs that hold half of the columns' operand
+// each (cta_group::2) move 74 KB per stage, but took 452 us: every stage then waits for arrivals from
+// the other CTA.
 // The order of the 32 values within a unit does not matter to the sum; both operands use the one
 // that unpacks cheapest (word_halves).
 #pragma once

@@ -200,6 +200,32 @@ def test_matmul_sizes(qtype, rows, n, k, dtype):
     check_product(got, *ref.product(x, w, qtype, dtype))
 
 
+@pytest.mark.parametrize("qtype", ref.TYPES)
+@pytest.mark.parametrize("rows", [130, 257])
+def test_matmul_wide_tiles(qtype, rows):
+    """Tiles of 256 slots that fill the GPU without splitting rows, an odd number of them, a ragged last one."""
+    rng = np.random.default_rng(rows)
+    k, n = (5 * 32 if ref.qk(qtype) == 32 else 512), 149 * 128 - 27 if rows < 256 else 75 * 128 - 27
+    w = ref.random_blocks(qtype, (n,), k, rng)
+    x = ref.random_blocks("q8_0", (rows,), k, rng)
+    got = ops.matmul(cuda(w), int(ref.GTYPE[qtype]), cuda(x), out_dtype=torch.bfloat16)
+    check_product(got, *ref.product(x, w, qtype, "bfloat16"))
+
+
+@pytest.mark.parametrize("qtype", ["q4_k", "q5_0"])
+@pytest.mark.parametrize("weighted", [False, True])
+def test_experts_wide_tiles(qtype, weighted):
+    rng = np.random.default_rng(41)
+    e, tokens, n, k = 8, 1300, 19 * 128, 256
+    w = ref.random_blocks(qtype, (e, n), k, rng)
+    x = ref.random_blocks("q8_0", (tokens,), k, rng)
+    ids = rng.integers(-1, e, (tokens, 1)).astype(np.int32)
+    ids[:700] = 5
+    wt = rng.random((tokens, 1)).astype(np.float32) if weighted else None
+    got = ops.matmul_experts(cuda(w), int(ref.GTYPE[qtype]), cuda(x), ops.expert_plan(cuda(ids), e), weights=None if wt is None else cuda(wt), out_dtype=torch.bfloat16)
+    check_product(got, *experts_want(x, w, qtype, ids, wt, True, "bfloat16"))
+
+
 @pytest.mark.parametrize("qtype", ["q8_0", "q4_k", "q6_k"])
 @pytest.mark.parametrize("rows", [2, 40])
 def test_matmul_strides(qtype, rows):
