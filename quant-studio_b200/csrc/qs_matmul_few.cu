@@ -5,11 +5,11 @@
 // where the format has such pairs (both nibbles of the same 32 bytes). LPR lanes share a weight row (all
 // 32, fewer for short rows); lane l takes the pairs l, l + LPR, ... The slots' Q8_0 rows are staged in
 // shared memory once per CTA. A warp's (rows, pair) steps form one sequence, loaded PF steps ahead, so
-// that loads are in flight across row ends too. The rows are dealt out so that the CTAs run in one wave.
+// that loads are in flight across row ends too. The CTAs run in one wave and take rows in turn.
 //
-// Measured for one slot: Q4_K 14336 x 4096 (33 MB) 14.5 us, 2.3 TB/s; Q4_K / Q4_0 / Q8_0 4096 x 4096 6.2 / 6.5 /
-// 6.8 us, of which about 3 us are launch, staging and first loads. Bound: 280 instructions per pair step of a
-// warp at 58 % of the issue slots. With more than a few slots the dot products (half rate on this GPU) take
+// Measured for one slot: Q4_K 14336 x 4096 (33 MB) 13.0 us, 2.6 TB/s (15.0 us with one run of rows per warp, whose
+// last warps idle); Q4_K / Q4_0 / Q8_0 4096 x 4096 6.5 / 6.7 / 6.8 us, of which about 3 us are launch, staging and first loads. Bound: 280 instructions per pair step of a
+// warp. With more than a few slots the dot products (half rate on this GPU) take
 // over: 4 slots 12 us, and from 5 on the tensor cores' kernel is faster.
 #include <algorithm>
 
@@ -33,7 +33,7 @@ struct FewCfg {
 };
 
 template <int T, int NT>
-__global__ void __launch_bounds__(512) few_kernel(MmArgs a, int rows_per_warp, int lpr) {
+__global__ void __launch_bounds__(512) few_kernel(MmArgs a, int lpr) {
     using L = Lv<T>;
     using C = FewCfg<T, NT>;
     constexpr int UPB = L::QK / 32, SUMS = C::SUMS, PF = C::PF, PPB = C::PPB;
@@ -44,27 +44,30 @@ __global__ void __launch_bounds__(512) few_kernel(MmArgs a, int rows_per_warp, i
     float* const xs = xd + NT * pairs * 2;                                           // [half][slot][unit of pair][pair]
     const Chunk ch = find_chunk<NT>(a, blockIdx.y);
     if (ch.group < 0) return;
-    const int n0 = (blockIdx.x * (blockDim.x >> 5) + warp) * rows_per_warp, cnt = ch.hi - ch.lo;
-    const int rows = min(rows_per_warp, a.n - n0);  // may be <= 0
-    auto put = [&](int r, int t, float v) {
+    const int cnt = ch.hi - ch.lo;
+    auto put = [&](int64_t r, int t, float v) {
         const int64_t slot = a.order ? __ldg(a.order + ch.lo + t) : ch.lo + t;
-        if (a.part) a.part[slot * a.n + n0 + r] = v;
-        else store_val(a.out, slot * a.out_stride + n0 + r, a.out_type, v);
+        if (a.part) a.part[slot * a.n + r] = v;
+        else store_val(a.out, slot * a.out_stride + r, a.out_type, v);
     };
     if (a.order && ch.group == a.n_exp) {  // slots without an expert
-        for (int i = lane; i < rows * cnt; i += 32) put(i / cnt, i % cnt, 0.0f);
+        for (int64_t r = (int64_t)blockIdx.x * blockDim.x + tid; r < a.n; r += (int64_t)gridDim.x * blockDim.x)
+            for (int t = 0; t < cnt; t++) put(r, t, 0.0f);
         return;
     }
     // lpr is a multiple of PPB, so lane l's pairs l + lpr i lie at the same place of their blocks
     const int l = lane & (lpr - 1), sub = lane / lpr, at_once = 32 / lpr;  // lane of the row, row of the pass
     const int iters = (pairs + lpr - 1) / lpr, hop = lpr / PPB * (UPB == 1 ? 2 : 1) * L::BB;
     const int place = l % PPB;
-    const uint8_t* row_at = a.w + ch.group * a.w_exp + (int64_t)(n0 + sub) * a.w_row + (UPB == 1 ? 2 * l : l / PPB) * L::BB;
+    // passes over at_once rows, dealt to the warps of all CTAs in turn
+    const int64_t first = ((int64_t)blockIdx.x * (blockDim.x >> 5) + warp) * at_once, turn = (int64_t)gridDim.x * (blockDim.x >> 5) * at_once;
+    const uint8_t* row_at = a.w + ch.group * a.w_exp + (first + sub) * a.w_row + (UPB == 1 ? 2 * l : l / PPB) * L::BB;
     const uint8_t* at = row_at;
     uint32_t raw[PF][2][L::WORDS];
-    int lr = sub, lp = l;  // row and pair of the next load
+    int64_t lr = first + sub;  // row and pair of the next load
+    int lp = l;
     auto load = [&](uint32_t (*r)[L::WORDS]) {
-        if (lr < rows && lp < pairs) {
+        if (lr < a.n && lp < pairs) {
             if constexpr (UPB == 1) {
                 L::template load<L::MAXAL>(at, 0, r[0]);
                 if (2 * lp + 1 < units) {
@@ -82,8 +85,8 @@ __global__ void __launch_bounds__(512) few_kernel(MmArgs a, int rows_per_warp, i
         lp += lpr;
         if (lp - l >= iters * lpr) {
             lp = l;
-            lr += at_once;
-            at = row_at += a.w_row * at_once;
+            lr += turn;
+            at = row_at += a.w_row * turn;
         }
     };
 #pragma unroll
@@ -115,13 +118,14 @@ __global__ void __launch_bounds__(512) few_kernel(MmArgs a, int rows_per_warp, i
     float acc[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) acc[t] = 0.0f;
-    int cr = 0, cp = l;  // first row of the pass, pair at hand
-    const int passes = rows > 0 ? (rows + at_once - 1) / at_once : 0, steps = passes * iters;
-    for (int s = 0; s < steps; s += PF) {
+    int64_t cr = first + sub;  // row and pair at hand
+    int cp = l;
+    const int64_t passes = first < a.n ? (a.n - first + turn - 1) / turn : 0, steps = passes * iters;
+    for (int64_t s = 0; s < steps; s += PF) {
 #pragma unroll
         for (int p = 0; p < PF; p++) {
             if (s + p >= steps) break;
-            const bool live = cp < pairs && cr + sub < rows;
+            const bool live = cp < pairs && cr < a.n;
             if (live) {
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
@@ -155,11 +159,11 @@ __global__ void __launch_bounds__(512) few_kernel(MmArgs a, int rows_per_warp, i
                 for (int t = 0; t < NT; t++) {
                     float v = acc[t];
                     for (int o = lpr >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-                    if (l == 0 && t < cnt && cr + sub < rows) put(cr + sub, t, v);
+                    if (l == 0 && t < cnt && cr < a.n) put(cr, t, v);
                     acc[t] = 0.0f;
                 }
                 cp = l;
-                cr += at_once;
+                cr += turn;
             }
         }
     }
@@ -218,18 +222,16 @@ cudaError_t launch_few_t(const MmArgs& a, const LaunchCtx& ctx) {
     while (lpr > 4 && lpr / 2 >= pairs) lpr /= 2;
     // Activations beyond a quarter of an SM's shared memory: fewer CTAs fit, with 16 warps each.
     const int warps = bytes <= 48 * 1024 ? 8 : 16;
-    // Rows per warp such that the CTAs of all chunks fit the SMs at once: one wave of equal shares.
+    // As many CTAs as the SMs hold at once (all chunks together), so that the rows are dealt out evenly.
     static const int regs = [] {
         cudaFuncAttributes f;
         return cudaFuncGetAttributes(&f, few_kernel<T, NT>) == cudaSuccess ? (f.numRegs + 7) / 8 * 8 : 128;
     }();
     const int per_sm = std::max(1, std::min({65536 / (regs * 32 * warps), 64 / warps, 227 * 1024 / (bytes + 1024)}));
     const int64_t ctas = std::max<int64_t>(1, (int64_t)per_sm * ctx.num_sms / chunks);
-    const int at_once = 32 / lpr;
-    int64_t rpw = std::min<int64_t>(16, (a.n + ctas * warps - 1) / (ctas * warps));
-    rpw = (rpw + at_once - 1) / at_once * at_once;
-    const dim3 grid((unsigned)((a.n + warps * rpw - 1) / (warps * rpw)), (unsigned)chunks);
-    few_kernel<T, NT><<<grid, 32 * warps, bytes, ctx.stream>>>(a, (int)rpw, lpr);
+    const int64_t groups = (a.n + 32 / lpr - 1) / (32 / lpr);
+    const dim3 grid((unsigned)std::min(ctas, (groups + warps - 1) / warps), (unsigned)chunks);
+    few_kernel<T, NT><<<grid, 32 * warps, bytes, ctx.stream>>>(a, lpr);
     return cudaGetLastError();
 }
 

@@ -44,6 +44,7 @@
 // that unpacks cheapest (word_halves).
 #pragma once
 
+#include <algorithm>
 #include <cooperative_groups.h>
 
 #include "qs_matmul.cuh"
@@ -173,8 +174,9 @@ __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cas
 // The slots' Q8_0 rows as the matrix unit reads them, [chunk][stage]: BN rows of 64 float16 values
 // (two units) in the 128-byte swizzle, with LO the rows' low parts behind them; then as many stages as
 // hold 64 scaled level sums each (of a unit, or of its halves), times 2^-7. All times the row's power
-// of two, whose inverse goes to xs[chunk][slot]. Rows without a slot are zero. One warp per row: the
-// largest scale first, then lane l the units l, l + 32, ...
+// of two, whose inverse goes to xs[chunk][slot]. Rows without a slot stay as they are: their columns
+// of the product are not stored. gridDim.z warps per row: each finds the largest scale, then takes every
+// gridDim.z-th run of 32 units.
 template <int BN, int SUMS, bool LO>
 __global__ void __launch_bounds__(256) xpack_kernel(MmArgs a, uint8_t* out, float* xs) {
     constexpr int B_BYTES = BN * 128, X_BYTES = B_BYTES * (LO ? 2 : 1);
@@ -182,14 +184,14 @@ __global__ void __launch_bounds__(256) xpack_kernel(MmArgs a, uint8_t* out, floa
     if (ch.group < 0 || (a.order && ch.group == a.n_exp)) return;
     const int lane = threadIdx.x & 31, t = blockIdx.x * 8 + (threadIdx.x >> 5), stages = (a.units + 1) / 2;
     const int blocks = (a.units * SUMS + 63) / 64;
-    const bool live = ch.lo + t < ch.hi;
-    const int slot = live ? (a.order ? __ldg(a.order + ch.lo + t) : ch.lo + t) : 0;
+    if (ch.lo + t >= ch.hi) return;
+    const int slot = a.order ? __ldg(a.order + ch.lo + t) : ch.lo + t;
     const uint8_t* row = a.x + (int64_t)(slot / a.x_div) * a.x_row;
     uint32_t top = 0;  // largest |scale| as float16 bits; above 0x7BFF: inf or NaN
     for (int u0 = lane; u0 < a.units; u0 += 32 * 8) {  // 8 loads under way
         uint32_t d[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) d[j] = live && u0 + 32 * j < a.units ? ld_u16<1>(row + (int64_t)(u0 + 32 * j) * 34) & 0x7FFFu : 0u;
+        for (int j = 0; j < 8; j++) d[j] = u0 + 32 * j < a.units ? ld_u16<1>(row + (int64_t)(u0 + 32 * j) * 34) & 0x7FFFu : 0u;
 #pragma unroll
         for (int j = 0; j < 8; j++) top = max(top, d[j]);
     }
@@ -197,7 +199,7 @@ __global__ void __launch_bounds__(256) xpack_kernel(MmArgs a, uint8_t* out, floa
     // 2^(7 - exponent): scales below 2^8, values at most 2^15
     float up = 1.0f;
     if (top > 0 && top <= 0x7BFFu) up = __uint_as_float((uint32_t)(127 + 7 + 127 - (int)(__float_as_uint(h2f(top)) >> 23)) << 23);
-    if (lane == 0) xs[(int64_t)blockIdx.y * BN + t] = 1.0f / up;
+    if (lane == 0 && blockIdx.z == 0) xs[(int64_t)blockIdx.y * BN + t] = 1.0f / up;
     uint8_t* o = out + (int64_t)blockIdx.y * (stages + blocks) * X_BYTES;
     auto put_sum = [&](int p, float v) {  // term p of the level sums
         const int c = (p & 63) >> 3;
@@ -211,18 +213,19 @@ __global__ void __launch_bounds__(256) xpack_kernel(MmArgs a, uint8_t* out, floa
     auto load = [&](int u) {
 #pragma unroll
         for (int e = 0; e < 9; e++) next[e] = 0;
-        if (live && u < a.units) {
+        if (u < a.units) {
             ld_words<8, 1>(row + (int64_t)u * 34 + 2, next);
             next[8] = ld_u16<1>(row + (int64_t)u * 34);
         }
     };
-    load(lane);
-    for (int u = lane; u < last; u += 32) {
+    const int hop = 32 * gridDim.z;
+    load(blockIdx.z * 32 + lane);
+    for (int u = blockIdx.z * 32 + lane; u < last; u += hop) {
         uint32_t q[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) q[e] = next[e];
         const float d = h2f(next[8]) * up;
-        load(u + 32);
+        load(u + hop);
         if (u < 2 * stages) {
             uint8_t* st = o + (int64_t)(u >> 1) * X_BYTES;
 #pragma unroll
@@ -295,7 +298,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
         const bool some = !a.order || ch.group < a.n_exp;
         for (int t = tid; t < BN; t += TC_THREADS) {
             s_slot[t] = ch.lo + t < ch.hi ? (a.order ? __ldg(a.order + ch.lo + t) : ch.lo + t) : 0;
-            s_up[t] = some ? __ldg(xs + (int64_t)blockIdx.y * BN + t) : 1.0f;
+            s_up[t] = some && ch.lo + t < ch.hi ? __ldg(xs + (int64_t)blockIdx.y * BN + t) : 1.0f;
         }
     }
     if (warp == 16) {
@@ -619,7 +622,9 @@ cudaError_t launch_tc_t(const MmArgs& a, void* ws, const LaunchCtx& ctx) {
     if (chunks > 65535) return cudaErrorInvalidConfiguration;
     float* xs = static_cast<float*>(ws);
     uint8_t* xp = static_cast<uint8_t*>(ws) + xs_bytes(chunks, BN);
-    xpack_kernel<BN, C::SUMS, LO><<<dim3(BN / 8, (unsigned)chunks), 256, 0, ctx.stream>>>(a, xp, xs);
+    // warps per row: up to four CTAs per SM in all, each warp with a run of 32 units at least
+    const int64_t rows8 = BN / 8 * chunks, runs = (a.units + 31) / 32, z = std::max<int64_t>(1, std::min(runs, 4 * 148 / rows8));
+    xpack_kernel<BN, C::SUMS, LO><<<dim3(BN / 8, (unsigned)chunks, (unsigned)z), 256, 0, ctx.stream>>>(a, xp, xs);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     auto kernel = tc_kernel<T, BN, LO>;
