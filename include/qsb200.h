@@ -226,7 +226,7 @@ int qs_expert_plan(const int32_t* ids, int64_t n_slots, int n_experts, int32_t* 
  * out[r, j] = sum_c W[j, c] X[r, c]: packed weights of any type above (n rows of k values), X
  * n_rows rows of Q8_0 blocks (qs_rms_norm_q8, or qs_quantize with QS_TYPE_Q8_0). Levels are
  * multiplied exactly; scales and sums are float32, rounded once to out_type. For BF16 results of more than
- * 64 rows the activations are rounded to 11 bits first (1/8 of the result's own rounding).
+ * 32 rows the activations are rounded to 11 bits first (1/8 of the result's own rounding).
  *   w                     weight row j at w + j * w_row_bytes; w and w_row_bytes multiples of 16
  *                         bytes for Q4_K and Q5_K, 8 for Q5_1 and IQ4_XS, 4 for Q4_1 and Q2_K, else 2
  *   x                     row r at x + r * x_row_bytes, any alignment
@@ -248,7 +248,7 @@ int qs_matmul_workspace(int ggml_type, int64_t n, int64_t k, int64_t n_rows, int
  *   weights               NULL: out has a row per slot, zeros where the slot has no expert.
  *                         Else n_tokens x top_k float32: out has a row per token, the sum over its
  *                         slots with an expert of weight * product, in slot order.
- * n_tokens * top_k <= 2^20. Strides, alignment, rounding (more than 64 slots per expert on average) and
+ * n_tokens * top_k <= 2^20. Strides, alignment, rounding (more than 32 slots per expert on average) and
  * workspace as qs_matmul; sum: weights given.
  */
 int qs_matmul_experts(int ggml_type, const void* w, int64_t w_row_bytes, int64_t w_expert_bytes, int n_experts, int64_t n,

@@ -445,6 +445,11 @@ bool has_min(int type) {
     return type == qs::QS_Q4_1 || type == qs::QS_Q5_1 || type == qs::QS_Q2_K || type == qs::QS_Q4_K || type == qs::QS_Q5_K;
 }
 
+// two scales per 32 values
+bool two_scales(int type) {
+    return type == qs::QS_Q2_K || type == qs::QS_Q3_K || type == qs::QS_Q6_K || type == qs::QS_IQ2_XS || type == qs::QS_IQ2_S;
+}
+
 // How a product runs: which kernel, its tile, over how many CTAs a tile's rows are split.
 struct MmPlan {
     enum { FEW, MID, TC } kind;
@@ -460,9 +465,16 @@ MmPlan mm_plan(int type, int64_t n, int64_t k, int64_t slots, int64_t groups, in
     const int64_t avg = (slots + groups - 1) / groups, units = k / 32, stages = (units + 1) / 2;
     // rows that the kernel for few slots can not hold go to the next one
     const bool holds = units * qs::FEW_SLOTS * qs::FEW_UNIT_MAX <= qs::FEW_SMEM_MAX;
-    p.kind = (experts ? avg <= 1 : slots <= 4) && holds ? MmPlan::FEW : avg <= 64 ? MmPlan::MID : MmPlan::TC;
+    // The tcgen05 kernel from 65 rows on; with experts from an average of 57, where many of them have over 64
+    // and so two tiles of 64 (32 of 2048 x 2048, float32 results, Q6_K: 56 rows each 160 / 176 us, 64 rows 231 /
+    // 176 us). For bfloat16 results from 33 rows on with superblocks, whose unpacking it does once for all
+    // rows (64 rows of 4096 x 14336: Q4_K 56 / 44 us, Q6_K 76 / 58 us; Q4_0 46 / 50 us), but not for small
+    // matrices with one scale per 32 values (2048 x 1024: Q4_K 14.1 / 15.9 us, Q6_K 17.8 / 16.3 us).
+    const bool early = !lo && find_type(type)->qk == 256 && (experts || two_scales(type) || n * k >= (int64_t)1 << 25);
+    const int64_t mid = early ? 32 : experts ? 56 : 64;
+    p.kind = (experts ? avg <= 1 : slots <= 4) && holds ? MmPlan::FEW : avg <= mid ? MmPlan::MID : MmPlan::TC;
     p.lo = lo;
-    p.bn = avg <= 8 ? 8 : avg <= 16 ? 16 : avg <= 32 ? 32 : avg <= 64 ? 64 : avg <= 128 || lo ? 128 : 256;
+    p.bn = avg <= 8 ? 8 : avg <= 16 ? 16 : avg <= 32 ? 32 : p.kind == MmPlan::MID ? 64 : avg <= 128 || lo ? 128 : 256;
     p.splits = 1;
     const int64_t chunks = groups == 1 ? (slots + p.bn - 1) / p.bn : slots / p.bn + (groups < slots ? groups : slots) / 2 + 1;
     const int64_t tiles = (n + 127) / 128 * chunks, ctas = p.kind == MmPlan::MID ? 2 * 148 : 148;

@@ -150,7 +150,7 @@ __device__ __forceinline__ int sum16(const uint4& v) {
 // and slot, for up to 4 slots
 constexpr int FEW_SMEM_MAX = 200 * 1024, FEW_SLOTS = 4, FEW_UNIT_MAX = 44;
 cudaError_t launch_mm_few(int type, const MmArgs& a, const LaunchCtx& ctx);
-// up to 64 slots a matrix (qs_matmul_mid.cu): tiles of bn = 8, 16, 32 or 64 slots; ws: mm_mid_workspace
+// up to 64 slots a matrix, for bfloat16 results 32 with superblocks (qs_matmul_mid.cu): tiles of bn = 8, 16, 32 or 64 slots; ws: mm_mid_workspace
 // bytes; rows: activation rows
 inline int64_t mm_mid_workspace(int64_t units, int64_t rows, int sums) { return rows * ((units + 3) / 4 * 4) * (32 + 4 * (1 + sums)); }
 cudaError_t launch_mm_mid(int type, const MmArgs& a, int bn, int rows, void* ws, const LaunchCtx& ctx);

@@ -1,5 +1,5 @@
-// Packed products for up to 64 slots per weight matrix: 16 weight rows per warp on the integer
-// tensor cores (mma.sync s8).
+// Packed products for up to 64 slots per weight matrix (32 for bfloat16 results from superblocks): 16
+// weight rows per warp on the integer tensor cores (mma.sync s8).
 //
 // Both operands are 8-bit levels, so a unit's 32 products sum exactly in the s32 accumulator; the
 // accumulator starts at the bit pattern of 1.5 * 2^23 and its result is that float plus the sum
@@ -19,7 +19,7 @@
 // 2 us, products 5 us (the float operations, 12 cycles per 16 x 8 product), joining the cluster's tiles 3 us;
 // fewer CTAs per cluster, or one per SM, are slower (24 against 21 us). Q6_K's unaligned bytes make
 // shared memory the bound (66 % of its cycles); pieces of 8 bytes, which halve the bank conflicts, cost more
-// copies than they save (38 us).
+// copies than they save (38 us), and 16-byte loads without conflicts more selects (36 us).
 #include <cooperative_groups.h>
 
 #include "qs_matmul.cuh"

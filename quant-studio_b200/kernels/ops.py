@@ -201,7 +201,7 @@ def _experts_workspace(*sizes: int) -> int:
 def matmul(blocks: torch.Tensor, ggml_type: int, x_q8: torch.Tensor, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """(rows, n) products of packed weights (n, row bytes) with Q8_0 activations (rows, k / 32 * 34):
     the decoded activations times the decoded weights transposed. Levels are multiplied exactly, scales
-    and sums are float32, rounded once to out_dtype (bfloat16 results of more than 64 rows: from
+    and sums are float32, rounded once to out_dtype (bfloat16 results of more than 32 rows: from
     activations rounded to 11 bits, 1/8 of the result's own rounding). Row strides may exceed the rows;
     weight rows must start on multiples of 16 bytes for Q4_K / Q5_K, 8 for Q5_1 / IQ4_XS, 4 for
     Q4_1 / Q2_K, 2 for the others.

@@ -212,6 +212,33 @@ def test_matmul_wide_tiles(qtype, rows):
     check_product(got, *ref.product(x, w, qtype, "bfloat16"))
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("qtype,n,k", [("q6_k", 131, 768), ("q2_k", 131, 768), ("q4_k", 131, 768), ("q4_k", 2048, 16384)])
+@pytest.mark.parametrize("rows", [32, 33, 64, 65])
+def test_matmul_between_kernels(qtype, n, k, rows, dtype):
+    """Row counts at which another kernel takes over, for formats and sizes on both sides of the rule."""
+    rng = np.random.default_rng(rows)
+    w = ref.random_blocks(qtype, (n,), k, rng)
+    x = ref.random_blocks("q8_0", (rows,), k, rng)
+    got = ops.matmul(cuda(w), int(ref.GTYPE[qtype]), cuda(x), out_dtype=DT[dtype])
+    check_product(got, *ref.product(x, w, qtype, dtype))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("qtype", ["q4_0", "q4_k", "q6_k"])
+@pytest.mark.parametrize("tokens", [32, 33, 56, 57])
+def test_experts_between_kernels(qtype, tokens, dtype):
+    """Averages at which another kernel takes over; one expert has no slot, one three times the average."""
+    rng = np.random.default_rng(tokens)
+    e, n, k = 4, 131, 512
+    w = ref.random_blocks(qtype, (e, n), k, rng)
+    x = ref.random_blocks("q8_0", (tokens * e,), k, rng)
+    ids = np.full((tokens * e, 1), 1, dtype=np.int32)
+    ids[:tokens] = 3
+    got = ops.matmul_experts(cuda(w), int(ref.GTYPE[qtype]), cuda(x), ops.expert_plan(cuda(ids), e), out_dtype=DT[dtype])
+    check_product(got, *experts_want(x, w, qtype, ids, None, True, dtype))
+
+
 @pytest.mark.parametrize("qtype", ["q4_k", "q5_0"])
 @pytest.mark.parametrize("weighted", [False, True])
 def test_experts_wide_tiles(qtype, weighted):
