@@ -30,9 +30,11 @@
 //                cover a row's share wherever it starts, adjacent lanes adjacent pieces
 // Stages are a ring in shared memory (full: unpacked + copied, empty: products done); the
 // accumulators are a ring in tensor memory; the weights' scales are a longer ring of their own, which
-// the unpacking can not lap: stage i waits for the products of stage i - NS, these for the release of
-// their accumulator, so the sums are at most NS + 7 stages behind. Every wait is bounded: one that runs
-// out records bit 0 of the fault word and its role leaves.
+// the unpacking can not lap: stage i waits for the products of stage i - NS, these for their accumulator,
+// which the sums released NB accumulators ago. With GROUP stages to an accumulator the oldest scale that is
+// still to be read is at most NS + (NB - 1) GROUP stages old (16 for tiles of 128 with GROUP = 4, else 10 at
+// most), less than the ring's length. Every wait is bounded: one that runs out records bit 0 of the fault
+// word and its role leaves.
 // Measured: 2048 slots of Q4_K 14336 x 4096 to bfloat16 338 us with xpack_kernel (11 us), 711 TFLOP/s, 43 % of the
 // measured bf16 rate; 4096 slots of 4096 x 4096 205 us; 1024 to float32 (LO) 108 us. Without any unpacking or
 // copying the same loop takes 247 us: a stage moves 105 KB through shared memory (operands read by
@@ -73,18 +75,20 @@ struct TcCfg {
     static constexpr int RS = L::QK == 256 ? 4 : 2, WB = RS * 64 / L::QK * L::BB;
     static constexpr int COVER = L::MAXAL >= 16 ? WB : (WB + 16 - L::MAXAL + 15) / 16 * 16, WP = COVER / 16 % 2 ? COVER : COVER + 16;
     static constexpr int RAW = TC_M * WP, RR = 2 * RAW <= 24 * 1024 ? 4 : 2;  // steps in the ring
-    static constexpr int DR = 16;                      // ring of scales, [slot][unit][128]
-    static constexpr int D_BYTES = DR * 2 * TC_M * 4;
-    static constexpr int FIT = (TC_SMEM - 1024 - 512 - BN * 8 - D_BYTES - RR * RAW) / STAGE, NS = FIT > 4 ? 4 : FIT;
     static constexpr int NB = BN == 256 ? 2 : 4;       // accumulators in tensor memory
     static constexpr int COLS = NB * BN;
+    static constexpr int NS_MAX = 4;
+    // ring of scales, [slot][unit][128]: longer than the stages that unpacking may be ahead of the sums
+    static constexpr int LEAD = NS_MAX + (NB - 1) * (GROUP ? GROUP : 1), DR = LEAD < 16 ? 16 : 32;
+    static constexpr int D_BYTES = DR * 2 * TC_M * 4;
+    static constexpr int FIT = (TC_SMEM - 1024 - 512 - BN * 8 - D_BYTES - RR * RAW) / STAGE, NS = FIT > NS_MAX ? NS_MAX : FIT;
     // the sums of 256 columns are 128 registers a thread: registers move to their two warpgroups
     // (160, 160, 64, 64, 32 a thread of the 96 at launch)
     static constexpr int R_SUM = 160, R_UNPACK = 64, R_REST = 32, R_LAUNCH = 96;
     static_assert(2 * R_SUM + 2 * R_UNPACK + R_REST <= 5 * R_LAUNCH, "the shares are what the launch has");
     static constexpr int OUT_PITCH = TC_M + 4;
     static constexpr int BYTES = NS * STAGE + D_BYTES + RR * RAW + 1024;  // 1024 to align the ring
-    static_assert(NS >= 2 && DR >= NS + 8, "ring lengths");
+    static_assert(NS >= 2 && DR > NS + (NB - 1) * (GROUP ? GROUP : 1), "ring lengths");
     static_assert(BN * OUT_PITCH * 4 <= NS * STAGE, "the tile leaves through the same memory");
     // further stages with the minima of `units` units: 64 terms each, with LO once for the hi and
     // once for the lo part of the weights' side
