@@ -155,11 +155,11 @@ cudaError_t launch_mm_few(int type, const MmArgs& a, const LaunchCtx& ctx);
 inline int64_t mm_mid_workspace(int64_t units, int64_t rows, int sums) { return rows * ((units + 3) / 4 * 4) * (32 + 4 * (1 + sums)); }
 cudaError_t launch_mm_mid(int type, const MmArgs& a, int bn, int rows, void* ws, const LaunchCtx& ctx);
 // tcgen05 tiles (qs_matmul_tc.cuh): tiles of bn slots; lo: both float16 parts of the activations. ws:
-// mm_tc_workspace bytes for `chunks` chunks (the rows' powers of two lead); sums: level sums per unit
-// (1 with minima, 2 with minima per 16 values, else 0)
+// mm_tc_workspace bytes for `chunks` chunks (the rows' powers of two lead); sums: sums of activations per unit
+// (1 with minima, 2 with minima per 16 values, else 0), 32 to a stage
 inline int64_t xs_bytes(int64_t chunks, int bn) { return (chunks * bn * 4 + 255) / 256 * 256; }
 inline int64_t mm_tc_workspace(int64_t units, int64_t chunks, int bn, bool lo, int sums) {
-    return xs_bytes(chunks, bn) + chunks * ((units + 1) / 2 + (units * sums + 63) / 64) * (int64_t)bn * 128 * (lo ? 2 : 1);
+    return xs_bytes(chunks, bn) + chunks * ((units + 1) / 2 + (units * sums + 31) / 32) * (int64_t)bn * 128 * (lo ? 2 : 1);
 }
 // by the file that holds the type
 cudaError_t launch_mm_tc_legacy(int type, const MmArgs& a, int bn, bool lo, void* ws, const LaunchCtx& ctx);

@@ -9,10 +9,17 @@
 // Activations: scale * level has 19 bits; times a power of two per row (so that the row's largest lies
 // below 2^15) it is float16 hi + lo, exact together down to 2^-39 of the row's largest. LO: the
 // products use both parts (Q6_K: hi hi, hi lo, lo hi), for float32 and float16 results. For
-// bfloat16 results hi alone is multiplied: its rounding, 2^-12 of a value, is 1/8 of the result's.
-// Minima: - ml[n, unit] * (scale * sum of levels)[t, unit] is a product of its own, with K / 32 (K / 16
-// for Q2_K) terms; it follows the levels as further stages of 64 terms, float16 like the activations
-// (LO: hi and lo of both), the weights' side times a power of two per row and 32 terms.
+// bfloat16 results hi alone is multiplied: that rounds the activations to 11 bits, by at most 2^-11 of a value
+// (2^-40 of the row's largest for values below 2^-29 of it), 1/8 of the result's own rounding where the terms
+// are of both signs (in the 2-norm 2.1e-4 and 1.66e-3). Q6_K's level * sub-scale above 2048 (5 % of the weights with
+// sub-scales of 40 to 127) is rounded to 11 bits there as well.
+// Minima: - ml[n, unit] * (sum of the unit's activations)[t, unit] is a product of its own, with K / 32 (K / 16
+// for Q2_K) terms; it follows the levels as further stages of 32 terms, the weights' side times a power of two
+// per row and stage. It nearly cancels the levels' product where the activations have one sign, so both sides are
+// hi + lo for every result (22 bits; the hi parts are the stage's first 32 columns, the lo parts the others, and
+// all four pairs are multiplied), and the sums are those of the activations as they are multiplied. With 11 bits
+// of either, the error of Q4_K with 4096 values was 6e-4 of the result for normal activations and 3e-3 for
+// equal ones.
 //
 // A pass over K = 32 of a 128 x 256 tile is 271 cycles of the matrix unit (540 with LO). Scaling every 32
 // values by both operands' scales instead, with exact integers in D, was built first and took 1235 us
@@ -90,9 +97,8 @@ struct TcCfg {
     static constexpr int BYTES = NS * STAGE + D_BYTES + RR * RAW + 1024;  // 1024 to align the ring
     static_assert(NS >= 2 && DR > NS + (NB - 1) * (GROUP ? GROUP : 1), "ring lengths");
     static_assert(BN * OUT_PITCH * 4 <= NS * STAGE, "the tile leaves through the same memory");
-    // further stages with the minima of `units` units: 64 terms each, with LO once for the hi and
-    // once for the lo part of the weights' side
-    __host__ __device__ static int min_blocks(int units) { return (units * SUMS + 63) / 64; }
+    // further stages with the minima of `units` units: 32 terms each
+    __host__ __device__ static int min_blocks(int units) { return (units * SUMS + 31) / 32; }
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -177,17 +183,17 @@ __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cas
 
 // The slots' Q8_0 rows as the matrix unit reads them, [chunk][stage]: BN rows of 64 float16 values
 // (two units) in the 128-byte swizzle, with LO the rows' low parts behind them; then as many stages as
-// hold 64 scaled level sums each (of a unit, or of its halves), times 2^-7. All times the row's power
-// of two, whose inverse goes to xs[chunk][slot]. Rows without a slot stay as they are: their columns
-// of the product are not stored. gridDim.z warps per row: each finds the largest scale, then takes every
-// gridDim.z-th run of 32 units.
+// hold 32 sums of a unit's values each (or of its halves'), times 2^-7, their hi parts, then their lo parts.
+// All times the row's power of two, whose inverse goes to xs[chunk][slot]. Rows without a slot stay as they
+// are: their columns of the product are not stored. gridDim.z warps per row: each finds the largest scale, then
+// takes every gridDim.z-th run of 32 units.
 template <int BN, int SUMS, bool LO>
 __global__ void __launch_bounds__(256) xpack_kernel(MmArgs a, uint8_t* out, float* xs) {
     constexpr int B_BYTES = BN * 128, X_BYTES = B_BYTES * (LO ? 2 : 1);
     const Chunk ch = find_chunk<BN>(a, blockIdx.y);
     if (ch.group < 0 || (a.order && ch.group == a.n_exp)) return;
     const int lane = threadIdx.x & 31, t = blockIdx.x * 8 + (threadIdx.x >> 5), stages = (a.units + 1) / 2;
-    const int blocks = (a.units * SUMS + 63) / 64;
+    const int blocks = (a.units * SUMS + 31) / 32;
     if (ch.lo + t >= ch.hi) return;
     const int slot = a.order ? __ldg(a.order + ch.lo + t) : ch.lo + t;
     const uint8_t* row = a.x + (int64_t)(slot / a.x_div) * a.x_row;
@@ -205,14 +211,14 @@ __global__ void __launch_bounds__(256) xpack_kernel(MmArgs a, uint8_t* out, floa
     if (top > 0 && top <= 0x7BFFu) up = __uint_as_float((uint32_t)(127 + 7 + 127 - (int)(__float_as_uint(h2f(top)) >> 23)) << 23);
     if (lane == 0 && blockIdx.z == 0) xs[(int64_t)blockIdx.y * BN + t] = 1.0f / up;
     uint8_t* o = out + (int64_t)blockIdx.y * (stages + blocks) * X_BYTES;
-    auto put_sum = [&](int p, float v) {  // term p of the level sums
-        const int c = (p & 63) >> 3;
-        uint8_t* at = o + (int64_t)(stages + (p >> 6)) * X_BYTES + t * 128 + ((c ^ (t & 7)) << 4) + (p & 7) * 2;
+    auto put_sum = [&](int p, float v) {  // term p of the sums
+        const int c = (p & 31) >> 3;
+        uint8_t* at = o + (int64_t)(stages + (p >> 5)) * X_BYTES + t * 128 + (p & 7) * 2;
         const __half h = __float2half_rn(v);
-        *reinterpret_cast<__half*>(at) = h;
-        if constexpr (LO) *reinterpret_cast<__half*>(at + B_BYTES) = __float2half_rn(v - __half2float(h));
+        *reinterpret_cast<__half*>(at + ((c ^ (t & 7)) << 4)) = h;
+        *reinterpret_cast<__half*>(at + (((4 + c) ^ (t & 7)) << 4)) = __float2half_rn(v - __half2float(h));
     };
-    const int last = max(2 * stages, SUMS ? blocks * 64 / SUMS : 0);
+    const int last = max(2 * stages, SUMS ? blocks * 32 / SUMS : 0);
     uint32_t next[9];  // the next unit's levels and scale
     auto load = [&](int u) {
 #pragma unroll
@@ -230,6 +236,7 @@ __global__ void __launch_bounds__(256) xpack_kernel(MmArgs a, uint8_t* out, floa
         for (int e = 0; e < 8; e++) q[e] = next[e];
         const float d = h2f(next[8]) * up;
         load(u + hop);
+        float half_sum[2] = {0.0f, 0.0f};  // of the values as they are multiplied (multiples of one small step: exact)
         if (u < 2 * stages) {
             uint8_t* st = o + (int64_t)(u >> 1) * X_BYTES;
 #pragma unroll
@@ -243,6 +250,7 @@ __global__ void __launch_bounds__(256) xpack_kernel(MmArgs a, uint8_t* out, floa
                     const __half2 h = __floats2half2_rn(v0, v1);
                     const float2 f = __half22float2(h);
                     hi[e] = h2_bits(h);
+                    if constexpr (SUMS > 0 && !LO) half_sum[c >> 1] += f.x + f.y;
                     if constexpr (LO) lo[e] = h2_bits(__floats2half2_rn(v0 - f.x, v1 - f.y));
                 }
                 uint8_t* p = st + t * 128 + (((4 * (u & 1) + c) ^ (t & 7)) << 4);
@@ -251,12 +259,15 @@ __global__ void __launch_bounds__(256) xpack_kernel(MmArgs a, uint8_t* out, floa
             }
         }
         if constexpr (SUMS > 0) {
-            const int s0 = sum16(make_uint4(q[0], q[1], q[2], q[3])), s1 = sum16(make_uint4(q[4], q[5], q[6], q[7]));
-            if (u < blocks * 64 / SUMS) {
-                if constexpr (SUMS == 1) put_sum(u, d * 0.0078125f * (float)(s0 + s1));
+            if constexpr (LO) {
+                half_sum[0] = d * (float)sum16(make_uint4(q[0], q[1], q[2], q[3]));
+                half_sum[1] = d * (float)sum16(make_uint4(q[4], q[5], q[6], q[7]));
+            }
+            if (u < blocks * 32 / SUMS) {
+                if constexpr (SUMS == 1) put_sum(u, 0.0078125f * (half_sum[0] + half_sum[1]));
                 else {
-                    put_sum(2 * u, d * 0.0078125f * (float)s0);
-                    put_sum(2 * u + 1, d * 0.0078125f * (float)s1);
+                    put_sum(2 * u, 0.0078125f * half_sum[0]);
+                    put_sum(2 * u + 1, 0.0078125f * half_sum[1]);
                 }
             }
         }
@@ -320,11 +331,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
     const bool real = !a.order || ch.group < a.n_exp;
     // this CTA's stages: k0 .. of the levels (`main` of them), then its share of the minima's blocks
     const int k0 = min((int)blockIdx.z * per, stages), main = real ? min(per, stages - k0) : 0;
-    const int e0 = blocks * (int)blockIdx.z / a.splits, extra = real ? (blocks * ((int)blockIdx.z + 1) / a.splits - e0) * (LO ? 2 : 1) : 0;
+    const int e0 = blocks * (int)blockIdx.z / a.splits, extra = real ? blocks * ((int)blockIdx.z + 1) / a.splits - e0 : 0;
     const int total = main + extra;
     // whether unit uu of stage i begins / ends an accumulator
-    auto begins = [&](int i, int uu) { return !GROUP || i >= main || (uu == 0 && i % (GROUP ? GROUP : 1) == 0); };
-    auto ends = [&](int i, int uu) { return !GROUP || i >= main || (uu == 1 && (i % (GROUP ? GROUP : 1) == GROUP - 1 || i + 1 == main)); };
+    auto begins = [&](int i, int uu) { return i >= main ? uu == 0 : !GROUP || (uu == 0 && i % (GROUP ? GROUP : 1) == 0); };
+    auto ends = [&](int i, int uu) { return i >= main ? uu == 1 : !GROUP || (uu == 1 && (i % (GROUP ? GROUP : 1) == GROUP - 1 || i + 1 == main)); };
 
     if (warp >= 16) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::R_REST));
@@ -349,6 +360,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
                         for (int kk = 0; kk < 2; kk++) {
                             constexpr uint32_t X = C::A_ALL >> 4;
                             const uint32_t at = st + uu * 4 + kk * 2;
+                            if (SUMS > 0 && i >= main) {  // one part of the minima with both of the sums
+                                mma_f16(tmem + b * BN, at, st + kk * 2 + X, idesc, !first || kk > 0);
+                                mma_f16(tmem + b * BN, at, st + kk * 2 + X + 4, idesc, true);
+                                continue;
+                            }
                             mma_f16(tmem + b * BN, at, at + X, idesc, !first || kk > 0);
                             if constexpr (LO) mma_f16(tmem + b * BN, at, at + X + (C::B_BYTES >> 4), idesc, true);
                             if constexpr (C::SPLIT) mma_f16(tmem + b * BN, at + (C::A_BYTES >> 4), at + X, idesc, true);
@@ -404,8 +420,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
             for (; i < total; i++) {
                 const int s = i % NS;
                 if (!mbar_wait(empty + 8 * s, ((i / NS) & 1) ^ 1, a.fault)) break;
-                const int k = i < main ? k0 + i : stages + e0 + (i - main) / (LO ? 2 : 1);
-                bulk_load(ring + s * C::STAGE + C::A_ALL, src + (int64_t)k * C::X_BYTES, C::X_BYTES, full + 8 * s);
+                const int k = i < main ? k0 + i : stages + e0 + i - main;
+                bulk_load(ring + s * C::STAGE + C::A_ALL, src + (int64_t)k * C::X_BYTES, i < main ? C::X_BYTES : C::B_BYTES, full + 8 * s);
             }
             // no copy outlives the CTA
             for (int j = max(0, i - NS); j < i; j++) mbar_wait(full + 8 * (j % NS), (j / NS) & 1, a.fault);
@@ -473,43 +489,38 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
                 scales[((i % C::DR) * 2 + uu) * TC_M + row] = L::FOLD ? base_of<L>(r[uu]) : dl[0];
             }
         };
-        // 2 x 32 minima of the row (negated), each half times a power of two, its inverse (and the sums' 2^7)
+        // 32 minima of the row (negated) times a power of two, hi and lo parts; its inverse (and the sums' 2^7)
         // as the scale
         auto unpack_minima = [&](int i, uint8_t* st) {
             if constexpr (SUMS > 0) {
                 constexpr int PER = UPB * SUMS;  // minima of a block
-                const int e = (i - main) / (LO ? 2 : 1), part = LO ? (i - main) & 1 : 0;
-#pragma unroll 1
-                for (int uu = 0; uu < 2; uu++) {
-                    const int p0 = (e0 + e) * 64 + uu * 32;
-                    float m[32], top = 0.0f;
+                const int p0 = (e0 + i - main) * 32;
+                float m[32], top = 0.0f;
 #pragma unroll
-                    for (int p = 0; p < 32; p += PER) {
-                        const bool in = mine && p0 + p < a.units * SUMS;
+                for (int p = 0; p < 32; p += PER) {
+                    const bool in = mine && p0 + p < a.units * SUMS;
 #pragma unroll
-                        for (int j = 0; j < PER; j++) m[p + j] = 0.0f;
-                        if (in) L::template minima<L::MAXAL>(w + (int64_t)((p0 + p) / PER) * L::BB, m + p);
-                    }
-#pragma unroll
-                    for (int p = 0; p < 32; p++) top = fmaxf(top, fabsf(m[p]));
-                    float up = 1.0f;  // the largest below 2^11
-                    if (top > 0.0f && top < INFINITY) up = __uint_as_float((uint32_t)(127 + 10 + 127 - (int)(__float_as_uint(top) >> 23)) << 23);
-#pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        __half2 h[4];
-#pragma unroll
-                        for (int x = 0; x < 4; x++) {
-                            const float v0 = -m[8 * c + 2 * x] * up, v1 = -m[8 * c + 2 * x + 1] * up;
-                            h[x] = __floats2half2_rn(v0, v1);
-                            if (LO && part) {
-                                const float2 f = __half22float2(h[x]);
-                                h[x] = __floats2half2_rn(v0 - f.x, v1 - f.y);
-                            }
-                        }
-                        put(st, 4 * uu + c, h);
-                    }
-                    scales[((i % C::DR) * 2 + uu) * TC_M + row] = 128.0f / up;
+                    for (int j = 0; j < PER; j++) m[p + j] = 0.0f;
+                    if (in) L::template minima<L::MAXAL>(w + (int64_t)((p0 + p) / PER) * L::BB, m + p);
                 }
+#pragma unroll
+                for (int p = 0; p < 32; p++) top = fmaxf(top, fabsf(m[p]));
+                float up = 1.0f;  // the largest below 2^11
+                if (top > 0.0f && top < INFINITY) up = __uint_as_float((uint32_t)(127 + 10 + 127 - (int)(__float_as_uint(top) >> 23)) << 23);
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    __half2 h[4], l[4];
+#pragma unroll
+                    for (int x = 0; x < 4; x++) {
+                        const float v0 = -m[8 * c + 2 * x] * up, v1 = -m[8 * c + 2 * x + 1] * up;
+                        h[x] = __floats2half2_rn(v0, v1);
+                        const float2 f = __half22float2(h[x]);
+                        l[x] = __floats2half2_rn(v0 - f.x, v1 - f.y);
+                    }
+                    put(st, c, h);
+                    put(st, 4 + c, l);
+                }
+                scales[((i % C::DR) * 2 + 1) * TC_M + row] = 128.0f / up;
             }
         };
         int s = odd % NS, ph = odd / NS & 1 ? 0 : 1;  // stage of the ring, the parity that its last use ended with

@@ -201,10 +201,12 @@ def _experts_workspace(*sizes: int) -> int:
 def matmul(blocks: torch.Tensor, ggml_type: int, x_q8: torch.Tensor, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """(rows, n) products of packed weights (n, row bytes) with Q8_0 activations (rows, k / 32 * 34):
     the decoded activations times the decoded weights transposed. Levels are multiplied exactly, scales
-    and sums are float32, rounded once to out_dtype (bfloat16 results of more than 32 rows: from
-    activations rounded to 11 bits, 1/8 of the result's own rounding). Row strides may exceed the rows;
-    weight rows must start on multiples of 16 bytes for Q4_K / Q5_K, 8 for Q5_1 / IQ4_XS, 4 for
-    Q4_1 / Q2_K, 2 for the others.
+    and sums are float32, rounded once to out_dtype. For bfloat16 results of more than 32 rows the activations
+    may be rounded to 11 bits first (at most 2^-11 of a value, 1/8 of the result's own rounding), and Q6_K's
+    products of level and sub-scale above 2048 as well. The last bits of a row's result depend on the number of
+    rows beside it (matmul_experts: per expert, on average), which decides the kernel; the same call gives the same
+    bits every time. Row strides may exceed the rows; weight rows must start on multiples of 16 bytes for
+    Q4_K / Q5_K, 8 for Q5_1 / IQ4_XS, 4 for Q4_1 / Q2_K, 2 for the others.
     """
     dev, k = _packed_args(blocks, ggml_type, x_q8, 2, out_dtype)
     n, rows = blocks.shape[0], x_q8.shape[0]

@@ -48,9 +48,9 @@ def configurations(tmp_path_factory):
 
 def accumulators(main, extra, group):
     """(first stage, last stage) of every accumulator: one per `group` of the `main` stages of levels (0: one per
-    unit of 32 values, two a stage), two per stage of the `extra` ones with minima."""
+    unit of 32 values, two a stage), one per stage of the `extra` ones with minima."""
     r = [(i, min(i + group, main) - 1) for i in range(0, main, group)] if group else [(i, i) for i in range(main) for _ in range(2)]
-    return r + [(i, i) for i in range(main, main + extra) for _ in range(2)]
+    return r + [(i, i) for i in range(main, main + extra)]
 
 
 def lapped(main, extra, ns, nb, group, dr):
