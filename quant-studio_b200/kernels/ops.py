@@ -243,7 +243,7 @@ def matmul_experts(blocks: torch.Tensor, ggml_type: int, x_q8: torch.Tensor, pla
     shape = (tokens, top_k, n) if weights is None else (tokens, n)
     if slots == 0:
         return torch.zeros(shape, dtype=out_dtype, device=blocks.device)
-    row = blocks.stride(1) if n > 1 else -(-blocks.shape[2] // 16) * 16  # a stride that nothing steps over fits any alignment
+    row = blocks.stride(1) if n > 1 else blocks.shape[2]  # whole blocks: as aligned as the format asks
     expert = blocks.stride(0) if experts > 1 else n * row
     per_slot, summed = int(rows != tokens), int(weights is not None)
     size = _experts_workspace(int(ggml_type), experts, n, k, tokens, top_k, per_slot, summed, SRC_IDS[out_dtype])
