@@ -5,10 +5,11 @@
 //   per 32 values: m = max |p|, levels sign(p) floor(127 |p| / m + 1/2), scale f16(m r / 127)
 //
 // The levels do not depend on r, and |p| / m is compared with the borders between two levels as in 64
-// bits: in float32 first, where a level's error is below 3e-5 of a step and a scale's below 3e-7; blocks
-// with a value within 4e-5 of a border, or a scale within 4e-7 of a float16 border, are done again in
-// double by their warp (about one warp pass of 8 blocks in 25). The sum of squares is in double
-// throughout. A row holding inf or NaN gets NaN scales and zero levels.
+// bits: in float32 first, where a level's error is below 4.6e-5 of a step (two units of __fdividef's last
+// place and the roundings of p and m, 3.6e-7 of up to 127.5) and a scale's below 2.4e-7; blocks with a value within
+// 5e-5 of a border, or a scale within 3e-7 of a float16 border, are done again in double by their warp (about
+// one warp pass of 8 blocks in 20). The sum of squares is in double throughout. A row holding inf or NaN gets
+// NaN scales and zero levels.
 //
 // Bound: device memory (read x and the residual, write their sum and 34 bytes per 32 values), then the
 // some 33 instructions per value (the part before the row's sum alone runs at the memory's pace). One
@@ -32,6 +33,10 @@ struct NormArgs {
     int k;
     double eps, inv_k;
 };
+
+// float32 remainders of levels below SURE, and scales that NEAR does not take across a float16 border, are
+// as in exact arithmetic
+constexpr float SURE = 0.49995f, NEAR = 4e-7f;
 
 // 1 / sqrt(x) to about one step: two Newton steps from the float32 approximation (2^-22, squared twice)
 __device__ __forceinline__ double rsqrt64(double x) {
@@ -199,7 +204,7 @@ __global__ void __launch_bounds__(1024) norm_kernel(NormArgs a) {
         const float ds = __fmul_rn(mh, r127f);
         uint16_t d = f16_bits(ds);
         const bool normal = mh > 1e-25f && mh < 1e37f;  // products and their remainders are normal numbers
-        const bool sure = off < 0.49996f && f16_bits(__fmul_rn(ds, 1.0f - 4e-7f)) == f16_bits(__fmul_rn(ds, 1.0f + 4e-7f));
+        const bool sure = off < SURE && f16_bits(__fmul_rn(ds, 1.0f - NEAR)) == f16_bits(__fmul_rn(ds, 1.0f + NEAR));
         if (!__all_sync(0xffffffffu, (normal && sure) || !live || bad)) {
             if (__all_sync(0xffffffffu, normal || !live || bad)) {
                 // the block's exact largest product: the largest remainder among the largest products
@@ -216,7 +221,7 @@ __global__ void __launch_bounds__(1024) norm_kernel(NormArgs a) {
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     const float n = __fadd_rn(__uint_as_float(z[i]), -12582912.0f), f = __fmaf_rn(p[i], inv, -n);
-                    if (live && fabsf(f) >= 0.49996f) {
+                    if (live && fabsf(f) >= SURE) {
                         const double h = (double)n + (f > 0.0f ? 0.5 : -0.5), x = (double)t[i] * (double)w[i];
                         // the distance from the border: next to it both differences are exact
                         const double y = 127.0 * x, over = fma(-h, m, y) + fma(127.0, x, -y);
