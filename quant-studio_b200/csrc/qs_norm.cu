@@ -14,7 +14,7 @@
 // Bound: device memory (read x and the residual, write their sum and 34 bytes per 32 values), then the
 // some 33 instructions per value (the part before the row's sum alone runs at the memory's pace). One
 // row per CTA, two chunks of 8 values per thread in registers between the passes. Measured: 4096 rows of
-// 4096 bfloat16 with a residual 34.5 us, 3.5 TB/s (four chunks per thread, fewer warps: 45 us; every
+// 4096 bfloat16 with a residual 35.3 us, 3.4 TB/s (four chunks per thread, fewer warps: 45 us; every
 // border in double by the full formula: 38 us); one row of 4096 3 us.
 #include "qs_kernels.h"
 
@@ -45,6 +45,32 @@ __device__ __forceinline__ double rsqrt64(double x) {
 #pragma unroll
     for (int i = 0; i < 2; i++) y = fma(y * 0.5, fma(-x * y, y, 1.0), y);
     return y;
+}
+
+// 127 x - h m, of the right sign for products x and m of two float32 values and h of 8 bits: next to the border
+// both differences are exact
+__device__ __forceinline__ double over_border(double x, double m, double h) {
+    const double y = 127.0 * x;
+    return fma(-h, m, y) + fma(127.0, x, -y);
+}
+
+// Levels (x, y) and scale (z) of 8 values of a block, whose 4 lanes call it together, for products of any size. Rarely
+// needed, and kept out of the kernel's registers (inlined: 36.6 us for 4096 rows of 4096).
+__device__ __noinline__ uint3 in_double(const float* t, const float* w, double r127) {
+    double m = 0.0;
+#pragma unroll 1
+    for (int i = 0; i < 8; i++) m = fmax(m, fabs((double)t[i] * (double)w[i]));
+    m = fmax(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = fmax(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    if (!(m <= 1.7e308)) return make_uint3(0, 0, 0x7E00);
+    unsigned long long q = 0;
+#pragma unroll 1
+    for (int i = 0; i < 8 && m > 0.0; i++) {
+        const double x = (double)t[i] * (double)w[i], h = floor(127.0 * (fabs(x) / m)) + 0.5;
+        const int l = (int)(over_border(fabs(x), m, h) >= 0.0 ? h + 0.5 : h - 0.5);
+        q |= (unsigned long long)((uint32_t)(x < 0.0 ? -l : l) & 0xFFu) << (8 * i);
+    }
+    return make_uint3((uint32_t)q, (uint32_t)(q >> 32), f16_bits((float)(m * r127)));
 }
 
 __device__ __forceinline__ double block_sum(double v, double* red) {
@@ -222,31 +248,23 @@ __global__ void __launch_bounds__(1024) norm_kernel(NormArgs a) {
                 for (int i = 0; i < 8; i++) {
                     const float n = __fadd_rn(__uint_as_float(z[i]), -12582912.0f), f = __fmaf_rn(p[i], inv, -n);
                     if (live && fabsf(f) >= SURE) {
-                        const double h = (double)n + (f > 0.0f ? 0.5 : -0.5), x = (double)t[i] * (double)w[i];
-                        // the distance from the border: next to it both differences are exact
-                        const double y = 127.0 * x, over = fma(-h, m, y) + fma(127.0, x, -y);
+                        const double h = (double)n + (f > 0.0f ? 0.5 : -0.5), over = over_border((double)t[i] * (double)w[i], m, h);
                         const int level = (int)(over > 0.0 || (over == 0.0 && h > 0.0) ? h + 0.5 : h - 0.5);
                         const int sh = 8 * (i & 3);
                         q[i >> 2] = (q[i >> 2] & ~(0xFFu << sh)) | (((uint32_t)level & 0xFFu) << sh);
                     }
                 }
             } else {
-                double m = 0.0;
+                float copy[16];
 #pragma unroll
-                for (int i = 0; i < 8; i++)
-                    if (live) m = fmax(m, fabs((double)t[i] * (double)w[i]));
-                m = fmax(m, __shfl_xor_sync(0xffffffffu, m, 1));
-                m = fmax(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                q[0] = q[1] = 0;
-                if (live && m > 0.0 && m <= 1.7e308) {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const double x = (double)t[i] * (double)w[i];
-                        const int l = (int)floor(__dadd_rn(__dmul_rn(127.0, fabs(x) / m), 0.5));
-                        q[i >> 2] |= ((uint32_t)(x < 0.0 ? -l : l) & 0xFFu) << (8 * (i & 3));
-                    }
+                for (int i = 0; i < 8; i++) {
+                    copy[i] = live ? t[i] : 0.0f;
+                    copy[8 + i] = live ? w[i] : 0.0f;
                 }
-                d = m <= 1.7e308 ? f16_bits((float)(m * r127)) : (uint16_t)0x7E00;
+                const uint3 r = in_double(copy, copy + 8, r127);
+                q[0] = r.x;
+                q[1] = r.y;
+                d = (uint16_t)r.z;
             }
         }
         if (bad) {
