@@ -197,7 +197,7 @@ int qs_rms_norm_q8(const void* x, int x_type, int64_t x_row_stride, const void* 
 #define QS_SCORE_SOFTMAX 0
 #define QS_SCORE_SIGMOID 1
 #define QS_GROUP_MAX 0   /* a group counts as its best expert */
-#define QS_GROUP_TOP2 1  /* ... as the sum of its two best */
+#define QS_GROUP_TOP2 1  /* ... as the sum of its two best; groups have two experts at least */
 
 /*
  * The experts of every token: top_k of n_experts by score + bias, best first, ties to the lowest
@@ -208,7 +208,8 @@ int qs_rms_norm_q8(const void* x, int x_type, int64_t x_row_stride, const void* 
  *   ids, weights   n_rows x top_k; weight = score (over the sum of the chosen scores if
  *                  renormalize) * scale; 0 where that sum is 0
  * An expert whose logit or score + bias is -inf or NaN is never chosen; where too few are
- * left the id is -1 and the weight 0. top_k <= 32.
+ * left the id is -1 and the weight 0. With QS_GROUP_TOP2 a group with fewer than two others comes
+ * after all that have two. top_k <= 32.
  */
 int qs_route(const void* logits, int logits_type, int64_t logits_row_stride, int64_t n_rows, int n_experts, int top_k,
              int score, const float* bias, int n_groups, int groups_kept, int group_score, int renormalize, float scale,

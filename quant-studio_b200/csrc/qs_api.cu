@@ -598,6 +598,7 @@ QS_API int qs_route(const void* logits, int logits_type, int64_t logits_row_stri
     if (group_score != QS_GROUP_MAX && group_score != QS_GROUP_TOP2) return fail(QS_EINVAL, "group score %d is neither max nor top2", group_score);
     if (n_groups < 1 || n_groups > 64 || n_experts % n_groups) return fail(QS_EINVAL, "%d groups do not divide %d experts (at most 64)", n_groups, n_experts);
     if (groups_kept < 1 || groups_kept > n_groups) return fail(QS_EINVAL, "%d of %d groups can not be kept", groups_kept, n_groups);
+    if (group_score == QS_GROUP_TOP2 && n_groups > 1 && n_groups == n_experts) return fail(QS_EINVAL, "groups of one expert have no two best");
     const int usable = n_experts / n_groups * groups_kept;
     if (top_k < 1 || top_k > 32 || top_k > usable) return fail(QS_EINVAL, "top_k %d is not in 1 .. %d", top_k, usable < 32 ? usable : 32);
     if (n_rows < 0 || n_rows > INT32_MAX) return fail(QS_EINVAL, "row count %lld is not in 0 .. 2^31 - 1", (long long)n_rows);

@@ -105,7 +105,8 @@ def route(logits: torch.Tensor, top_k: int, score: str = "softmax", bias: torch.
 
     Chosen by softmax or sigmoid score + bias (float32, for the choice alone), from the
     groups_kept best of n_groups equal runs of experts (a group counts as its best expert, or as
-    the sum of its two best: group_score "max" / "top2"); ties go to the lowest expert. Weights
+    the sum of its two best: group_score "max" / "top2"; for the latter groups have two experts at
+    least, and those with fewer than two that can be chosen come last); ties go to the lowest expert. Weights
     are the scores, over their sum if renormalize, times scale. Experts at -inf or NaN are
     never chosen; a slot left over has id -1 and weight 0. Returns ((n, top_k) int32, (n, top_k) float32).
     """

@@ -46,6 +46,14 @@ def test_route(bad):
     assert route(**bad) == E
 
 
+def test_route_two_best_of_groups_of_one():
+    """A group of one expert has no second best; a single group's score decides nothing."""
+    assert route(g=8, kept=2, k=2, gscore=1) == E
+    assert route(n=0, z=None, ids=None, w=None, g=8, kept=2, k=2, gscore=0) == OK
+    assert route(n=0, z=None, ids=None, w=None, g=4, kept=2, k=2, gscore=1) == OK
+    assert route(n=0, z=None, ids=None, w=None, g=1, kept=1, e=1, zs=1, k=1, gscore=1) == OK
+
+
 @pytest.mark.parametrize("bad", [dict(n=-1), dict(n=(1 << 20) + 1), dict(e=0), dict(e=1025), dict(ids=None), dict(order=None), dict(off=None), dict(ids=A + 2)])
 def test_plan(bad):
     a = dict(ids=A, n=4, e=8, order=A, off=A) | bad
