@@ -265,8 +265,10 @@ int qs_matmul_experts_workspace(int ggml_type, int n_experts, int64_t n, int64_t
 
 /*
  * Fault word of `device`: bit 0 is set when a quantize kernel gave up waiting for one of its
- * own bulk copies (every wait in the kernels is bounded; on that path the kernel records
- * the fault and returns instead of hanging the GPU). Synchronous; clears the word.
+ * own bulk copies, or a product of many rows for one of its own copies or matrix products
+ * (every wait in the kernels is bounded; on that path the kernel records the fault and returns instead
+ * of hanging the GPU; a product's results that it could not finish are NaN). The call that launched
+ * the kernel has returned QS_OK by then. Synchronous; clears the word.
  * No counterpart in the reference (its kernels have no waits).
  */
 int qs_device_fault(int device, int* bits);

@@ -41,7 +41,7 @@
 // which the sums released NB accumulators ago. With GROUP stages to an accumulator the oldest scale that is
 // still to be read is at most NS + (NB - 1) GROUP stages old (16 for tiles of 128 with GROUP = 4, else 10 at
 // most), less than the ring's length. Every wait is bounded: one that runs out records bit 0 of the fault
-// word and its role leaves.
+// word and its role leaves; the roles behind it run out in turn, and the sums store a tile of NaN.
 // Measured: 2048 slots of Q4_K 14336 x 4096 to bfloat16 338 us with xpack_kernel (11 us), 711 TFLOP/s, 43 % of the
 // measured bf16 rate; 4096 slots of 4096 x 4096 205 us; 1024 to float32 (LO) 108 us. Without any unpacking or
 // copying the same loop takes 247 us: a stage moves 105 KB through shared memory (operands read by
@@ -582,6 +582,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_kernel(MmArgs a, const uint8
                     b_ph ^= 1;
                 }
             }
+        }
+        if (!ok) {  // no sums: the result must not pass for one
+#pragma unroll
+            for (int i = 0; i < HALF / 2; i++) acc[i] = f2_splat(NAN);
         }
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         asm volatile("bar.sync 1, 288;" ::: "memory");

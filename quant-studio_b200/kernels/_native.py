@@ -130,6 +130,15 @@ def quantize(ggml_type: int, x: torch.Tensor, qw: torch.Tensor | None) -> torch.
     return quantize_into(ggml_type, x, qw, out)
 
 
+def device_fault(device: int = 0) -> int:
+    """Fault word of a device, which is cleared: bit 0 is set when a kernel gave up one of its bounded waits
+    (quantizing 32-value blocks, or a product of many rows, whose unfinished results are NaN); 0 after every
+    normal run. Waits for the device's work."""
+    bits = ctypes.c_int()
+    check(lib().qs_device_fault(int(device), ctypes.byref(bits)))
+    return bits.value
+
+
 def _blocks_arg(blocks: torch.Tensor, ggml_type: int) -> tuple[int, int]:
     """(n_rows, k) of a (n_rows, row_bytes) uint8 block tensor (row stride may exceed row_bytes)."""
     if blocks.device.type != "cuda":

@@ -5,7 +5,8 @@ The next step after quantizing: a layer whose weights stay packed. `rms_norm_q8`
 8-bit activations, `route` and `expert_plan` choose and group the experts, `matmul` and
 `matmul_experts` multiply. Everything runs on the current stream of the operands' device;
 outputs and workspaces are new tensors, so calls may be captured into a CUDA graph (after a
-first call on the device outside of a capture, which prepares it).
+first call on the device outside of a capture, which prepares it). A kernel whose bounded waits run
+out leaves NaN and sets the word that `_native.device_fault` reads.
 """
 
 from __future__ import annotations
