@@ -16,7 +16,6 @@ import functools
 from dataclasses import dataclass
 
 import torch
-from torch._C import _cuda_getCurrentRawStream as _stream  # handle of a device's current stream
 
 from ._native import QS_EINVAL, SRC_IDS, QsError, block_info, check, lib
 
@@ -24,6 +23,10 @@ Q8_0 = 8
 _SCORES = {"softmax": 0, "sigmoid": 1}
 _GROUP_SCORES = {"max": 0, "top2": 1}
 
+
+def _stream(index: int) -> int:
+    """Handle of a device's current stream (looked up per call: a torch built without CUDA has no such function)."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _bad(msg: str) -> None:
