@@ -147,3 +147,44 @@ def test_float32_results(qtype, kind, rows):
     size = y if kind == "normal" else terms(x, wq, qtype)
     err = np.linalg.norm(got - y) / np.linalg.norm(size)
     assert err <= 2.0 ** -20, f"{err:.3g}"
+
+
+@pytest.mark.parametrize("qtype", ref.TYPES)
+@pytest.mark.parametrize("rows", [1, 9, 100])
+def test_float16_results(qtype, rows):
+    """float16's own rounding: its half steps lie 8 times closer than bfloat16's, 2.1e-4 in the 2-norm. 2^-20 of
+    float32 sums (test_float32_results) beside it are sqrt(2.1e-4^2 + 9.5e-7^2), 1.00001 of it."""
+    rng = np.random.default_rng(rows)
+    wq, xq = centred(qtype, N, K, rng), activations("normal", rows, K, rng)
+    y = ref.decode64(xq, "q8_0") @ ref.decode64(wq, qtype).T
+    got = matmul(wq, qtype, xq, torch.float16)
+    # values below 2^-14 round to steps of 2^-24
+    alone = np.linalg.norm(y.astype(np.float16).astype(np.float64) - y)
+    assert np.linalg.norm(got - y) <= 1.01 * alone
+
+
+@pytest.mark.parametrize("qtype", ["q4_k", "q2_k", "q5_1", "q6_k", "q4_0"])
+@pytest.mark.parametrize("kind", ["normal", "one sign"])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("tokens", [2, 60, 400])
+def test_experts(qtype, kind, dtype, tokens):
+    """The same for the products of experts, for all three kernels (averages of 1, 30 and 200 slots)."""
+    rng = np.random.default_rng(tokens)
+    e, n, k = 4, 67, 2048
+    wq = np.stack([centred(qtype, n, k, rng) for _ in range(e)])
+    xq = activations(kind, tokens, k, rng)
+    ids = rng.integers(0, e, (tokens, 2)).astype(np.int32)
+    plan = ops.expert_plan(torch.from_numpy(ids).cuda(), e)
+    got = ops.matmul_experts(torch.from_numpy(wq).cuda(), int(ref.GTYPE[qtype]), torch.from_numpy(xq).cuda(), plan,
+                             out_dtype=getattr(torch, dtype)).double().cpu().numpy()
+    x = ref.decode64(xq, "q8_0")
+    y, size = np.zeros(got.shape), np.zeros(got.shape)
+    for i in range(e):
+        t, j = np.nonzero(ids == i)
+        y[t, j] = x[t] @ ref.decode64(wq[i], qtype).T
+        size[t, j] = np.abs(y[t, j]) if kind == "normal" else terms(x[t], wq[i], qtype)
+    err = np.linalg.norm(got - y)
+    if dtype == "float32":
+        assert err <= 2.0 ** -20 * np.linalg.norm(size)
+    else:
+        assert err <= 1.03 * np.linalg.norm(bf16(y) - y)

@@ -1,15 +1,18 @@
 """Calls of the operators on packed blocks at the edges of what they allow, on the GPU."""
 
+import subprocess
+import sys
 from fractions import Fraction
 from math import floor
+from pathlib import Path
 
 import numpy as np
 import pytest
 import torch
 
 import ops_reference as ref
-from kernels import ops
-from test_gpu_ops import check_product, cuda, experts_want
+from kernels import _native, ops
+from test_gpu_ops import check_product, check_route, cuda, experts_want
 
 pytestmark = pytest.mark.gpu
 
@@ -70,3 +73,74 @@ def test_norm_next_to_borders(scale):
         x, wt = (x * scale).astype(np.float32), wt.astype(np.float32)
         _, q = ref.split_q8(ops.rms_norm_q8(cuda(x), cuda(wt), 1e-6).cpu().numpy())
         assert q[0, 0, 0] == 127 and q[0, 0, 1] == -level, (t0, w0, t, w)
+
+
+@pytest.mark.parametrize("k", [32, 512, 8224, 20480])
+@pytest.mark.parametrize("off,gap", [(0, 0), (1, 0), (2, 6), (16, 48), (3, 5)])
+def test_norm_into_any_address(k, off, gap):
+    """Blocks at any address and row distance; bytes before, between and behind the rows stay."""
+    n, row = 5, k // 32 * 34
+    g = torch.Generator(device="cuda").manual_seed(k)
+    x, w = torch.randn((n, k), device="cuda", generator=g), torch.rand(k, device="cuda", generator=g) + 0.5
+    want = ops.rms_norm_q8(x, w)
+    buf = torch.full((off + n * (row + gap) + 64,), 171, dtype=torch.uint8, device="cuda")
+    _native.check(_native.lib().qs_rms_norm_q8(x.data_ptr(), 0, k, None, 0, None, 0, w.data_ptr(), 1e-6, n, k, buf.data_ptr() + off, row + gap,
+                                               torch.cuda.current_stream().cuda_stream))
+    rows = buf[off:off + n * (row + gap)].reshape(n, row + gap)
+    assert torch.equal(rows[:, :row], want)
+    assert (rows[:, row:] == 171).all() and (buf[:off] == 171).all() and (buf[off + n * (row + gap):] == 171).all()
+
+
+CAPTURED = """
+import sys
+sys.path[:0] = [sys.argv[1], sys.argv[2]]
+import torch
+import test_gpu_ops as t
+from kernels import _native, ops
+_native.check(_native.lib().qs_init(0))
+a = t.layer_inputs(int(sys.argv[3]), 1) if sys.argv[4] == "layer" else None
+g = torch.cuda.CUDAGraph()
+if a is not None:
+    with torch.cuda.graph(g):
+        got = t.layer(*a)
+    want = lambda: t.layer(*a)
+else:
+    rows = int(sys.argv[3])
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    def blocks(n, nb):
+        b = torch.randint(0, 256, (n, 4, nb), device="cuda", generator=gen, dtype=torch.uint8)
+        b[..., 1] = 0x1C
+        b[..., -1] = 0x1C
+        return b.reshape(n, 4 * nb)
+    w, x = blocks(300, 66), torch.randint(0, 256, (rows, 32, 34), device="cuda", generator=gen, dtype=torch.uint8)
+    x[..., 1] = 0x1C
+    x = x.reshape(rows, -1)
+    with torch.cuda.graph(g):
+        got = ops.matmul(w, 16, x, out_dtype=torch.bfloat16),
+    want = lambda: (ops.matmul(w, 16, x, out_dtype=torch.bfloat16),)
+g.replay()
+torch.cuda.synchronize()
+got = [v.clone() for v in got]
+assert all(torch.equal(p, q) and torch.isfinite(p.float()).all() for p, q in zip(got, want()))
+"""
+
+
+@pytest.mark.parametrize("rows,what", [(1, "layer"), (40, "layer"), (3, "matmul"), (20, "matmul"), (100, "matmul"), (300, "matmul")])
+def test_first_call_of_a_kernel_is_captured(rows, what):
+    """qs_init is all that a capture needs: no kernel of the calls has run in the process."""
+    here = Path(__file__).resolve().parent
+    r = subprocess.run([sys.executable, "-c", CAPTURED, str(here), str(here.parent / "quant-studio_b200"), str(rows), what], capture_output=True,
+                       text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+def test_route_biases_whose_sums_leave_float32(sign):
+    """Sums of two biases beyond float32's range still order the groups."""
+    rng = np.random.default_rng(9)
+    z = rng.standard_normal((40, 8)).astype(np.float32)
+    bias = np.array([2.0e38, 2.1e38, 3.0e38, 3.3e38, 1.8e38, 1.9e38, 2.5e38, 2.6e38], np.float32) * sign
+    for score in ("softmax", "sigmoid"):
+        for kept in (1, 2):
+            check_route(cuda(z), top_k=2, score=score, bias=bias, n_groups=4, groups_kept=kept, group_score="top2")
+            check_route(cuda(z), top_k=2, score=score, bias=bias, n_groups=4, groups_kept=kept)
