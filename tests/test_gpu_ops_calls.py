@@ -144,3 +144,59 @@ def test_route_biases_whose_sums_leave_float32(sign):
         for kept in (1, 2):
             check_route(cuda(z), top_k=2, score=score, bias=bias, n_groups=4, groups_kept=kept, group_score="top2")
             check_route(cuda(z), top_k=2, score=score, bias=bias, n_groups=4, groups_kept=kept)
+
+
+def sampled(got, xq, wq, qtype, rows, cols, out="float32"):
+    """Check of some rows and columns of a large product (blocks on the GPU)."""
+    r, c = torch.tensor(rows, device="cuda"), torch.tensor(cols, device="cuda")
+    check_product(got[r][:, c], *ref.product(xq[r].cpu().numpy(), wq[c].cpu().numpy(), qtype, out))
+
+
+def q8_rows(n, k, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    b = torch.randint(0, 256, (n, k // 32, 34), device="cuda", generator=g, dtype=torch.uint8)
+    b[..., 1] = 0x1C  # scales of 2^-8 .. 2^-7
+    return b.reshape(n, -1)
+
+
+def test_results_beyond_32_bits():
+    """More than 2^31 results."""
+    rows, n, k = 140_000, 16_400, 256
+    x, w = q8_rows(rows, k, 1), q8_rows(n, k, 2)
+    got = ops.matmul(w, 8, x, out_dtype=torch.bfloat16)
+    assert got.numel() > 1 << 31
+    sampled(got, x, w, "q8_0", [0, 1, 65_535, 130_943, 130_944, 139_998, 139_999], [0, 127, 128, 8191, 16_383, 16_384, 16_399], "bfloat16")
+
+
+@pytest.mark.parametrize("rows", [1, 4, 40, 100])
+def test_weights_beyond_32_bits(rows):
+    """More than 2^32 bytes of weights."""
+    n, k = 500_001, 8192
+    x, w = q8_rows(rows, k, 3), q8_rows(n, k, 4)
+    assert w.numel() > 1 << 32
+    sampled(ops.matmul(w, 8, x), x, w, "q8_0", [0, rows - 1], [0, 1, 246_723, 246_724, 493_447, 493_448, 499_999, 500_000])
+
+
+def test_norm_and_route_beyond_32_bits():
+    n, k = 270_000, 8192
+    x = torch.randn((n, 64), device="cuda", dtype=torch.bfloat16).repeat(1, k // 64)
+    w = torch.rand(k, device="cuda") + 0.5
+    got = ops.rms_norm_q8(x, w)
+    at = torch.tensor([0, 1, 131_071, 262_143, 262_144, 262_145, n - 1], device="cuda")
+    assert torch.equal(got[at], ops.rms_norm_q8(x[at], w))
+    z = x.reshape(n * 64, 128)
+    at = torch.tensor([0, 1, (1 << 24) - 1, 1 << 24, (1 << 24) + 1, n * 64 - 1], device="cuda")
+    ids, ws = ops.route(z, 8)
+    one, wone = ops.route(z[at], 8)
+    assert torch.equal(ids[at], one) and torch.equal(ws[at], wone)
+
+
+@pytest.mark.parametrize("qtype", ["q4_k", "q8_0", "q2_k"])
+@pytest.mark.parametrize("rows", [1, 3, 40, 100])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_very_long_rows(qtype, rows, dtype):
+    rng = np.random.default_rng(rows)
+    n, k = 131, 131_072
+    w, x = ref.random_blocks(qtype, (n,), k, rng), ref.random_blocks("q8_0", (rows,), k, rng)
+    got = ops.matmul(cuda(w), int(ref.GTYPE[qtype]), cuda(x), out_dtype=getattr(torch, dtype))
+    check_product(got, *ref.product(x, w, qtype, dtype))
