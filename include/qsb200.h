@@ -229,15 +229,18 @@ int qs_expert_plan(const int32_t* ids, int64_t n_slots, int n_experts, int32_t* 
  * multiplied exactly; scales and sums are float32, rounded once to out_type. For BF16 results of more than
  * 32 rows the activations may be rounded to 11 bits first (at most 2^-11 of a value, 1/8 of the result's own
  * rounding; values below 2^-29 of their row's largest by at most 2^-40 of that), and Q6_K's products of level and
- * sub-scale above 2048 as well. Which kernel runs, and so the last bits of a row's result, depends on the number
- * of rows (per expert, on average), on the type and on n and k; the same call gives the same bits every time.
+ * sub-scale above 2048 as well; F32 and F16 results of many rows hold values to 2^-40 of their row's largest. Which kernel
+ * runs, and so the last bits of a row's result, depends on the number of rows (per expert, on average), on the
+ * type and on n and k; the same call gives the same bits every time.
  *   w                     weight row j at w + j * w_row_bytes; w and w_row_bytes multiples of 16
  *                         bytes for Q4_K and Q5_K, 8 for Q5_1 and IQ4_XS, 4 for Q4_1 and Q2_K, else 2
  *   x                     row r at x + r * x_row_bytes, any alignment
  *   out                   F32 / F16 / BF16, row stride in elements; overlaps no input
  *   workspace             16-byte aligned, of at least qs_matmul_workspace bytes (may be NULL if
  *                         that is 0); its contents do not matter before or after. Calls that may
- *                         run at the same time need a workspace each.
+ *                         run at the same time need a workspace each. It holds the activations laid
+ *                         out: 0 for up to 4 rows, 1.1 to 1.4 bytes per value for some more, then 2
+ *                         (F32 and F16 results: 4) for rows in whole tiles of 128 or 256.
  * n_rows <= 2^20 and n_rows * n <= 2^38.
  */
 int qs_matmul(int ggml_type, const void* w, int64_t w_row_bytes, int64_t n, int64_t k, const void* x, int64_t x_row_bytes,
@@ -252,6 +255,8 @@ int qs_matmul_workspace(int ggml_type, int64_t n, int64_t k, int64_t n_rows, int
  *   weights               NULL: out has a row per slot, zeros where the slot has no expert.
  *                         Else n_tokens x top_k float32: out has a row per token, the sum over its
  *                         slots with an expert of weight * product, in slot order.
+ * The workspace counts activations in tiles once per slot, and adds 4 bytes per slot and weight row with
+ * weights given.
  * n_tokens * top_k <= 2^20. Strides, alignment, rounding (more than 32 slots per expert on average) and
  * workspace as qs_matmul; sum: weights given.
  */

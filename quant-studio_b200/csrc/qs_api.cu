@@ -468,8 +468,9 @@ MmPlan mm_plan(int type, int64_t n, int64_t k, int64_t slots, int64_t groups, in
     // The tcgen05 kernel from 65 rows on; with experts from an average of 57, where many of them have over 64
     // and so two tiles of 64 (32 of 2048 x 2048, float32 results, Q6_K: 56 rows each 160 / 176 us, 64 rows 231 /
     // 176 us). For bfloat16 results from 33 rows on with superblocks, whose unpacking it does once for all
-    // rows (64 rows of 4096 x 14336: Q4_K 56 / 44 us, Q6_K 76 / 58 us; Q4_0 46 / 50 us), but not for small
-    // matrices with one scale per 32 values (2048 x 1024: Q4_K 14.1 / 15.9 us, Q6_K 17.8 / 16.3 us).
+    // rows (64 rows of 4096 x 14336: Q4_K 57 / 46 us, Q6_K 77 / 59 us; Q4_0 46 / 50 us), but not for small
+    // matrices with one scale per 32 values (Q4_K 2048 x 1024: 13.8 / 15.4 us, 4096 x 4096: 21.0 / 20.1 us, 8192 x 4096:
+    // 32.8 / 29.2 us; Q6_K 2048 x 1024: 17.7 / 16.5 us).
     const bool early = !lo && find_type(type)->qk == 256 && (experts || two_scales(type) || n * k >= (int64_t)1 << 25);
     const int64_t mid = early ? 32 : experts ? 56 : 64;
     p.kind = (experts ? avg <= 1 : slots <= 4) && holds ? MmPlan::FEW : avg <= mid ? MmPlan::MID : MmPlan::TC;

@@ -1,4 +1,4 @@
-// Shared pieces of the packed products (qs_matmul_few.cu, qs_matmul_tile.cu).
+// Shared pieces of the packed products (qs_matmul_few.cu, qs_matmul_mid.cu, qs_matmul_tc.cuh).
 //
 // y[slot, n] = sum over the 32-value units u of a row of
 //   dx[slot, u] * (dl[n, u] * sum lw * lx  -  ml[n, u] * sum lx)

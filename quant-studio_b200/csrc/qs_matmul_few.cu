@@ -7,9 +7,10 @@
 // shared memory once per CTA. A warp's (rows, pair) steps form one sequence, loaded PF steps ahead, so
 // that loads are in flight across row ends too. The CTAs run in one wave and take rows in turn.
 //
-// Measured for one slot: Q4_K 14336 x 4096 (33 MB) 13.0 us, 2.6 TB/s (15.0 us with one run of rows per warp, whose
-// last warps idle); Q4_K / Q4_0 / Q8_0 4096 x 4096 6.5 / 6.7 / 6.8 us, of which about 3 us are launch, staging and first loads. Bound: 280 instructions per pair step of a
-// warp. With more than a few slots the dot products (half rate on this GPU) take
+// Measured for one slot: Q4_K 14336 x 4096 (33 MB) 13.4 us, 2.5 TB/s (15.0 us with one run of rows per warp, whose
+// last warps idle); Q4_K / Q4_0 / Q8_0 4096 x 4096 6.5 / 6.7 / 6.8 us, of which about 3 us are launch, staging and first loads. Neither memory nor
+// the issue slots are full: 280 instructions per pair step of a warp are 60 % of the slots, and 24 warps per SM (79
+// registers) wait for their loads and for one another's results in between. With more than a few slots the dot products (half rate on this GPU) take
 // over: 4 slots 12 us, and from 5 on the tensor cores' kernel is faster.
 #include <algorithm>
 

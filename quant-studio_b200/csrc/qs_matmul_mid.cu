@@ -14,11 +14,12 @@
 // tiles is split over the CTAs of a cluster, which add their tiles through distributed shared memory in
 // rank order.
 //
-// Measured (with pack_kernel, 3 us): Q4_0 4096 x 4096 10.7 us for 5 slots, 19 us for 64; Q6_K 4096 x 14336 34 us
+// Measured (with pack_kernel, 3 us): Q4_0 4096 x 4096 10.7 us for 5 slots, 19 us for 64; Q6_K 4096 x 14336 35 us
 // for 7. Of the 15 us of a CTA with 64 slots and 16 units of Q4_0, set-up is 1.5 us, staging 1.5 us, unpacking
 // 2 us, products 5 us (the float operations, 12 cycles per 16 x 8 product), joining the cluster's tiles 3 us;
-// fewer CTAs per cluster, or one per SM, are slower (24 against 21 us). Q6_K's unaligned bytes make
-// shared memory the bound (66 % of its cycles); pieces of 8 bytes, which halve the bank conflicts, cost more
+// fewer CTAs per cluster, or one per SM, are slower (24 against 21 us). For Q6_K
+// shared memory is what is busiest (66 % of its cycles, 37 % of them conflicts of the unpacking's words at unaligned
+// addresses), the issue slots are at 49 % with 16 warps per SM; pieces of 8 bytes, which halve the bank conflicts, cost more
 // copies than they save (38 us), and 16-byte loads without conflicts more selects (36 us).
 #include <cooperative_groups.h>
 

@@ -42,10 +42,11 @@
 // still to be read is at most NS + (NB - 1) GROUP stages old (16 for tiles of 128 with GROUP = 4, else 10 at
 // most), less than the ring's length. Every wait is bounded: one that runs out records bit 0 of the fault
 // word and its role leaves; the roles behind it run out in turn, and the sums store a tile of NaN.
-// Measured: 2048 slots of Q4_K 14336 x 4096 to bfloat16 338 us with xpack_kernel (11 us), 711 TFLOP/s, 43 % of the
-// measured bf16 rate; 4096 slots of 4096 x 4096 205 us; 1024 to float32 (LO) 108 us. Without any unpacking or
-// copying the same loop takes 247 us: a stage moves 105 KB through shared memory (operands read by
-// the matrix unit, unpacked and copied data), 820 cycles at 128 bytes each, against 512 of products. Tiles of
+// Measured: 2048 slots of Q4_K 14336 x 4096 to bfloat16 344 us with xpack_kernel (11 us), 700 TFLOP/s, 42 % of the
+// measured bf16 rate (338 us with minima of 11 bits); 4096 slots of 4096 x 4096 208 us; 1024 to float32 (LO) 99 us.
+// The matrix unit is active for 43 % of the time. Without any unpacking or copying the loop took 247 us: a stage
+// moves 105 KB through shared memory (operands read by the matrix unit, unpacked and copied data), 820 cycles at
+// 128 bytes each, against 512 of products. Tiles of
 // 256 columns halve what a column costs in unpacking. Pairs of CTAs that hold half of the columns' operand
 // each (cta_group::2) move 74 KB per stage, but took 452 us: every stage then waits for arrivals from
 // the other CTA.

@@ -5,7 +5,8 @@ The next step after quantizing: a layer whose weights stay packed. `rms_norm_q8`
 8-bit activations, `route` and `expert_plan` choose and group the experts, `matmul` and
 `matmul_experts` multiply. Everything runs on the current stream of the operands' device;
 outputs and workspaces are new tensors, so calls may be captured into a CUDA graph (after a
-first call on the device outside of a capture, which prepares it). A kernel whose bounded waits run
+first call on the device outside of a capture, which prepares it). Nothing here is differentiable: outputs
+are cut from the graph, also where an input requires a gradient. A kernel whose bounded waits run
 out leaves NaN and sets the word that `_native.device_fault` reads.
 """
 
@@ -208,7 +209,8 @@ def matmul(blocks: torch.Tensor, ggml_type: int, x_q8: torch.Tensor, out_dtype: 
     the decoded activations times the decoded weights transposed. Levels are multiplied exactly, scales
     and sums are float32, rounded once to out_dtype. For bfloat16 results of more than 32 rows the activations
     may be rounded to 11 bits first (at most 2^-11 of a value, 1/8 of the result's own rounding), and Q6_K's
-    products of level and sub-scale above 2048 as well. The last bits of a row's result depend on the number of
+    products of level and sub-scale above 2048 as well; float32 and float16 results of many rows hold values to 2^-40
+    of their row's largest. The last bits of a row's result depend on the number of
     rows beside it (matmul_experts: per expert, on average), which decides the kernel; the same call gives the same
     bits every time. Row strides may exceed the rows; weight rows must start on multiples of 16 bytes for
     Q4_K / Q5_K, 8 for Q5_1 / IQ4_XS, 4 for Q4_1 / Q2_K, 2 for the others.
@@ -229,7 +231,8 @@ def matmul_experts(blocks: torch.Tensor, ggml_type: int, x_q8: torch.Tensor, pla
 
     x_q8: one Q8_0 row per token, or per slot (token * top_k + j). Without weights: (tokens, top_k, n),
     zeros where a slot has no expert. With weights (tokens, top_k) float32: (tokens, n), the sum of
-    weight * product over a token's slots that have an expert. Otherwise as matmul.
+    weight * product over a token's slots that have an expert. Otherwise as matmul; long batches take a workspace
+    of 2 bytes (float32 and float16 results: 4) per slot and activation, and 4 per slot and output with weights.
     """
     dev, k = _packed_args(blocks, ggml_type, x_q8, 3, out_dtype)
     experts, n, _ = blocks.shape
