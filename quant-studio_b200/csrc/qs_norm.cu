@@ -232,7 +232,8 @@ __global__ void __launch_bounds__(1024) norm_kernel(NormArgs a) {
         const float ds = __fmul_rn(mh, r127f);
         uint16_t d = f16_bits(ds);
         const bool normal = mh > 1e-25f && mh < 1e37f;  // products and their remainders are normal numbers
-        const bool sure = off < SURE && f16_bits(__fmul_rn(ds, 1.0f - NEAR)) == f16_bits(__fmul_rn(ds, 1.0f + NEAR));
+        // (r / 127 below the normal range, in rows of values beyond 6e35, has few bits)
+        const bool sure = off < SURE && r127f >= 1.1754944e-38f && f16_bits(__fmul_rn(ds, 1.0f - NEAR)) == f16_bits(__fmul_rn(ds, 1.0f + NEAR));
         if (!__all_sync(0xffffffffu, (normal && sure) || !live || bad)) {
             if (__all_sync(0xffffffffu, normal || !live || bad)) {
                 // the block's exact largest product: the largest remainder among the largest products

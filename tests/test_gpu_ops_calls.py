@@ -12,7 +12,7 @@ import torch
 
 import ops_reference as ref
 from kernels import _native, ops
-from test_gpu_ops import check_product, check_route, cuda, experts_want
+from test_gpu_ops import check_norm, check_product, check_route, cuda, experts_want
 
 pytestmark = pytest.mark.gpu
 
@@ -32,9 +32,12 @@ def test_experts_of_one_row(qtype, tokens, padded):
         wide = torch.full((e, 2, w.shape[2] + 16), 255, dtype=torch.uint8, device="cuda")
         wide[:, :1, :w.shape[2]] = wc
         wc = wide[:, :1, :w.shape[2]]
+    p = ops.expert_plan(cuda(ids), e)
     if wc.stride(0) % {"q4_k": 16, "q5_k": 16, "q5_1": 8, "iq4_xs": 8, "q4_1": 4, "q2_k": 4}.get(qtype, 2):
-        pytest.skip("this stride is refused for this format")
-    got = ops.matmul_experts(wc, int(ref.GTYPE[qtype]), cuda(x), ops.expert_plan(cuda(ids), e))
+        with pytest.raises(_native.QsError):
+            ops.matmul_experts(wc, int(ref.GTYPE[qtype]), cuda(x), p)
+        return
+    got = ops.matmul_experts(wc, int(ref.GTYPE[qtype]), cuda(x), p)
     check_product(got, *experts_want(x, w, qtype, ids, None, False))
 
 
@@ -73,6 +76,17 @@ def test_norm_next_to_borders(scale):
         x, wt = (x * scale).astype(np.float32), wt.astype(np.float32)
         _, q = ref.split_q8(ops.rms_norm_q8(cuda(x), cuda(wt), 1e-6).cpu().numpy())
         assert q[0, 0, 0] == 127 and q[0, 0, 1] == -level, (t0, w0, t, w)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("scale", [3e35, 2e36, 1e37])
+def test_norm_of_rows_whose_factor_is_subnormal(dtype, scale):
+    """1 / (127 rms) below float32's normal range, with products inside it."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = (torch.randn((64, 1024), device="cuda", generator=g) * scale).to(getattr(torch, dtype))
+    w = 0.01 + 0.1 * torch.rand(1024, device="cuda", generator=g)
+    assert torch.isfinite(x).all()
+    check_norm(x, w, 1e-6, None, ops.rms_norm_q8(x, w, 1e-6))
 
 
 @pytest.mark.parametrize("k", [32, 512, 8224, 20480])
