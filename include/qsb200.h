@@ -228,10 +228,10 @@ int qs_expert_plan(const int32_t* ids, int64_t n_slots, int n_experts, int32_t* 
  * n_rows rows of Q8_0 blocks (qs_rms_norm_q8, or qs_quantize with QS_TYPE_Q8_0). Levels are
  * multiplied exactly; scales and sums are float32, rounded once to out_type. For BF16 results of more than
  * 32 rows the activations may be rounded to 11 bits first (at most 2^-11 of a value, 1/8 of the result's own
- * rounding; values below 2^-29 of their row's largest by at most 2^-40 of that), and Q6_K's products of level and
- * sub-scale above 2048 as well; F32 and F16 results of many rows hold values to 2^-40 of their row's largest. Which kernel
- * runs, and so the last bits of a row's result, depends on the number of rows (per expert, on average), on the
- * type and on n and k; the same call gives the same bits every time.
+ * rounding), and Q6_K's products of level and sub-scale above 2048 as well. Of many rows (any result) activations
+ * far below their row's largest are held to 2^-39 of 128 times the row's largest scale. Which kernel runs, and so
+ * the last bits of a row's result, depends on the number of rows (per expert, on average), on the type and on n
+ * and k; the same call gives the same bits every time.
  *   w                     weight row j at w + j * w_row_bytes; w and w_row_bytes multiples of 16
  *                         bytes for Q4_K and Q5_K, 8 for Q5_1 and IQ4_XS, 4 for Q4_1 and Q2_K, else 2
  *   x                     row r at x + r * x_row_bytes, any alignment

@@ -6,11 +6,12 @@
 //   acc[n, t] += d[n, superblock] * D[n, t]
 // in float32 registers. Formats with a scale per 32 values are scaled and added every 32. Q6_K's
 // level * sub-scale (up to 4096) is float16 hi + lo, exact together.
-// Activations: scale * level has 19 bits; times a power of two per row (so that the row's largest lies
-// below 2^15) it is float16 hi + lo, exact together down to 2^-39 of the row's largest. LO: the
+// Activations: scale * level has 19 bits; times a power of two per row (that takes the largest scale to 2^7 ..
+// 2^8, values below 2^15) it is float16 hi + lo, exact together but for 2^-25, which is at most 2^-39 of 128 times the
+// row's largest scale. LO: the
 // products use both parts (Q6_K: hi hi, hi lo, lo hi), for float32 and float16 results. For
 // bfloat16 results hi alone is multiplied: that rounds the activations to 11 bits, by at most 2^-11 of a value
-// (2^-40 of the row's largest for values below 2^-29 of it), 1/8 of the result's own rounding where the terms
+// (or those 2^-25), 1/8 of the result's own rounding where the terms
 // are of both signs (in the 2-norm 2.1e-4 and 1.66e-3). Q6_K's level * sub-scale above 2048 (5 % of the weights with
 // sub-scales of 40 to 127) is rounded to 11 bits there as well.
 // Minima: - ml[n, unit] * (sum of the unit's activations)[t, unit] is a product of its own, with K / 32 (K / 16

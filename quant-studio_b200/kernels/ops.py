@@ -209,8 +209,8 @@ def matmul(blocks: torch.Tensor, ggml_type: int, x_q8: torch.Tensor, out_dtype: 
     the decoded activations times the decoded weights transposed. Levels are multiplied exactly, scales
     and sums are float32, rounded once to out_dtype. For bfloat16 results of more than 32 rows the activations
     may be rounded to 11 bits first (at most 2^-11 of a value, 1/8 of the result's own rounding), and Q6_K's
-    products of level and sub-scale above 2048 as well; float32 and float16 results of many rows hold values to 2^-40
-    of their row's largest. The last bits of a row's result depend on the number of
+    products of level and sub-scale above 2048 as well. Of many rows activations far below their row's largest are
+    held to 2^-39 of 128 times the row's largest scale. The last bits of a row's result depend on the number of
     rows beside it (matmul_experts: per expert, on average), which decides the kernel; the same call gives the same
     bits every time. Row strides may exceed the rows; weight rows must start on multiples of 16 bytes for
     Q4_K / Q5_K, 8 for Q5_1 / IQ4_XS, 4 for Q4_1 / Q2_K, 2 for the others.

@@ -149,6 +149,26 @@ def test_float32_results(qtype, kind, rows):
     assert err <= 2.0 ** -20, f"{err:.3g}"
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("ratio", [10, 16, 22])
+@pytest.mark.parametrize("rows", [9, 100, 130])
+def test_one_large_block_that_no_weight_meets(dtype, ratio, rows):
+    """Values 2^-ratio of their row's largest, which alone make the result: held to 2^-39 of 128 times the row's
+    largest scale (a level of 1 lies at 2^-7 of its block's largest)."""
+    rng = np.random.default_rng(ratio)
+    wq, xq = centred("q8_0", N, 1024, rng), activations("normal", rows, 1024, rng)
+    x = xq.reshape(rows, -1, 34)
+    x[:, 5, :2], d = halves(np.full(rows, 16.0)), x[..., :2].copy().view(np.float16)[..., 0]
+    d = d.astype(np.float64) / d.astype(np.float64).max() * 16 * 2.0 ** -ratio
+    keep = np.arange(32) != 5
+    x[:, keep, :2] = halves(d[:, keep])
+    wq.reshape(N, -1, 34)[:, 5, :2] = 0
+    got = matmul(wq, "q8_0", xq, getattr(torch, dtype))
+    y, bound = ref.product(xq, wq, "q8_0", dtype)
+    bound = bound + 2.0 ** -39 * 128 * 16 * np.abs(ref.decode64(wq, "q8_0")).sum(1)
+    assert (np.abs(got - y) <= bound + ref.rounding(np.abs(y) + bound, dtype)).all()
+
+
 @pytest.mark.parametrize("qtype", ref.TYPES)
 @pytest.mark.parametrize("rows", [1, 9, 100])
 def test_float16_results(qtype, rows):
